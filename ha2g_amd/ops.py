@@ -9,7 +9,7 @@ import torch
 
 from ._lib import check, lib
 
-ACT_NONE, ACT_RELU, ACT_LEAKY, ACT_SIGMOID = 0, 1, 2, 3
+ACT_NONE, ACT_RELU, ACT_LEAKY, ACT_SIGMOID, ACT_SILU = 0, 1, 2, 3, 4      # ACT_SILU: the gates of block_tail only
 (OP_ADD, OP_MUL, OP_ADD_RELU, OP_RELU_BWD, OP_LEAKY_BWD, OP_SIGMOID_BWD, OP_ELU, OP_ELU_BWD, OP_REPARAM,
  OP_REPARAM_BWD_LOGVAR, OP_AXPBY, OP_LEAKY, OP_RELU, OP_SCALE, OP_MUL_SCALAR, OP_SIGMOID, OP_SIGMOID_BWD_PRE, OP_RSQRT_EPS, OP_LEAKY_A) = range(19)
 
@@ -1900,3 +1900,242 @@ def merge_rows(ids, rows, map_scratch):
     vals = torch.zeros(n + 1, C, dtype=torch.float32, device=dev)
     check(lib.ha2g_embedding_bwd_f32(remap.data_ptr(), rows.contiguous().data_ptr(), vals.data_ptr(), n, C, 0, workspace(dev).data_ptr(), _stream()))
     return uniq, count, vals
+
+
+# ------------------------------------------------------------------------------------------------
+# linear attention with a decay per head (csrc/linattn.hip)
+# ------------------------------------------------------------------------------------------------
+
+def _need(cond, msg, *args):
+    if not cond:
+        raise ValueError('ha2g_amd: ' + msg % args)
+
+
+def _on(t):
+    """launches go to the device their tensors live on, also where another one is current"""
+    return _null() if t.device.index == _cur_device() else torch.cuda.device(t.device)
+
+
+def _inner1(x):
+    return x if x.shape[-1] == 1 or x.stride(-1) == 1 else x.contiguous()
+
+
+def _la_check(what, q, k, v, log_decay, state, nd):
+    for n, x in (('q', q), ('k', k), ('v', v)):
+        _need(x.dim() == nd and x.dtype in (torch.float32, torch.bfloat16) and x.dtype == q.dtype and x.device == q.device,
+              '%s: %s is %s %s: %d dimensions, fp32 or bf16, all alike', what, n, x.dtype, tuple(x.shape), nd)
+    _need(q.shape[:-2] == k.shape[:-2] == v.shape[:-2], '%s: q %s, k %s, v %s', what, tuple(q.shape), tuple(k.shape), tuple(v.shape))
+    H, Dk, Dv = log_decay.numel(), q.shape[-1], v.shape[-1]
+    _need(k.shape[-1] == Dk and 1 <= Dk <= 128 and 1 <= Dv <= 128, '%s: head sizes %d / %d / %d (q and k alike, 1 to 128)', what, Dk, k.shape[-1], Dv)
+    _need(log_decay.dim() == 1 and log_decay.dtype == torch.float32 and log_decay.device == q.device and log_decay.is_contiguous(),
+          '%s: log_decay is one fp32 value per head', what)
+    _need(not log_decay.requires_grad, '%s: the decays are constants (no gradient)', what)
+    _need(H >= 1 and all(x.shape[-2] >= 1 and H % x.shape[-2] == 0 for x in (q, k, v)), '%s: %d / %d / %d heads do not divide %d decays', what, q.shape[-2],
+          k.shape[-2], v.shape[-2], H)
+    if state is not None:
+        _need(state.shape == (q.shape[0], H, Dk, Dv) and state.dtype == torch.float32 and state.device == q.device,
+              '%s: state is fp32 [%d, %d, %d, %d], got %s %s', what, q.shape[0], H, Dk, Dv, state.dtype, tuple(state.shape))
+    _need(q.is_cuda, '%s: GPU tensors (there is no CPU path)', what)
+    return H
+
+
+def _la_strides(*ts):
+    import array
+    return array.array('l', [s for t in ts for s in (t.stride() if t.dim() == 4 else (t.stride(0), 0, t.stride(1)))[:3]])
+
+
+def _la_call(q, k, v, o, log_decay, s_in, s_out, lengths, transposed, o_scale, u_scale, reverse):
+    B, T, H = q.shape[0], q.shape[1], log_decay.numel()
+    q, k, v = _inner1(q), _inner1(k), _inner1(v)
+    check(lib.ha2g_linattn(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), log_decay.data_ptr(), _p(s_in), _p(s_out), _p(lengths),
+                           _la_strides(q, k, v, o), B, T, H, H // q.shape[2], H // k.shape[2], H // v.shape[2], q.shape[3], v.shape[3], int(transposed),
+                           o_scale, u_scale, int(reverse), int(q.dtype == torch.bfloat16), int(o.dtype == torch.bfloat16), _stream()))
+
+
+def _la_grad(like, H, dtype):
+    """gradient buffer of an operand with like.shape[2] heads: per-head sums in fp32 first where several heads read one"""
+    B, T, Hx, D = like.shape
+    return torch.empty(B, T, H, D, dtype=dtype if Hx == H else torch.float32, device=like.device)
+
+
+def _la_share(d, like):
+    B, T, Hx, D = like.shape
+    if d.shape[2] == Hx:
+        return d
+    out = torch.empty(B, T, Hx, D, dtype=like.dtype, device=like.device)
+    check(lib.ha2g_head_sum(d.data_ptr(), out.data_ptr(), B * T, Hx, d.shape[2] // Hx, D, int(out.dtype == torch.bfloat16), _stream()))
+    return out
+
+
+class LinearAttentionFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, log_decay, scale, state, lengths, want_state):
+        B, T, H = q.shape[0], q.shape[1], log_decay.numel()
+        ctx.set_materialize_grads(False)
+        with _on(q):
+            o = torch.empty(B, T, H, v.shape[3], dtype=v.dtype, device=q.device)
+            s = torch.empty(B, H, q.shape[3], v.shape[3], dtype=torch.float32, device=q.device) if want_state else None
+            _la_call(q, k, v, o, log_decay, state, s, lengths, False, scale, 1.0, False)
+        ctx.scale = scale
+        ctx.save_for_backward(q, k, v, log_decay, state, lengths)
+        return o, s
+
+    @staticmethod
+    def backward(ctx, do, ds):
+        q, k, v, g, state, lengths = ctx.saved_tensors
+        H, scale = g.numel(), ctx.scale
+        with _on(q):
+            if do is None:
+                do = torch.zeros(1, 1, 1, v.shape[3], dtype=v.dtype, device=q.device).expand(q.shape[0], q.shape[1], H, -1)
+            if ds is not None:
+                ds = ds.contiguous()
+            dq = dk = dv = dstate = None
+            if ctx.needs_input_grad[0]:
+                dq = _la_grad(q, H, q.dtype)
+                _la_call(do, v, k, dq, g, state, None, lengths, True, scale, 1.0, False)
+                dq = _la_share(dq, q)
+            if ctx.needs_input_grad[1]:
+                dk = _la_grad(k, H, k.dtype)
+                _la_call(v, do, q, dk, g, ds, None, lengths, True, 1.0, scale, True)
+                dk = _la_share(dk, k)
+            if ctx.needs_input_grad[2] or ctx.needs_input_grad[5]:
+                dv = _la_grad(v, H, v.dtype)
+                if ctx.needs_input_grad[5]:
+                    dstate = torch.empty(q.shape[0], H, q.shape[3], v.shape[3], dtype=torch.float32, device=q.device)
+                _la_call(k, q, do, dv, g, ds, dstate, lengths, False, 1.0, scale, True)
+                dv = _la_share(dv, v) if ctx.needs_input_grad[2] else None
+        return dq, dk, dv, None, None, dstate, None, None
+
+
+def linear_attention(q, k, v, log_decay, scale=None, state=None, lengths=None, return_state=False):
+    """Causal linear attention with one decay per head, over whole sequences, differentiable in q, k, v and state:
+        S_t = exp(log_decay) S_{t-1} + k_t v_t^T,   o_t = scale * q_t S_t          (scale: Dk ** -0.5 by default)
+    q [B, T, Hq, Dk], k [B, T, Hk, Dk], v [B, T, Hv, Dv]: fp32 or bf16, any strides with unit inner stride (slices of a fused projection are
+    read in place), Dk and Dv from 1 to 128.  log_decay [H] fp32 <= 0, a constant; Hq, Hk, Hv divide H, head h reads head h // (H // Hx).
+    state [B, H, Dk, Dv] fp32: what stands before the first token (None: zero).  lengths [B] int32 on the device: row b ends after lengths[b]
+    tokens (clipped to 0 .. T); what lies behind is not read, the output and the gradients there are zero.
+    Returns o [B, T, H, Dv] in v's type, with return_state also the state behind each row's last token, fp32."""
+    _la_check('linear_attention', q, k, v, log_decay, state, 4)
+    _need(lengths is None or (lengths.shape == (q.shape[0],) and lengths.dtype == torch.int32 and lengths.device == q.device and lengths.is_contiguous()),
+          'linear_attention: lengths is int32 [%d] on the device of q', q.shape[0])
+    scale = float(q.shape[3] ** -0.5 if scale is None else scale)
+    o, s = LinearAttentionFunction.apply(q, k, v, log_decay, scale, None if state is None else state.contiguous(), lengths, bool(return_state))
+    return (o, s) if return_state else o
+
+
+def linear_attention_step(q, k, v, log_decay, state, scale=None):
+    """One token of linear_attention: q [B, Hq, Dk], k [B, Hk, Dk], v [B, Hv, Dv] -> o [B, H, Dv]; `state` (fp32, contiguous) is updated in place.
+    For generation: no gradient passes through it."""
+    H = _la_check('linear_attention_step', q, k, v, log_decay, state, 3)
+    _need(state is not None and state.is_contiguous(), 'linear_attention_step: needs a contiguous state')
+    _need(not (torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, state))), 'linear_attention_step: no gradient (use linear_attention)')
+    q, k, v = _inner1(q), _inner1(k), _inner1(v)
+    with _on(q):
+        o = torch.empty(q.shape[0], H, v.shape[2], dtype=v.dtype, device=q.device)
+        check(lib.ha2g_linattn_step(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), log_decay.data_ptr(), state.data_ptr(), _la_strides(q, k, v, o),
+                                    q.shape[0], H, H // q.shape[1], H // k.shape[1], H // v.shape[1], q.shape[2], v.shape[2],
+                                    float(q.shape[2] ** -0.5 if scale is None else scale), int(q.dtype == torch.bfloat16), _stream()))
+    torch.autograd.graph.increment_version(state)
+    return o
+
+
+# ------------------------------------------------------------------------------------------------
+# row norms and the fused tail of a block (csrc/rownorm.hip)
+# ------------------------------------------------------------------------------------------------
+
+_NORMS = ('rms', 'layer')
+
+
+class BlockTailFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, res, gate, w, b, s, w2, b2, groups, layer, act, alpha, eps):
+        ctx.set_materialize_grads(False)
+        C = y.shape[-1]
+        c = lambda t: None if t is None else t.contiguous()      # noqa: E731
+        y, res, gate, w, b, s, w2, b2 = (c(t) for t in (y, res, gate, w, b, s, w2, b2))
+        rows = y.numel() // C
+        shared = gate is not None and gate.shape != y.shape
+        outer, inner = (y.shape[0], rows // max(y.shape[0], 1)) if shared else (1, rows)
+        keep = any(ctx.needs_input_grad)
+
+        def stat(n, want=True):
+            return torch.empty(n, dtype=torch.float32, device=y.device) if keep and want else None
+        with _on(y):
+            h = torch.empty_like(y)
+            z = torch.empty_like(y) if w2 is not None else None
+            mu, rs = stat(rows * groups, layer and w is not None), stat(rows * groups, w is not None)
+            mu2, rs2 = stat(rows, layer and w2 is not None), stat(rows, w2 is not None)
+            check(lib.ha2g_block_tail_fwd(y.data_ptr(), _p(res), _p(gate), _p(w), _p(b), _p(s), _p(w2), _p(b2), h.data_ptr(), _p(z), _p(mu), _p(rs),
+                                          _p(mu2), _p(rs2), outer, inner, int(shared), C, groups, int(layer), act, alpha, eps,
+                                          int(y.dtype == torch.bfloat16), _stream()))
+        ctx.shape = outer, inner, shared, C, groups, layer, act, alpha, eps
+        ctx.save_for_backward(y, res, gate, w, b, s, w2, b2, mu, rs, mu2, rs2)
+        return h, z
+
+    @staticmethod
+    def backward(ctx, dh, dz):
+        y, res, gate, w, b, s, w2, b2, mu, rs, mu2, rs2 = ctx.saved_tensors
+        outer, inner, shared, C, groups, layer, act, alpha, eps = ctx.shape
+        need = ctx.needs_input_grad
+        dh, dz = (None if t is None else t.contiguous() for t in (dh, dz))
+        with _on(y):
+            dy = torch.empty_like(y) if need[0] else None
+            dres = torch.empty_like(y) if res is not None and need[1] else None
+            dgate = torch.empty_like(gate) if gate is not None and (need[2] or shared) else None
+            nvec = 2 * (w is not None) + (s is not None) + 2 * (w2 is not None)
+            n = lib.ha2g_block_tail_slices(outer, inner, C)
+            ws = torch.empty(max(1, n * outer * (nvec + int(shared)) * C), dtype=torch.float32, device=y.device)
+            # no rows: the sums over them are zero
+            dp = (torch.empty if y.numel() else torch.zeros)(nvec, C, dtype=torch.float32, device=y.device)
+            if y.numel() == 0 and dgate is not None:
+                dgate.zero_()
+            check(lib.ha2g_block_tail_bwd(y.data_ptr(), _p(res), _p(gate), _p(w), _p(b), _p(s), _p(w2), _p(b2), _p(mu), _p(rs), _p(mu2), _p(rs2),
+                                          _p(dh), _p(dz), _p(dy), _p(dres), _p(dgate), ws.data_ptr(), ws.data_ptr() + 4 * n * outer * nvec * C if shared else 0,
+                                          dp.data_ptr(), n, outer, inner, int(shared), C, groups, int(layer), act, alpha, eps,
+                                          int(y.dtype == torch.bfloat16), _stream()))
+        it = iter(dp)
+        dw, db = (next(it), next(it)) if w is not None else (None, None)
+        dsc = next(it) if s is not None else None
+        dw2, db2 = (next(it), next(it)) if w2 is not None else (None, None)
+        return (dy, dres, dgate if need[2] else None, dw, db if b is not None else None, dsc, dw2, db2 if b2 is not None else None) + (None,) * 5
+
+
+def _norm_check(what, y, groups, kind, vectors):
+    _need(y.dim() >= 1 and y.dtype in (torch.float32, torch.bfloat16) and 1 <= y.shape[-1] <= 16384, '%s: fp32 or bf16 rows of 1 to 16384 values, got %s %s',
+          what, y.dtype, tuple(y.shape))
+    C = y.shape[-1]
+    _need(groups >= 1 and C % groups == 0, '%s: %d values in %d groups', what, C, groups)
+    _need((C // groups) % 4 == 0 or C <= 8192, '%s: rows of more than 8192 values need groups of a multiple of 4', what)
+    _need(kind in _NORMS, '%s: kind %r (one of %s)', what, kind, ', '.join(_NORMS))
+    for n, t in vectors:
+        _need(t is None or (t.shape == (C,) and t.dtype == torch.float32 and t.device == y.device), '%s: %s is fp32 [%d]', what, n, C)
+    _need(y.is_cuda, '%s: GPU tensors (there is no CPU path)', what)
+
+
+def row_norm(x, weight, bias=None, kind='rms', groups=1, eps=1e-5):
+    """The norm in front of a block: x [..., C] (fp32 or bf16) -> norm(x) * weight + bias, normalised over each of `groups` equal parts of a row.
+    kind: 'rms' or 'layer' (the mean is removed).  weight, bias [C] fp32.  C up to 16384 (8192 where C / groups is no multiple of 4)."""
+    _need(weight is not None, 'row_norm: needs a weight')
+    _norm_check('row_norm', x, groups, kind, (('weight', weight), ('bias', bias)))
+    return BlockTailFunction.apply(x, None, None, weight, bias, None, None, None, groups, kind == 'layer', ACT_NONE, 1.0, float(eps))[0]
+
+
+def block_tail(y, residual=None, gate=None, weight=None, bias=None, scale=None, alpha=1.0, kind='rms', groups=1, gate_act=ACT_SILU, next_weight=None,
+               next_bias=None, eps=1e-5):
+    """What follows a block, in one pass over its output y [..., C] (fp32 or bf16):
+        u = (norm(y) * weight + bias) * gate_act(gate);   h = alpha * residual + scale * u;   z = norm(h) * next_weight + next_bias
+    Every part is optional: weight None = no norm in front of the gate, next_weight None = no z.  The first norm runs over `groups` equal parts of a
+    row (heads), the second over the whole row.  gate: y's shape, or [B, 1, ..., C] = one row per sequence y[b].  gate_act: ACT_NONE, ACT_SIGMOID or
+    ACT_SILU.  scale [C] fp32 weights the branch, alpha the residual.  z is taken of h before it is rounded to y's type.
+    Returns h, or (h, z) with next_weight."""
+    _norm_check('block_tail', y, groups, kind, (('weight', weight), ('bias', bias), ('scale', scale), ('next_weight', next_weight), ('next_bias', next_bias)))
+    _need(bias is None or weight is not None, 'block_tail: a bias without a weight')
+    _need(next_bias is None or next_weight is not None, 'block_tail: a next_bias without a next_weight')
+    _need(residual is None or (residual.shape == y.shape and residual.dtype == y.dtype and residual.device == y.device), 'block_tail: residual is like y')
+    _need(gate_act in (ACT_NONE, ACT_SIGMOID, ACT_SILU), 'block_tail: gate_act %r', gate_act)
+    if gate is not None:
+        _need(gate.dtype == y.dtype and gate.device == y.device, 'block_tail: gate has the type and device of y')
+        _need(gate.shape == y.shape or (y.dim() >= 2 and gate.shape == (y.shape[0],) + (1,) * (y.dim() - 2) + (y.shape[-1],) and y.shape[0] <= 65535),
+              'block_tail: gate %s for y %s (like y, or one row for each of at most 65535 sequences)', tuple(gate.shape), tuple(y.shape))
+    h, z = BlockTailFunction.apply(y, residual, gate, weight, bias, scale, next_weight, next_bias, groups, kind == 'layer', gate_act, float(alpha), float(eps))
+    return h if next_weight is None else (h, z)

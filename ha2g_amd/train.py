@@ -6,7 +6,7 @@ import torch
 from .hierarchy_net import (Hierarchical_ConvDiscriminator, Hierarchical_PoseGenerator, Hierarchical_WavEncoder,
                             TextEncoderTCN)
 from . import ops
-from .optim import FusedAdam
+from .optim import FusedAdam, FusedAdamW
 from .train_hierarchy import train_iter_hierarchy, train_iter_hierarchy_expressive
 
 
@@ -38,7 +38,7 @@ class HierarchyTrainer:
         from . import ddp
         self.args, self.device = args, device
         if sparse_embeddings is None:
-            sparse_embeddings = ddp.active()
+            sparse_embeddings = ddp.active() and getattr(args, 'optimizer', 'adam') == 'adam'
         self.sparse_embeddings = bool(sparse_embeddings)
         self.expressive = len(pose_dims) == 6        # scripts/train_expressive.py:160-168: six generators 24/30/36/66/96/126
         _, self.discriminator, self.audio_encoder, self.text_encoder, _ = init_model(args, lang_model, speaker_model, pose_dim, device,
@@ -56,6 +56,23 @@ class HierarchyTrainer:
         a = self.args
         lr = float(a.learning_rate)
         sp = (lambda enc: [enc.embedding.weight]) if self.sparse_embeddings else (lambda enc: [])
+        # args.optimizer: 'adam' (the reference's, default), 'adamw' or 'adamw8' = decoupled weight decay (args.weight_decay; vectors are not decayed)
+        # with fp32 or 8-bit moments
+        kind = getattr(a, 'optimizer', 'adam')
+        if kind in ('adamw', 'adamw8'):
+            if self.sparse_embeddings:
+                raise ValueError('ha2g_amd: row-wise embedding updates need args.optimizer = "adam" (sparse_embeddings=False keeps the tables dense)')
+
+            def make(m, lr):
+                ps = list(m.parameters())
+                return FusedAdamW(ps, lr=lr, betas=(0.5, 0.999), weight_decay=float(getattr(a, 'weight_decay', 0.01)),
+                                  no_decay=[p for p in ps if p.dim() < 2], state_bits=8 if kind == 'adamw8' else 32, seed=int(getattr(a, 'random_seed', 0)))
+            self.gen_opts = [make(g, lr) for g in self.gens]
+            self.audio_opt, self.text_opt = make(self.audio_encoder, lr), make(self.text_encoder, lr)
+            self.dis_opt = make(self.discriminator, lr * a.discriminator_lr_weight)
+            return
+        if kind != 'adam':
+            raise ValueError('ha2g_amd: args.optimizer = %r (adam, adamw, adamw8)' % (kind,))
         self.gen_opts = [FusedAdam(g.parameters(), lr=lr, betas=(0.5, 0.999), sparse=sp(g.text_encoder)) for g in self.gens]
         self.audio_opt = FusedAdam(self.audio_encoder.parameters(), lr=lr, betas=(0.5, 0.999))
         self.text_opt = FusedAdam(self.text_encoder.parameters(), lr=lr, betas=(0.5, 0.999), sparse=sp(self.text_encoder))

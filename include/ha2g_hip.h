@@ -572,6 +572,49 @@ long ha2g_logmel_workspace_floats(int B, long n_samples);
 int ha2g_logmel_f32(const float* y, int B, long n_samples, int pad_reflect, const float* tables, int round_f16, float* out,
                     float* ws, void* stream);
 
+/* ---- linear attention with one decay per head (no reference counterpart; stands beside the GRU recurrence of model/hierarchy_net.py:87-88,144) ----
+ *   S_t = e^{log_decay} S_{t-1} + u_scale k_t v_t^T,  o_t = o_scale q_t S_t     per batch row and head, S fp32 [Dk][Dv], 1 <= Dk, Dv <= 128
+ * q, k, v, o: strides = HOST array {batch, token, head} x {q, k, v, o} in elements, inner stride 1; fp32, or bf16 with b16_in (o: b16_out).
+ * Head h of H reads head h / rq of q, h / rk of k, h / rv of v.  s_in / s_out [B][H][Dk][Dv] (s_transposed: [B][H][Dv][Dk]); s_in NULL = zero,
+ * s_out NULL = not wanted.  lengths [B] (device int32, NULL = T): tokens at and behind a row's length are not read, o is zero there.
+ * reverse: from the last token to the first, a step adds, reads and THEN decays.  The backward pass is three calls (all strides of the tensors named):
+ *   dq = (q, k, v) := (do, v, k), s_in := S_0 transposed;  dk = (v, do, q) reverse, s_in := dS_T transposed, u_scale = scale, o_scale = 1;
+ *   dv = (k, q, do) reverse, s_in := dS_T, u_scale = scale, o_scale = 1, s_out = dS_0. */
+int ha2g_linattn(const void* q, const void* k, const void* v, void* o, const float* log_decay, const float* s_in, float* s_out, const int* lengths,
+                 const long* strides, int B, int T, int H, int rq, int rk, int rv, int Dk, int Dv, int s_transposed, float o_scale, float u_scale,
+                 int reverse, int b16_in, int b16_out, void* stream);
+/* one token: q [B][..][Dk] ..., state updated in place; the token strides are not read */
+int ha2g_linattn_step(const void* q, const void* k, const void* v, void* o, const float* log_decay, float* state, const long* strides, int B, int H,
+                      int rq, int rk, int rv, int Dk, int Dv, float o_scale, int b16_io, void* stream);
+/* out [rows][heads][D] = the sum over n consecutive heads of x [rows][heads][n][D] (gradients of shared heads) */
+int ha2g_head_sum(const float* x, void* out, long rows, int heads, int n, int D, int b16_out, void* stream);
+
+/* ---- row norms and the fused tail of a block (no reference counterpart; stands beside BatchNorm and the SE tail of model/ResNetBlocks.py:30-37,81-95) ----
+ *   n = norm(y) w + b in G groups of C / G (layer != 0: mean removed; otherwise RMS), u = n act(gate), h = alpha res + s u, z = norm(h) w2 + b2 over C.
+ * y, res, gate, h, z: rows of C values, fp32 or (b16_io) bf16; parameters [C] fp32; w, b, gate, s, res, w2, b2 may be NULL (w NULL: no norm; w2 NULL:
+ * no z).  rows = outer * inner; gate_shared: one gate row per `inner` rows.  act: 0 none, 3 sigmoid, 4 SiLU.  mu, rs [rows * G], mu2, rs2 [rows]:
+ * kept for the backward pass (NULL = not kept; mu, mu2 only for layer).  C <= 16384; C <= 8192 where C / G % 4 != 0 or an operand is not aligned to 16.
+ * bwd: dh, dz (NULL = zero) -> dy, dres, dgate (NULL = not wanted; with gate_shared required), and dparams = [dw][db][ds][dw2][db2] (those whose
+ * weight is there; db with w, db2 with w2); part = slices * outer * (their number) * C floats, gpart = slices * outer * C (gate_shared), slices =
+ * ha2g_block_tail_slices().  Every sum has a fixed order. */
+int ha2g_block_tail_slices(int outer, long inner, int C);
+int ha2g_block_tail_fwd(const void* y, const void* res, const void* gate, const float* w, const float* b, const float* s, const float* w2, const float* b2,
+                        void* h, void* z, float* mu, float* rs, float* mu2, float* rs2, int outer, long inner, int gate_shared, int C, int G, int layer,
+                        int act, float alpha, float eps, int b16_io, void* stream);
+int ha2g_block_tail_bwd(const void* y, const void* res, const void* gate, const float* w, const float* b, const float* s, const float* w2, const float* b2,
+                        const float* mu, const float* rs, const float* mu2, const float* rs2, const void* dh, const void* dz, void* dy, void* dres,
+                        void* dgate, float* part, float* gpart, float* dparams, int slices, int outer, long inner, int gate_shared, int C, int G,
+                        int layer, int act, float alpha, float eps, int b16_io, void* stream);
+
+/* ---- AdamW over many tensors in one launch (torch.optim.AdamW semantics; the reference sets up Adam, train.py:155-170) ----
+ * p, g, m, v, sm, sr: HOST arrays of n device pointers; len: HOST array of n lengths.  p fp32 or (p_b16) bf16, g likewise.  bits = 32: m, v fp32.
+ * bits = 8: m, v = e4m3 codes of m and of sqrt(v), sm / sr = fp32 scales (powers of two), one per 128 consecutive elements of a tensor; the rounding
+ * to codes is dithered by a hash of (seed, *step, first + tensor, place).  step: device int32 holding this step's number; guard as in
+ * ha2g_adam_guarded_f32. */
+int ha2g_adamw_multi(int n, const long* p, const long* g, const long* m, const long* v, const long* sm, const long* sr, const long* len, int p_b16,
+                     int g_b16, int bits, double lr, double b1, double b2, double eps, double wd, unsigned seed, int first, const int* step,
+                     const int* guard, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

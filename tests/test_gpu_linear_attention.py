@@ -1,0 +1,256 @@
+"""ops.linear_attention / linear_attention_step against the recurrence in 64 bits.
+
+Tolerance: every output is a sum of products; with `mag` = the same sum over the operands' absolute values, n additions in fp32 (in any order or
+grouping) are off by at most n 2^-24 mag.  n = tokens + head size + 64 (the powers of the decay: exp to 2 ulp of an exponent rounded once, counted
+with the 64).  bf16 operands: intermediate factors (scores, states) are held as two bf16 pieces, 2^-16 mag more, and the result is rounded
+once, 2^-8 of its value."""
+import pytest
+import torch
+
+from ha2g_amd import ops
+
+pytestmark = pytest.mark.gpu
+DEV = 'cuda:0'
+
+
+def ref(q, k, v, g, state, n, scale, do=None, ds=None):
+    """the recurrence, in 64 bits on the CPU; n = tokens per row"""
+    H = g.numel()
+    up = lambda x: x.double().cpu().repeat_interleave(H // x.shape[2], 2)      # noqa: E731
+    shapes = q.shape[2], k.shape[2], v.shape[2]
+    q, k, v, g = up(q), up(k), up(v), g.double().cpu()
+    B, T, _, Dk = q.shape
+    Dv = v.shape[3]
+    S = torch.zeros(B, H, Dk, Dv, dtype=torch.float64) if state is None else state.double().cpu().clone()
+    lam = g.exp()[:, None, None]
+    o, dq, dk, dv = (torch.zeros(B, T, H, d, dtype=torch.float64) for d in (Dv, Dk, Dk, Dv))
+    do = None if do is None else do.double().cpu()
+    for b in range(B):
+        for t in range(int(n[b])):
+            S[b] = lam * S[b] + k[b, t, :, :, None] * v[b, t, :, None, :]
+            o[b, t] = scale * torch.einsum('hd,hde->he', q[b, t], S[b])
+            if do is not None:
+                dq[b, t] = scale * torch.einsum('hde,he->hd', S[b], do[b, t])
+    out = dict(o=o, state=S.clone())
+    if do is None:
+        return out
+    R = torch.zeros_like(S) if ds is None else ds.double().cpu().clone()
+    for b in range(B):
+        for t in reversed(range(int(n[b]))):
+            R[b] = R[b] + scale * q[b, t, :, :, None] * do[b, t, :, None, :]
+            dk[b, t] = torch.einsum('hde,he->hd', R[b], v[b, t])
+            dv[b, t] = torch.einsum('hde,hd->he', R[b], k[b, t])
+            R[b] = lam * R[b]
+    down = lambda d, h: d.unflatten(2, (h, -1)).sum(3)      # noqa: E731
+    out.update(dq=down(dq, shapes[0]), dk=down(dk, shapes[1]), dv=down(dv, shapes[2]), dstate=R)
+    return out
+
+
+def make(B, T, H, Hq, Hk, Hv, Dk, Dv, dt, seed=0, with_state=True, layout='plain'):
+    gen = torch.Generator().manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=gen)      # noqa: E731
+    q, k, v = r(B, T, Hq, Dk).to(dt), r(B, T, Hk, Dk).to(dt), r(B, T, Hv, Dv).to(dt)
+    if layout == 'fused':                   # slices of one projection's output, heads side by side
+        w = Hq * Dk + Hk * Dk + Hv * Dv
+        x = torch.cat([q.flatten(2), k.flatten(2), v.flatten(2)], 2).to(DEV)
+        assert x.shape[2] == w
+        a, b = Hq * Dk, Hq * Dk + Hk * Dk
+        q, k, v = x[:, :, :a].unflatten(2, (Hq, Dk)), x[:, :, a:b].unflatten(2, (Hk, Dk)), x[:, :, b:].unflatten(2, (Hv, Dv))
+    elif layout == 'heads_first':
+        q, k, v = (x.transpose(1, 2).contiguous().to(DEV).transpose(1, 2) for x in (q, k, v))
+    elif layout == 'inner':
+        q, k, v = (x.transpose(2, 3).contiguous().to(DEV).transpose(2, 3) for x in (q, k, v))
+    elif layout == 'odd':                   # bases that are not aligned to 16 bytes
+        q, k, v = (torch.cat([x.new_zeros(1), x.flatten()]).to(DEV)[1:].view(x.shape) for x in (q, k, v))
+    else:
+        q, k, v = q.to(DEV), k.to(DEV), v.to(DEV)
+    g = torch.log1p(-torch.exp2(-1.0 - 9.0 * torch.rand(H, generator=gen))).to(DEV)
+    return q, k, v, g, r(B, H, Dk, Dv).to(DEV) if with_state else None, r(B, T, H, Dv).to(dt).to(DEV), r(B, H, Dk, Dv).to(DEV)
+
+
+def near(got, want, mag, n, dt, what):
+    u = n * 2.0 ** -24 * mag
+    if dt == torch.bfloat16:
+        u = u + 2.0 ** -16 * mag
+    if got.dtype == torch.bfloat16:
+        u = u + 2.0 ** -8 * (want.abs() + u)
+    off = (got.double().cpu() - want).abs()
+    assert (off <= u + 1e-37).all(), (what, float((off / (u + 1e-37)).max()))
+
+
+def check_all(q, k, v, g, state, do, ds, lengths=None, scale=None, grad=True, want_ds=True):
+    dt, B, T = q.dtype, q.shape[0], q.shape[1]
+    n = torch.full((B,), T) if lengths is None else lengths.clamp(0, T).cpu()
+    sc = q.shape[3] ** -0.5 if scale is None else scale
+    leaves = [x for x in (q, k, v, state) if x is not None]
+    for x in leaves:
+        x.requires_grad_(grad)
+    o, s = ops.linear_attention(q, k, v, g, scale=scale, state=state, lengths=lengths, return_state=True)
+    assert o.dtype == dt and s.dtype == torch.float32
+    with torch.no_grad():
+        zero = torch.zeros_like(s)
+        want = ref(q, k, v, g, state, n, sc, do if grad else None, ds if want_ds else zero)
+        ab = lambda x: None if x is None else x.abs()      # noqa: E731
+        mag = ref(ab(q), ab(k), ab(v), g, ab(state), n, abs(sc), ab(do) if grad else None, ab(ds) if want_ds else zero)
+    got = dict(o=o.detach(), state=s.detach())
+    if grad:
+        grads = torch.autograd.grad([o, s] if want_ds else [o], leaves, [do, ds] if want_ds else [do])
+        got.update(zip(('dq', 'dk', 'dv', 'dstate'), grads))
+    cnt = T + max(q.shape[3], v.shape[3]) + 64 + g.numel()
+    for name, x in got.items():
+        near(x, want[name], mag[name], cnt, dt, name)
+    return got
+
+
+@pytest.mark.parametrize('dt', (torch.float32, torch.bfloat16), ids=('fp32', 'bf16'))
+@pytest.mark.parametrize('T', (0, 1, 2, 15, 16, 17, 31, 33, 63, 64, 65, 100, 129))
+def test_lengths_around_the_tiles(T, dt):
+    check_all(*make(2, T, 3, 3, 3, 3, 60, 60, dt, seed=T))
+
+
+@pytest.mark.parametrize('dt', (torch.float32, torch.bfloat16), ids=('fp32', 'bf16'))
+@pytest.mark.parametrize('Dk,Dv', ((1, 1), (4, 8), (8, 4), (16, 16), (25, 50), (32, 64), (33, 31), (64, 128), (75, 75), (128, 32), (128, 128), (127, 96)))
+def test_head_sizes(Dk, Dv, dt):
+    check_all(*make(1, 70, 2, 2, 2, 2, Dk, Dv, dt, seed=Dk))
+
+
+@pytest.mark.parametrize('dt', (torch.float32, torch.bfloat16), ids=('fp32', 'bf16'))
+@pytest.mark.parametrize('heads', ((4, 4, 4, 4), (4, 1, 1, 4), (6, 2, 3, 6), (4, 4, 4, 1), (6, 1, 6, 2)))
+def test_shared_heads_and_their_gradients(heads, dt):
+    check_all(*make(2, 40, *heads, 16, 24, dt, seed=3))
+
+
+@pytest.mark.parametrize('dt', (torch.float32, torch.bfloat16), ids=('fp32', 'bf16'))
+@pytest.mark.parametrize('layout', ('fused', 'heads_first', 'inner', 'odd'))
+def test_layouts(layout, dt):
+    check_all(*make(2, 37, 4, 4, 2, 4, 20, 28, dt, seed=4, layout=layout))
+
+
+@pytest.mark.parametrize('dt', (torch.float32, torch.bfloat16), ids=('fp32', 'bf16'))
+def test_ragged_rows_whose_padding_is_not_a_number(dt):
+    """rows of no token, of one, of all, and lengths outside 0 .. T; NaN and infinities behind a row's end reach nothing"""
+    q, k, v, g, state, do, ds = make(6, 50, 3, 3, 1, 3, 16, 32, dt, seed=5)
+    lengths = torch.tensor([0, 1, 50, 33, -4, 99], dtype=torch.int32, device=DEV)
+    for b, n in enumerate((0, 1, 50, 33, 0, 50)):
+        q[b, n:], k[b, n:], v[b, n:], do[b, n:] = float('nan'), float('inf'), float('-inf'), float('nan')
+    clean = [torch.where((torch.arange(50, device=DEV) < lengths[:, None])[:, :, None, None], x, 0.0).to(dt) for x in (q, k, v, do)]
+    got = {}
+    leaves = [x.requires_grad_() for x in (q, k, v, state)]
+    o, s = ops.linear_attention(q, k, v, g, state=state, lengths=lengths, return_state=True)
+    got.update(o=o, state=s, **dict(zip(('dq', 'dk', 'dv', 'dstate'), torch.autograd.grad([o, s], leaves, [do, ds]))))
+    want = check_all(clean[0], clean[1], clean[2], g, state.detach().clone(), clean[3], ds, lengths=lengths)
+    for n, x in got.items():
+        assert torch.equal(x, want[n]), n
+
+
+@pytest.mark.parametrize('with_state,want_ds', ((False, True), (True, False), (False, False)))
+def test_without_a_first_state_or_a_last_gradient(with_state, want_ds):
+    check_all(*make(2, 45, 2, 2, 2, 2, 32, 16, torch.float32, seed=6, with_state=with_state), want_ds=want_ds)
+
+
+def test_scale_decay_one_and_decay_zero():
+    q, k, v, g, state, do, ds = make(1, 66, 3, 3, 3, 3, 8, 8, torch.float32, seed=7)
+    check_all(q, k, v, torch.zeros_like(g), state, do, ds, scale=-2.5)
+    check_all(q.detach(), k.detach(), v.detach(), torch.full_like(g, -60.0), state.detach(), do, ds, scale=1.0)
+    # log(0): only the token itself is left
+    o = ops.linear_attention(q.detach(), k.detach(), v.detach(), torch.full_like(g, float('-inf')), scale=1.0)
+    want = torch.einsum('bthd,bthd->bth', q.detach().double(), k.detach().double())[..., None] * v.detach().double()
+    assert ((o.double() - want).abs() <= 80 * 2.0 ** -24 * (q * k).abs().sum(3, keepdim=True).detach() * v.detach().abs() + 1e-30).all()
+
+
+@pytest.mark.parametrize('dt', (torch.float32, torch.bfloat16), ids=('fp32', 'bf16'))
+def test_one_long_sequence_equals_its_parts(dt):
+    """the time axis split over the chip: 9001 tokens of one row against the same call in three parts that hand the state on, and a 64-bit recurrence"""
+    q, k, v, g, state, do, ds = make(1, 9001, 2, 2, 2, 2, 32, 48, dt, seed=8)
+    got = check_all(q, k, v, g, state, do, ds)
+    s, parts = state.detach(), []
+    for a, b in ((0, 1), (1, 4097), (4097, 9001)):
+        o, s = ops.linear_attention(q[:, a:b].detach(), k[:, a:b].detach(), v[:, a:b].detach(), g, state=s, return_state=True)
+        parts.append(o)
+    o = torch.cat(parts, 1).double()
+    tol = 2.0 ** -7 if dt == torch.bfloat16 else 2.0 ** -13
+    assert float((o - got['o'].double()).norm() / o.norm()) <= tol and float((s - got['state']).norm() / s.norm()) <= 2.0 ** -13
+
+
+def test_gradients_against_differences():
+    """d/de of <o, do> + <S_T, ds> along random directions, the loss summed in 64 bits from fp32 outputs: central differences of step 2^-5 of a loss
+    that is at most of third degree in the step (no third-degree term in a single operand): exact up to the outputs' rounding"""
+    q, k, v, g, state, do, ds = make(2, 70, 2, 2, 1, 2, 12, 20, torch.float32, seed=9)
+    leaves = [x.requires_grad_() for x in (q, k, v, state)]
+    o, s = ops.linear_attention(q, k, v, g, state=state, return_state=True)
+    grads = torch.autograd.grad([o, s], leaves, [do, ds])
+    for i, (x, d) in enumerate(zip(leaves, grads)):
+        r = torch.randn(x.shape, generator=torch.Generator().manual_seed(i)).to(DEV)
+        vals = []
+        for sign in (1, -1):
+            args = [y.detach() for y in leaves]
+            args[i] = args[i] + sign * 2.0 ** -5 * r
+            oo, ss = ops.linear_attention(*args[:3], g, state=args[3], return_state=True)
+            vals.append((oo.double() * do.double()).sum() + (ss.double() * ds.double()).sum())
+        num, ana = (vals[0] - vals[1]) * 2.0 ** 4, (d.double() * r.double()).sum()
+        size = (o.double() * do.double()).abs().sum() + (s.double() * ds.double()).abs().sum()
+        assert abs(num - ana) <= 2.0 ** 5 * 200 * 2.0 ** -24 * size, (i, float(num), float(ana))
+
+
+@pytest.mark.parametrize('dt', (torch.float32, torch.bfloat16), ids=('fp32', 'bf16'))
+@pytest.mark.parametrize('B,H,Hq,Hk,Hv,Dk,Dv', ((1, 5, 5, 5, 5, 60, 60), (3, 4, 1, 2, 4, 128, 128), (2, 1, 1, 1, 1, 1, 1), (7, 6, 3, 6, 2, 25, 75), (0, 2, 2, 2, 2, 8, 8),
+                                                   (2, 2, 2, 2, 2, 128, 4), (2, 2, 2, 2, 2, 3, 128), (300, 2, 2, 2, 2, 33, 64)))
+def test_single_tokens_follow_the_sequence(B, H, Hq, Hk, Hv, Dk, Dv, dt):
+    q, k, v, g, state, _, _ = make(B, 4, H, Hq, Hk, Hv, Dk, Dv, dt, seed=11)
+    s = state.clone()
+    before = s._version
+    outs = [ops.linear_attention_step(q[:, t], k[:, t], v[:, t], g, s) for t in range(4)]
+    assert s._version > before
+    n = torch.full((B,), 4)
+    sc = Dk ** -0.5
+    want, mag = ref(q, k, v, g, state, n, sc), ref(q.abs(), k.abs(), v.abs(), g, state.abs(), n, sc)
+    near(torch.stack(outs, 1), want['o'], mag['o'], 4 + max(Dk, Dv) + 64, torch.float32 if dt == torch.float32 else dt, 'o')
+    near(s, want['state'], mag['state'], 4 + 64, torch.float32, 'state')
+
+
+def test_step_refuses_gradients_and_strided_states():
+    q, k, v, g, state, _, _ = make(2, 1, 2, 2, 2, 2, 8, 8, torch.float32)
+    with pytest.raises(ValueError):
+        ops.linear_attention_step(q[:, 0].requires_grad_(), k[:, 0], v[:, 0], g, state)
+    with pytest.raises(ValueError):
+        ops.linear_attention_step(q[:, 0].detach(), k[:, 0], v[:, 0], g, state.transpose(2, 3))
+
+
+def test_two_streams_and_a_captured_graph():
+    """forward, backward and a token in one graph, replayed with new contents between eager calls, and two streams at once: every run's bits are the eager
+    run's on the same contents"""
+    a, b = make(2, 300, 2, 2, 1, 2, 32, 32, torch.float32, seed=12), make(2, 300, 2, 2, 1, 2, 32, 32, torch.float32, seed=13)
+
+    def run(t):
+        q, k, v, g, state, do, ds = t
+        leaves = [x.detach().requires_grad_() for x in (q, k, v, state)]
+        o, s = ops.linear_attention(*leaves[:3], g, state=leaves[3], return_state=True)
+        grads = torch.autograd.grad([o, s], leaves, [do, ds])
+        st = state.detach().clone()
+        one = ops.linear_attention_step(q[:, 0].detach(), k[:, 0].detach(), v[:, 0].detach(), g, st)
+        return [o.detach(), s.detach(), *grads, one, st]
+    want = [[x.clone() for x in run(t)] for t in (a, b)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(3):
+        for i, t in enumerate((a, b)):
+            with torch.cuda.stream(streams[i]):
+                got.append((i, run(t)))
+    torch.cuda.synchronize()
+    for i, x in got:
+        assert all(torch.equal(p, q) for p, q in zip(x, want[i]))
+    held = [x.detach().clone() for x in a]
+    with torch.cuda.stream(streams[0]):
+        run(held)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=streams[0]):
+        out = run(held)
+    for src, w in ((b, want[1]), (a, want[0]), (b, want[1])):
+        for x, y in zip(held, src):
+            x.copy_(y.detach())
+        graph.replay()
+        eager = run(a)
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(out, w)) and all(torch.equal(p, q) for p, q in zip(eager, want[0]))
