@@ -1947,9 +1947,12 @@ def _la_strides(*ts):
 def _la_call(q, k, v, o, log_decay, s_in, s_out, lengths, transposed, o_scale, u_scale, reverse):
     B, T, H = q.shape[0], q.shape[1], log_decay.numel()
     q, k, v = _inner1(q), _inner1(k), _inner1(v)
+    bf = int(q.dtype == torch.bfloat16)
+    n = lib.ha2g_linattn_workspace_floats(B, T, H, q.shape[3], v.shape[3], bf)
+    ws = torch.empty(n, dtype=torch.float32, device=q.device) if n else None
     check(lib.ha2g_linattn(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), log_decay.data_ptr(), _p(s_in), _p(s_out), _p(lengths),
                            _la_strides(q, k, v, o), B, T, H, H // q.shape[2], H // k.shape[2], H // v.shape[2], q.shape[3], v.shape[3], int(transposed),
-                           o_scale, u_scale, int(reverse), int(q.dtype == torch.bfloat16), int(o.dtype == torch.bfloat16), _stream()))
+                           o_scale, u_scale, int(reverse), bf, int(o.dtype == torch.bfloat16), _p(ws), _stream()))
 
 
 def _la_grad(like, H, dtype):

@@ -582,7 +582,9 @@ int ha2g_logmel_f32(const float* y, int B, long n_samples, int pad_reflect, cons
  *   dv = (k, q, do) reverse, s_in := dS_T, u_scale = scale, o_scale = 1, s_out = dS_0. */
 int ha2g_linattn(const void* q, const void* k, const void* v, void* o, const float* log_decay, const float* s_in, float* s_out, const int* lengths,
                  const long* strides, int B, int T, int H, int rq, int rk, int rv, int Dk, int Dv, int s_transposed, float o_scale, float u_scale,
-                 int reverse, int b16_in, int b16_out, void* stream);
+                 int reverse, int b16_in, int b16_out, float* ws, void* stream);
+/* floats of `ws` (0: may be NULL): the states between the segments of a time axis that is split over the chip */
+long ha2g_linattn_workspace_floats(int B, int T, int H, int Dk, int Dv, int b16_in);
 /* one token: q [B][..][Dk] ..., state updated in place; the token strides are not read */
 int ha2g_linattn_step(const void* q, const void* k, const void* v, void* o, const float* log_decay, float* state, const long* strides, int B, int H,
                       int rq, int rk, int rv, int Dk, int Dv, float o_scale, int b16_io, void* stream);
