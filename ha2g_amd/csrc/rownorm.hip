@@ -24,46 +24,78 @@ struct TailArgs {
     float alpha, eps;
 };
 
-template <int VEC> __device__ __forceinline__ void load_row(const float* p, long at, float* x) {
-    if constexpr (VEC == 4) { const float4 v = *reinterpret_cast<const float4*>(p + at); x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w; }
-    else x[0] = p[at];
+// VEC values as they lie in memory, 16 bytes at most
+template <typename T, int VEC> struct Raw { unsigned u[(VEC * sizeof(T) + 3) / 4]; };
+template <typename T, int VEC> __device__ __forceinline__ Raw<T, VEC> load_raw(const T* p, long at) {
+    Raw<T, VEC> r;
+    if constexpr (VEC * sizeof(T) == 16) { const uint4 v = *reinterpret_cast<const uint4*>(p + at); r.u[0] = v.x; r.u[1] = v.y; r.u[2] = v.z; r.u[3] = v.w; }
+    else if constexpr (VEC * sizeof(T) == 8) { const uint2 v = *reinterpret_cast<const uint2*>(p + at); r.u[0] = v.x; r.u[1] = v.y; }
+    else if constexpr (sizeof(T) == 4) r.u[0] = __float_as_uint(p[at]);
+    else r.u[0] = p[at];
+    return r;
 }
-template <int VEC> __device__ __forceinline__ void load_row(const b16* p, long at, float* x) {
-    if constexpr (VEC == 4) { const float4 v = ld4(p + at, 0); x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w; }
-    else x[0] = ld1(p, at);
+template <int VEC> __device__ __forceinline__ void unpack(const Raw<float, VEC>& r, float* x) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) x[j] = __uint_as_float(r.u[j]);
+}
+template <int VEC> __device__ __forceinline__ void unpack(const Raw<b16, VEC>& r, float* x) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) x[j] = __uint_as_float((j & 1) ? r.u[j >> 1] & 0xffff0000u : r.u[j >> 1] << 16);
 }
 template <int VEC> __device__ __forceinline__ void store_row(float* p, long at, const float* x) {
-    if constexpr (VEC == 4) *reinterpret_cast<float4*>(p + at) = make_float4(x[0], x[1], x[2], x[3]);
-    else p[at] = x[0];
+    if constexpr (VEC >= 4) {
+#pragma unroll
+        for (int j = 0; j < VEC; j += 4) *reinterpret_cast<float4*>(p + at + j) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
+    } else p[at] = x[0];
 }
 template <int VEC> __device__ __forceinline__ void store_row(b16* p, long at, const float* x) {
-    if constexpr (VEC == 4) st4(p + at, 0, make_float4(x[0], x[1], x[2], x[3]));
-    else { unsigned h, l; split2_bf16(x[0], 0.f, h, l); p[at] = (b16)(h & 0xffff); }
+    unsigned h[(VEC + 1) / 2], l;
+#pragma unroll
+    for (int j = 0; j < VEC; j += 2) split2_bf16(x[j], VEC > 1 ? x[j + (VEC > 1)] : 0.f, h[j >> 1], l);
+    if constexpr (VEC == 8) *reinterpret_cast<uint4*>(p + at) = make_uint4(h[0], h[1], h[2], h[3]);
+    else if constexpr (VEC == 4) *reinterpret_cast<uint2*>(p + at) = make_uint2(h[0], h[1]);
+    else p[at] = (b16)(h[0] & 0xffff);
+}
+template <int VEC> __device__ __forceinline__ void load_vec(const float* p, long at, float* x) {
+    if constexpr (VEC >= 4) {
+#pragma unroll
+        for (int j = 0; j < VEC; j += 4) { const float4 v = *reinterpret_cast<const float4*>(p + at + j); x[j] = v.x; x[j + 1] = v.y; x[j + 2] = v.z; x[j + 3] = v.w; }
+    } else x[0] = p[at];
+}
+template <int VEC> __device__ __forceinline__ void fill(float* x, float v) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) x[j] = v;
 }
 
 // the gate's activation and its derivative
-__device__ __forceinline__ float gate_act(float g, int act) { return act == 0 ? g : (act == 3 ? sigmoidf_(g) : g * sigmoidf_(g)); }
-__device__ __forceinline__ float gate_act_d(float g, int act) {
-    if (act == 0) return 1.f;
+__device__ __forceinline__ void gate_act(float g, int act, float& a, float& d) {
+    if (act == 0) { a = g; d = 1.f; return; }
     const float s = sigmoidf_(g);
-    return act == 3 ? s * (1.f - s) : s * (1.f + g * (1.f - s));
+    a = act == 3 ? s : g * s;
+    d = act == 3 ? s * (1.f - s) : s * (1.f + g * (1.f - s));
 }
 
-// Sums over the row's TPR threads of one value per chunk: r[i] = the sum over the group chunk i belongs to.  One group: a butterfly (and, for more
-// than a wave, LDS).  Several: every chunk's value goes to LDS, 16 lanes add up a group, its sum is read back from the group's first place.
+// Sums over the row's TPR threads of one value per chunk: r[i] = the sum over the group chunk i belongs to.  The whole row: a butterfly, and beyond a
+// wave one meeting in LDS (two places in turn).  Groups of 2^n <= 64 chunks: a butterfly over their lanes.  Others (heads of 60): every chunk's
+// value goes to LDS, 16 lanes add up a group, its sum is read back from the group's first place.  A row of one wave needs no barrier.
 // Every thread of the block calls it the same number of times.
 template <int TPR, int NI> struct RowSum {
-    float* lds;                  // this row's TPR * NI floats
-    int lane, G, cpg, nch;       // thread of the row, groups, chunks per group, chunks
+    float *lds, *meet;           // this row's TPR * NI floats; two times TPR / 64
+    int lane, G, cpg, nch, phase;      // thread of the row, groups, chunks per group, chunks
+    __device__ __forceinline__ static void sync() {
+        if constexpr (TPR > 64) __syncthreads();
+        else { __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront"); __builtin_amdgcn_wave_barrier(); __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront"); }
+    }
     __device__ __forceinline__ float all(float s) {
         s = wave_sum(s);
         if constexpr (TPR > 64) {
-            __syncthreads();
-            if ((lane & 63) == 0) lds[lane >> 6] = s;
+            float* m = meet + phase * (TPR / 64);
+            phase ^= 1;
+            if ((lane & 63) == 0) m[lane >> 6] = s;
             __syncthreads();
             s = 0.f;
 #pragma unroll
-            for (int i = 0; i < TPR / 64; ++i) s += lds[i];
+            for (int i = 0; i < TPR / 64; ++i) s += m[i];
         }
         return s;
     }
@@ -77,13 +109,21 @@ template <int TPR, int NI> struct RowSum {
             for (int i = 0; i < NI; ++i) r[i] = s;
             return;
         }
-        __syncthreads();
+        if (cpg <= 64 && (cpg & (cpg - 1)) == 0) {
+#pragma unroll
+            for (int i = 0; i < NI; ++i) r[i] = p[i];
+            for (int o = cpg >> 1; o > 0; o >>= 1)
+#pragma unroll
+                for (int i = 0; i < NI; ++i) r[i] += __shfl_xor(r[i], o, 64);
+            return;
+        }
+        sync();
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
             const int c = lane + i * TPR;
             if (c < nch) lds[c] = p[i];
         }
-        __syncthreads();
+        sync();
         for (int g = lane >> 4; g < G; g += TPR / 16) {
             float s = 0.f;
             for (int c = lane & 15; c < cpg; c += 16) s += lds[g * cpg + c];
@@ -91,7 +131,7 @@ template <int TPR, int NI> struct RowSum {
             for (int o = 8; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
             if ((lane & 15) == 0) lds[g * cpg] = s;
         }
-        __syncthreads();
+        sync();
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
             const int c = lane + i * TPR;
@@ -100,7 +140,7 @@ template <int TPR, int NI> struct RowSum {
     }
 };
 
-// x -> x^ in place; r / m: 1 / std and mean per chunk
+// x -> x^ in place; m / r: mean and 1 / std per chunk
 template <int TPR, int NI, int VEC>
 __device__ __forceinline__ void normalise(RowSum<TPR, NI>& rsum, float (&x)[NI][VEC], float (&m)[NI], float (&r)[NI], bool layer, float inv, float eps) {
     float p[NI];
@@ -139,24 +179,50 @@ __device__ __forceinline__ void normalise(RowSum<TPR, NI>& rsum, float (&x)[NI][
 
 template <int TPR> constexpr int block_of() { return TPR > 256 ? TPR : 256; }
 
+// The parameters' columns of a thread: kept in registers over the rows where a thread has one chunk, read from the caches per row otherwise.
+template <int NI, int VEC> struct Columns {
+    static constexpr bool KEEP = NI == 1;
+    float w[VEC], b[VEC], s[VEC], w2[VEC], b2[VEC];
+    __device__ __forceinline__ void load(const TailArgs& a, long at, bool in) {
+        fill<VEC>(w, 1.f); fill<VEC>(b, 0.f); fill<VEC>(s, 1.f); fill<VEC>(w2, 0.f); fill<VEC>(b2, 0.f);
+        if (!in) return;
+        if (a.w) load_vec<VEC>(a.w, at, w);
+        if (a.b) load_vec<VEC>(a.b, at, b);
+        if (a.s) load_vec<VEC>(a.s, at, s);
+        if (a.w2) load_vec<VEC>(a.w2, at, w2);
+        if (a.b2) load_vec<VEC>(a.b2, at, b2);
+    }
+};
+
 template <typename T, int TPR, int NI, int VEC>
 __global__ __launch_bounds__(block_of<TPR>()) void tail_fwd_kernel(const TailArgs a) {
     constexpr int RPB = block_of<TPR>() / TPR;
-    __shared__ float lds[RPB * TPR * NI];
+    __shared__ float lds[RPB * TPR * NI], meet[2][2 * (TPR / 64)];
     const int sub = threadIdx.x / TPR, lane = threadIdx.x % TPR, nch = a.C / VEC;
     const long rows = a.inner * a.outer;
-    RowSum<TPR, NI> gsum{lds + sub * TPR * NI, lane, a.G, nch / a.G, nch}, rsum{lds + sub * TPR * NI, lane, 1, nch, nch};
+    RowSum<TPR, NI> gsum{lds + sub * TPR * NI, meet[0], lane, a.G, nch / a.G, nch, 0}, rsum{lds + sub * TPR * NI, meet[1], lane, 1, nch, nch, 0};
+    Columns<NI, VEC> col;
+    if constexpr (Columns<NI, VEC>::KEEP) col.load(a, (long)lane * VEC, lane < nch);
     for (long r0 = (long)blockIdx.x * RPB; r0 < rows; r0 += (long)gridDim.x * RPB) {
         const long row = r0 + sub;
         const bool in = row < rows;
         const long at = row * a.C, gat = a.gate_shared ? row / a.inner * a.C : at;
+        Raw<T, VEC> ry[NI], rg[NI], rr[NI];
         float x[NI][VEC], m[NI], r[NI];
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
             const int c = lane + i * TPR;
+            if (in && c < nch) {
+                ry[i] = load_raw<T, VEC>((const T*)a.y, at + (long)c * VEC);
+                if (a.gate) rg[i] = load_raw<T, VEC>((const T*)a.gate, gat + (long)c * VEC);
+                if (a.res) rr[i] = load_raw<T, VEC>((const T*)a.res, at + (long)c * VEC);
+            }
+        }
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) x[i][j] = 0.f;
-            if (in && c < nch) load_row<VEC>((const T*)a.y, at + (long)c * VEC, x[i]);
+        for (int i = 0; i < NI; ++i) {
+            const int c = lane + i * TPR;
+            fill<VEC>(x[i], 0.f);
+            if (in && c < nch) unpack<VEC>(ry[i], x[i]);
         }
         if (a.w) {
             normalise<TPR, NI, VEC>(gsum, x, m, r, a.layer, (float)a.G / a.C, a.eps);
@@ -175,29 +241,23 @@ __global__ __launch_bounds__(block_of<TPR>()) void tail_fwd_kernel(const TailArg
         for (int i = 0; i < NI; ++i) {
             const int c = lane + i * TPR;
             if (!(in && c < nch)) continue;
+            if constexpr (!Columns<NI, VEC>::KEEP) col.load(a, (long)c * VEC, true);
             float t[VEC];
             if (a.w) {
-                load_row<VEC>(a.w, (long)c * VEC, t);
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) x[i][j] *= t[j];
-            }
-            if (a.b) {
-                load_row<VEC>(a.b, (long)c * VEC, t);
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) x[i][j] += t[j];
+                for (int j = 0; j < VEC; ++j) x[i][j] = x[i][j] * col.w[j] + col.b[j];
             }
             if (a.gate) {
-                load_row<VEC>((const T*)a.gate, gat + (long)c * VEC, t);
+                unpack<VEC>(rg[i], t);
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) x[i][j] *= gate_act(t[j], a.act);
+                for (int j = 0; j < VEC; ++j) { float ga, gd; gate_act(t[j], a.act, ga, gd); x[i][j] *= ga; }
             }
             if (a.s) {
-                load_row<VEC>(a.s, (long)c * VEC, t);
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) x[i][j] *= t[j];
+                for (int j = 0; j < VEC; ++j) x[i][j] *= col.s[j];
             }
             if (a.res) {
-                load_row<VEC>((const T*)a.res, at + (long)c * VEC, t);
+                unpack<VEC>(rr[i], t);
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) x[i][j] = a.alpha * t[j] + x[i][j];
             }
@@ -213,108 +273,123 @@ __global__ __launch_bounds__(block_of<TPR>()) void tail_fwd_kernel(const TailArg
             for (int i = 0; i < NI; ++i) {
                 const int c = lane + i * TPR;
                 if (!(in && c < nch)) continue;
-                float t[VEC];
-                load_row<VEC>(a.w2, (long)c * VEC, t);
+                if constexpr (!Columns<NI, VEC>::KEEP) col.load(a, (long)c * VEC, true);
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) x[i][j] *= t[j];
-                if (a.b2) {
-                    load_row<VEC>(a.b2, (long)c * VEC, t);
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) x[i][j] += t[j];
-                }
+                for (int j = 0; j < VEC; ++j) x[i][j] = x[i][j] * col.w2[j] + col.b2[j];
                 store_row<VEC>((T*)a.z, at + (long)c * VEC, x[i]);
             }
         }
     }
 }
 
+// One row's operands on their way: loaded a row ahead, so that a row's sums and barriers lie under the next row's loads
+template <typename T, int NI, int VEC, bool FULL> struct RowIn {
+    Raw<T, VEC> y[NI], dh[NI], dz[FULL ? NI : 1], gate[FULL ? NI : 1], res[FULL ? NI : 1];
+    float mu[NI], rs[NI], mu2, rs2;
+    __device__ __forceinline__ void load(const TailArgs& a, long row, long gat, bool in, int lane, int tpr, int nch, const int* grp) {
+        mu2 = rs2 = 0.f;
+        const long at = row * a.C;
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            const int c = lane + i * tpr;
+            mu[i] = rs[i] = 0.f;
+            if (!(in && c < nch)) continue;
+            y[i] = load_raw<T, VEC>((const T*)a.y, at + (long)c * VEC);
+            if (a.dh) dh[i] = load_raw<T, VEC>((const T*)a.dh, at + (long)c * VEC);
+            if (a.w) {
+                rs[i] = a.rs[row * a.G + grp[i]];
+                if (a.layer) mu[i] = a.mu[row * a.G + grp[i]];
+            }
+            if constexpr (FULL) {
+                if (a.dz) dz[i] = load_raw<T, VEC>((const T*)a.dz, at + (long)c * VEC);
+                if (a.gate) gate[i] = load_raw<T, VEC>((const T*)a.gate, gat + (long)c * VEC);
+                if (a.res && a.w2) res[i] = load_raw<T, VEC>((const T*)a.res, at + (long)c * VEC);
+            }
+        }
+        if constexpr (FULL) {
+            if (a.w2 && in) {
+                rs2 = a.rs2[row];
+                if (a.layer) mu2 = a.mu2[row];
+            }
+        }
+    }
+};
+
 // A block walks through the rows of its slice of a sequence and keeps the columns' sums in registers; its partial sums leave it once.
 // FULL: with gate, scale, residual or second norm; otherwise the norm alone (w, b).
 template <typename T, int TPR, int NI, int VEC, bool FULL>
 __global__ __launch_bounds__(block_of<TPR>()) void tail_bwd_kernel(const TailArgs a) {
     constexpr int RPB = block_of<TPR>() / TPR, NV = FULL ? 6 : 2;      // w, b, s, w2, b2, gate
-    __shared__ float lds[RPB * TPR * NI * (VEC > 1 && RPB > 1 ? VEC : 1)];
+    __shared__ float lds[RPB * TPR * NI * (RPB > 1 ? VEC : 1)], meet[2][2 * (TPR / 64)];
     const int sub = threadIdx.x / TPR, lane = threadIdx.x % TPR, nch = a.C / VEC;
     float* const mine = lds + sub * TPR * NI;
-    RowSum<TPR, NI> gsum{mine, lane, a.G, nch / a.G, nch}, rsum{mine, lane, 1, nch, nch};
+    RowSum<TPR, NI> gsum{mine, meet[0], lane, a.G, nch / a.G, nch, 0}, rsum{mine, meet[1], lane, 1, nch, nch, 0};
     const long per = (a.inner + gridDim.x - 1) / gridDim.x, beg = blockIdx.x * per, end = min(a.inner, beg + per);
     const float inv = (float)a.G / a.C, inv2 = 1.0f / a.C;
+    const long row0 = (long)blockIdx.y * a.inner, gat0 = (long)blockIdx.y * a.C;
+    int grp[NI];
+#pragma unroll
+    for (int i = 0; i < NI; ++i) grp[i] = (lane + i * TPR) / gsum.cpg;
     float acc[NV][NI][VEC];
 #pragma unroll
     for (int n = 0; n < NV; ++n)
 #pragma unroll
-        for (int i = 0; i < NI; ++i)
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) acc[n][i][j] = 0.f;
+        for (int i = 0; i < NI; ++i) fill<VEC>(acc[n][i], 0.f);
+    Columns<NI, VEC> col;
+    if constexpr (Columns<NI, VEC>::KEEP) col.load(a, (long)lane * VEC, lane < nch);
+    RowIn<T, NI, VEC, FULL> cur, nxt;
+    cur.load(a, row0 + beg + sub, a.gate_shared ? gat0 : (row0 + beg + sub) * a.C, beg + sub < end, lane, TPR, nch, grp);
     for (long q0 = beg; q0 < end; q0 += RPB) {
         const bool in = q0 + sub < end;
-        const long row = (long)blockIdx.y * a.inner + q0 + sub;
-        const long at = row * a.C, gat = a.gate_shared ? (long)blockIdx.y * a.C : at;
-        float y[NI][VEC], d[NI][VEC], r[NI];
+        const long row = row0 + q0 + sub, at = row * a.C;
+        nxt.load(a, row + RPB, a.gate_shared ? gat0 : (row + RPB) * a.C, q0 + RPB + sub < end, lane, TPR, nch, grp);
+        float xh[NI][VEC], n[NI][VEC], d[NI][VEC], ga[FULL ? NI : 1][VEC], gd[FULL ? NI : 1][VEC];
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
             const int c = lane + i * TPR;
-            r[i] = 0.f;
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) y[i][j] = d[i][j] = 0.f;
+            fill<VEC>(xh[i], 0.f); fill<VEC>(n[i], 0.f); fill<VEC>(d[i], 0.f);
+            if constexpr (FULL) { fill<VEC>(ga[i], 1.f); fill<VEC>(gd[i], 0.f); }
             if (!(in && c < nch)) continue;
-            load_row<VEC>((const T*)a.y, at + (long)c * VEC, y[i]);
-            if (a.dh) load_row<VEC>((const T*)a.dh, at + (long)c * VEC, d[i]);
+            if constexpr (!Columns<NI, VEC>::KEEP) col.load(a, (long)c * VEC, true);
+            unpack<VEC>(cur.y[i], xh[i]);
+            if (a.dh) unpack<VEC>(cur.dh[i], d[i]);
             if (a.w) {
-                const long g = row * a.G + c / gsum.cpg;
-                const float m = a.layer ? a.mu[g] : 0.f;
-                r[i] = a.rs[g];
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) y[i][j] = (y[i][j] - m) * r[i];
+                for (int j = 0; j < VEC; ++j) xh[i][j] = (xh[i][j] - cur.mu[i]) * cur.rs[i];
+            }
+            if constexpr (FULL) {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) n[i][j] = a.w ? xh[i][j] * col.w[j] + col.b[j] : xh[i][j];
+                if (a.gate) {
+                    float t[VEC];
+                    unpack<VEC>(cur.gate[i], t);
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) gate_act(t[j], a.act, ga[i][j], gd[i][j]);
+                }
             }
         }
-        // y = x^ (or x without a norm), d = dh
         if constexpr (FULL) {
             if (a.w2) {
                 float hh[NI][VEC], e[NI][VEC], s1 = 0.f, s2 = 0.f;
-                const float m2 = (in && a.layer) ? a.mu2[row] : 0.f, r2 = in ? a.rs2[row] : 0.f;
 #pragma unroll
                 for (int i = 0; i < NI; ++i) {
                     const int c = lane + i * TPR;
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) hh[i][j] = e[i][j] = 0.f;
+                    fill<VEC>(hh[i], 0.f); fill<VEC>(e[i], 0.f);
                     if (!(in && c < nch)) continue;
+                    if constexpr (!Columns<NI, VEC>::KEEP) col.load(a, (long)c * VEC, true);
                     float t[VEC];
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) hh[i][j] = y[i][j];
-                    if (a.w) {
-                        load_row<VEC>(a.w, (long)c * VEC, t);
-#pragma unroll
-                        for (int j = 0; j < VEC; ++j) hh[i][j] *= t[j];
-                    }
-                    if (a.b) {
-                        load_row<VEC>(a.b, (long)c * VEC, t);
-#pragma unroll
-                        for (int j = 0; j < VEC; ++j) hh[i][j] += t[j];
-                    }
-                    if (a.gate) {
-                        load_row<VEC>((const T*)a.gate, gat + (long)c * VEC, t);
-#pragma unroll
-                        for (int j = 0; j < VEC; ++j) hh[i][j] *= gate_act(t[j], a.act);
-                    }
-                    if (a.s) {
-                        load_row<VEC>(a.s, (long)c * VEC, t);
-#pragma unroll
-                        for (int j = 0; j < VEC; ++j) hh[i][j] *= t[j];
-                    }
-                    if (a.res) {
-                        load_row<VEC>((const T*)a.res, at + (long)c * VEC, t);
-#pragma unroll
-                        for (int j = 0; j < VEC; ++j) hh[i][j] = a.alpha * t[j] + hh[i][j];
-                    }
-                    if (a.dz) load_row<VEC>((const T*)a.dz, at + (long)c * VEC, e[i]);
-                    load_row<VEC>(a.w2, (long)c * VEC, t);
+                    fill<VEC>(t, 0.f);
+                    if (a.res) unpack<VEC>(cur.res[i], t);
+                    if (a.dz) unpack<VEC>(cur.dz[i], e[i]);
 #pragma unroll
                     for (int j = 0; j < VEC; ++j) {
-                        hh[i][j] = (hh[i][j] - m2) * r2;
+                        float h = n[i][j] * ga[i][j];
+                        if (a.s) h *= col.s[j];
+                        if (a.res) h = a.alpha * t[j] + h;
+                        hh[i][j] = (h - cur.mu2) * cur.rs2;
                         acc[3][i][j] += e[i][j] * hh[i][j];
                         acc[4][i][j] += e[i][j];
-                        e[i][j] *= t[j];
+                        e[i][j] *= col.w2[j];
                         s1 += e[i][j] * hh[i][j];
                         s2 += e[i][j];
                     }
@@ -324,7 +399,7 @@ __global__ __launch_bounds__(block_of<TPR>()) void tail_bwd_kernel(const TailArg
 #pragma unroll
                 for (int i = 0; i < NI; ++i)
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) d[i][j] += r2 * (e[i][j] - hh[i][j] * s1 - s2);
+                    for (int j = 0; j < VEC; ++j) d[i][j] += cur.rs2 * (e[i][j] - hh[i][j] * s1 - s2);
             }
         }
         // d = the whole gradient of h (of n, where there is nothing behind it) -> d(x^)
@@ -333,45 +408,25 @@ __global__ __launch_bounds__(block_of<TPR>()) void tail_bwd_kernel(const TailArg
         for (int i = 0; i < NI; ++i) {
             const int c = lane + i * TPR;
             p1[i] = p2[i] = 0.f;
-            if (!(in && c < nch)) {
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) d[i][j] = 0.f;
-                continue;
-            }
-            float w[VEC], t[VEC];
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) w[j] = 1.f;
-            if (a.w) load_row<VEC>(a.w, (long)c * VEC, w);
+            if (!(in && c < nch)) { fill<VEC>(d[i], 0.f); continue; }
+            if constexpr (!Columns<NI, VEC>::KEEP) col.load(a, (long)c * VEC, true);
             if constexpr (FULL) {
-                float n[VEC], gt[VEC], ga[VEC];
+                float t[VEC];
                 if (a.dres) {
 #pragma unroll
                     for (int j = 0; j < VEC; ++j) t[j] = a.alpha * d[i][j];
                     store_row<VEC>((T*)a.dres, at + (long)c * VEC, t);
                 }
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) { n[j] = y[i][j] * w[j]; ga[j] = 1.f; }
-                if (a.b) {
-                    load_row<VEC>(a.b, (long)c * VEC, t);
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) n[j] += t[j];
-                }
-                if (a.gate) {
-                    load_row<VEC>((const T*)a.gate, gat + (long)c * VEC, gt);
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) ga[j] = gate_act(gt[j], a.act);
-                }
                 if (a.s) {
-                    load_row<VEC>(a.s, (long)c * VEC, t);
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) { acc[2][i][j] += d[i][j] * (n[j] * ga[j]); d[i][j] *= t[j]; }
+                    for (int j = 0; j < VEC; ++j) { acc[2][i][j] += d[i][j] * (n[i][j] * ga[i][j]); d[i][j] *= col.s[j]; }
                 }
                 if (a.gate) {
 #pragma unroll
                     for (int j = 0; j < VEC; ++j) {
-                        t[j] = d[i][j] * n[j] * gate_act_d(gt[j], a.act);
+                        t[j] = d[i][j] * n[i][j] * gd[i][j];
                         acc[5][i][j] += t[j];
-                        d[i][j] *= ga[j];
+                        d[i][j] *= ga[i][j];
                     }
                     if (a.dgate && !a.gate_shared) store_row<VEC>((T*)a.dgate, at + (long)c * VEC, t);
                 }
@@ -379,10 +434,10 @@ __global__ __launch_bounds__(block_of<TPR>()) void tail_bwd_kernel(const TailArg
             if (a.w) {
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) {
-                    acc[0][i][j] += d[i][j] * y[i][j];
+                    acc[0][i][j] += d[i][j] * xh[i][j];
                     acc[1][i][j] += d[i][j];
-                    d[i][j] *= w[j];
-                    p1[i] += d[i][j] * y[i][j];
+                    d[i][j] *= col.w[j];
+                    p1[i] += d[i][j] * xh[i][j];
                     p2[i] += d[i][j];
                 }
             }
@@ -394,7 +449,7 @@ __global__ __launch_bounds__(block_of<TPR>()) void tail_bwd_kernel(const TailArg
 #pragma unroll
             for (int i = 0; i < NI; ++i)
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) d[i][j] = r[i] * (d[i][j] - y[i][j] * (c1[i] * inv) - (a.layer ? c2[i] * inv : 0.f));
+                for (int j = 0; j < VEC; ++j) d[i][j] = cur.rs[i] * (d[i][j] - xh[i][j] * (c1[i] * inv) - (a.layer ? c2[i] * inv : 0.f));
         }
         if (a.dy) {
 #pragma unroll
@@ -403,38 +458,37 @@ __global__ __launch_bounds__(block_of<TPR>()) void tail_bwd_kernel(const TailArg
                 if (in && c < nch) store_row<VEC>((T*)a.dy, at + (long)c * VEC, d[i]);
             }
         }
+        cur = nxt;
     }
     const bool have[6] = {a.w != nullptr, a.w != nullptr, a.s != nullptr, a.w2 != nullptr, a.w2 != nullptr, a.gate_shared && a.gpart};
     int nvec = 0, k = 0;
 #pragma unroll
-    for (int n = 0; n < 5; ++n) nvec += have[n];
+    for (int q = 0; q < 5; ++q) nvec += have[q];
     const long blk = (long)blockIdx.y * gridDim.x + blockIdx.x;
 #pragma unroll
-    for (int n = 0; n < NV; ++n) {
-        if (!have[n]) continue;
-        float* out = n == 5 ? a.gpart + blk * a.C : a.part + (blk * nvec + k) * a.C;
+    for (int q = 0; q < NV; ++q) {
+        if (!have[q]) continue;
+        float* out = q == 5 ? a.gpart + blk * a.C : a.part + (blk * nvec + k) * a.C;
         ++k;
-        if constexpr (RPB > 1) {                     // the block's rows in turn: the sums of its RPB rows meet in LDS, in the order of the rows
+        if constexpr (RPB > 1) {                     // the sums of the block's RPB rows meet in LDS, in the order of the rows
             __syncthreads();
 #pragma unroll
             for (int i = 0; i < NI; ++i) {
                 const int c = lane + i * TPR;
-                if (c < nch)
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) lds[(sub * NI * TPR + c) * VEC + j] = acc[n][i][j];
+                if (c < nch) store_row<VEC>(lds, (long)(sub * NI * TPR + c) * VEC, acc[q][i]);
             }
             __syncthreads();
             for (int c = threadIdx.x; c < a.C; c += RPB * TPR) {
                 float s = 0.f;
 #pragma unroll
-                for (int q = 0; q < RPB; ++q) s += lds[q * NI * TPR * VEC + c];
+                for (int z = 0; z < RPB; ++z) s += lds[z * NI * TPR * VEC + c];
                 out[c] = s;
             }
         } else {
 #pragma unroll
             for (int i = 0; i < NI; ++i) {
                 const int c = lane + i * TPR;
-                if (c < nch) store_row<VEC>(out, (long)c * VEC, acc[n][i]);
+                if (c < nch) store_row<VEC>(out, (long)c * VEC, acc[q][i]);
             }
         }
     }
@@ -466,20 +520,31 @@ __global__ __launch_bounds__(1024) void slab_sum_kernel(const float* __restrict_
     }
 }
 
-// threads per row and chunks per thread: a wave holds up to 1 024 values (256 one by one), 256 threads up to 4 096, a block of 1 024 the rest
+// Threads per row and chunks per thread: a wave alone up to 128 chunks, then one chunk per thread as far as 256 threads go, then two; the widest rows
+// take what the registers of 1 024 threads hold.
 #define TAIL_SHAPES(VEC, CASE)                                                                                                                     \
     {                                                                                                                                              \
         const int nch = a.C / VEC;                                                                                                                 \
         if (nch <= 64) CASE(64, 1, VEC)                                                                                                            \
         else if (nch <= 128) CASE(64, 2, VEC)                                                                                                      \
-        else if (nch <= 256) CASE(64, 4, VEC)                                                                                                      \
+        else if (nch <= 256) CASE(256, 1, VEC)                                                                                                     \
         else if (nch <= 512) CASE(256, 2, VEC)                                                                                                     \
-        else if (nch <= 1024) CASE(256, 4, VEC)                                                                                                    \
-        else if (nch <= 4096) CASE(1024, 4, VEC)                                                                                                   \
-        else CASE(1024, 8, VEC)                                                                                                                    \
+        else if (nch <= 1024) CASE(512, 2, VEC)                                                                                                    \
+        else if (nch <= 2048 || VEC == 8) CASE(1024, 2, VEC)                                                                                       \
+        else if (nch <= 4096 || VEC == 4) CASE(1024, 4, VEC == 8 ? 4 : VEC)                                                                        \
+        else CASE(1024, 8, 1)                                                                                                                      \
+    }
+#define TAIL_VECS(CASE)                                                                                                                            \
+    if constexpr (sizeof(T) == 2) {                                                                                                                \
+        if (vec == 8) TAIL_SHAPES(8, CASE)                                                                                                         \
+        else if (vec == 4) TAIL_SHAPES(4, CASE)                                                                                                    \
+        else TAIL_SHAPES(1, CASE)                                                                                                                  \
+    } else {                                                                                                                                       \
+        if (vec == 4) TAIL_SHAPES(4, CASE)                                                                                                         \
+        else TAIL_SHAPES(1, CASE)                                                                                                                  \
     }
 
-template <typename T> void tail_fwd_launch(const TailArgs& a, bool vec, hipStream_t st) {
+template <typename T> void tail_fwd_launch(const TailArgs& a, int vec, hipStream_t st) {
     const long rows = a.inner * a.outer;
 #define FWD_CASE(TPR, NI, VEC)                                                                                             \
     {                                                                                                                      \
@@ -487,23 +552,30 @@ template <typename T> void tail_fwd_launch(const TailArgs& a, bool vec, hipStrea
         const long want = (rows + rpb - 1) / rpb, cap = 8L * hw_cu_count();                                                \
         hipLaunchKernelGGL((tail_fwd_kernel<T, TPR, NI, VEC>), dim3((unsigned)(want < cap ? want : cap)), dim3(block_of<TPR>()), 0, st, a); \
     }
-    if (vec) TAIL_SHAPES(4, FWD_CASE)
-    else TAIL_SHAPES(1, FWD_CASE)
+    TAIL_VECS(FWD_CASE)
 #undef FWD_CASE
 }
-template <typename T> void tail_bwd_launch(const TailArgs& a, bool vec, int slices, hipStream_t st) {
+template <typename T> void tail_bwd_launch(const TailArgs& a, int vec, int slices, hipStream_t st) {
     const bool full = a.res || a.gate || a.s || a.w2 || !a.w;
 #define BWD_CASE(TPR, NI, VEC)                                                                                                                  \
     {                                                                                                                                           \
         if (full) hipLaunchKernelGGL((tail_bwd_kernel<T, TPR, NI, VEC, true>), dim3(slices, a.outer), dim3(block_of<TPR>()), 0, st, a);         \
         else hipLaunchKernelGGL((tail_bwd_kernel<T, TPR, NI, VEC, false>), dim3(slices, a.outer), dim3(block_of<TPR>()), 0, st, a);             \
     }
-    if (vec) TAIL_SHAPES(4, BWD_CASE)
-    else TAIL_SHAPES(1, BWD_CASE)
+    TAIL_VECS(BWD_CASE)
 #undef BWD_CASE
 }
 
-bool aligned(const void* p, size_t n) { return (uintptr_t)p % n == 0; }
+// values per access: 16 bytes' worth where groups and addresses allow it (bf16: or 8 bytes'), one otherwise
+int tail_vec(const TailArgs& a, int b16_io) {
+    const uintptr_t io = (uintptr_t)a.y | (uintptr_t)a.res | (uintptr_t)a.gate | (uintptr_t)a.h | (uintptr_t)a.z | (uintptr_t)a.dh | (uintptr_t)a.dz |
+                         (uintptr_t)a.dy | (uintptr_t)a.dres | (uintptr_t)a.dgate;
+    const uintptr_t par = (uintptr_t)a.w | (uintptr_t)a.b | (uintptr_t)a.s | (uintptr_t)a.w2 | (uintptr_t)a.b2 | (uintptr_t)a.part | (uintptr_t)a.gpart;
+    const int D = a.C / a.G;
+    if (par % 16 || D % 4) return 1;
+    if (b16_io) return D % 8 == 0 && io % 16 == 0 ? 8 : (io % 8 == 0 ? 4 : 1);
+    return io % 16 == 0 ? 4 : 1;
+}
 
 int tail_check(const char* what, const TailArgs& a) {
     HA2G_REQUIRE(a.C >= 1 && a.C <= 16384 && a.G >= 1 && a.C % a.G == 0, "%s: C=%d in %d groups (C <= 16384)", what, a.C, a.G);
@@ -519,7 +591,7 @@ extern "C" {
 // slices of a sequence's rows in the backward pass: ~2 blocks per compute unit over all sequences
 int ha2g_block_tail_slices(int outer, long inner, int C) {
     if (outer < 1 || inner < 1) return 1;
-    const long rpb = C <= 1024 ? 4 : 1;
+    const long rpb = C <= 512 ? 4 : 1;
     long s = (2L * hw_cu_count() + outer - 1) / outer;
     const long most = (inner + rpb - 1) / rpb;
     return (int)(s < 1 ? 1 : (s < most ? s : most));
@@ -535,10 +607,8 @@ int ha2g_block_tail_fwd(const void* y, const void* res, const void* gate, const 
     if (const int rc = tail_check("block_tail_fwd", a)) return rc;
     if (outer == 0 || inner == 0) return 0;
     HA2G_REQUIRE(y && h && (!w2 || z) && (!layer || !rs || mu) && (!layer || !rs2 || mu2), "block_tail_fwd: null operand");
-    const size_t e = b16_io ? 8 : 16;
-    const bool vec = (C / G) % 4 == 0 && aligned(y, e) && aligned(res, e) && aligned(gate, e) && aligned(h, e) && aligned(z, e) && aligned(w, 16) &&
-                     aligned(b, 16) && aligned(s, 16) && aligned(w2, 16) && aligned(b2, 16);
-    HA2G_REQUIRE(vec || C <= 8192, "block_tail_fwd: C=%d > 8192 needs groups of a multiple of 4 and 16-byte aligned operands", C);
+    const int vec = tail_vec(a, b16_io);
+    HA2G_REQUIRE(vec > 1 || C <= 8192, "block_tail_fwd: C=%d > 8192 needs groups of a multiple of 4 and 16-byte aligned operands", C);
     if (b16_io) tail_fwd_launch<b16>(a, vec, (hipStream_t)stream);
     else tail_fwd_launch<float>(a, vec, (hipStream_t)stream);
     HA2G_CHECK_LAUNCH("block_tail_fwd");
@@ -560,11 +630,8 @@ int ha2g_block_tail_bwd(const void* y, const void* res, const void* gate, const 
     const int nvec = (w ? 2 : 0) + (s ? 1 : 0) + (w2 ? 2 : 0);
     HA2G_REQUIRE(y && (!w || rs) && (!w2 || rs2) && (!layer || !w || mu) && (!layer || !w2 || mu2) && (nvec == 0 || (part && dparams)) &&
                  (!(gate && gate_shared) || (gpart && dgate)), "block_tail_bwd: null operand");
-    const size_t e = b16_io ? 8 : 16;
-    const bool vec = (C / G) % 4 == 0 && aligned(y, e) && aligned(res, e) && aligned(gate, e) && aligned(dh, e) && aligned(dz, e) && aligned(dy, e) &&
-                     aligned(dres, e) && aligned(dgate, e) && aligned(w, 16) && aligned(b, 16) && aligned(s, 16) && aligned(w2, 16) && aligned(b2, 16) &&
-                     aligned(part, 16) && aligned(gpart, 16);
-    HA2G_REQUIRE(vec || C <= 8192, "block_tail_bwd: C=%d > 8192 needs groups of a multiple of 4 and 16-byte aligned operands", C);
+    const int vec = tail_vec(a, b16_io);
+    HA2G_REQUIRE(vec > 1 || C <= 8192, "block_tail_bwd: C=%d > 8192 needs groups of a multiple of 4 and 16-byte aligned operands", C);
     const hipStream_t st = (hipStream_t)stream;
     if (b16_io) tail_bwd_launch<b16>(a, vec, slices, st);
     else tail_bwd_launch<float>(a, vec, slices, st);
