@@ -8,18 +8,24 @@
 
 namespace {
 
-struct LinAttnArgs {
-    const void *q, *k, *v;
+struct Operand { const void* p; long b, t, h; int r, vec; };      // element strides of batch row, token, head; head h reads head h / r; 16-byte pieces possible
+
+// one recurrence: reads q k v, adds k v^T, writes o
+struct Job {
+    Operand q, k, v;
     void* o;
-    const float* g;              // [H] log decay
-    const float* s_in;           // [B][H] states, strides s_h (one head), element (i, j) at i * s_i + j * s_j; nullptr = zero
-    float* s_out;                // the same layout as s_in, or nullptr
-    const int* lengths;          // [B] tokens of each sequence, or nullptr = T
-    long qb, qt, qh, kb, kt, kh, vb, vt, vh, ob, ot, oh;      // element strides of batch row, token and head (inner stride 1)
-    int B, T, H, Dk, Dv, rq, rk, rv;                          // head h reads head h / rq of q, h / rk of k, h / rv of v
-    int si, sj;
+    long ob, ot, oh;
+    const float* s_in;           // states in front of the first token, one after another for (b, h), element (i, j) at i * si + j * sj; nullptr = zero
+    float* s_out;                // those behind the last one, laid out alike, or nullptr
+    float* seg;                  // [B * H][nseg - 1] states between the segments, element (i, j) at i * gi + j * gj
+    int si, sj, gi, gj, Dk, Dv, rev, o16, ovec;
     float oscale, uscale;        // on what is read, on what is added
-    int rev;
+};
+struct LinAttnArgs {
+    Job job[3];
+    const float* g;              // [H] log decay
+    const int* lengths;          // [B] tokens of each sequence, or nullptr = T
+    int B, T, H, nseg, seg_len;  // segments of seg_len tokens (a multiple of the chunk)
 };
 
 template <typename T> __device__ __forceinline__ void st1(T* p, long i, float v);
@@ -31,7 +37,7 @@ template <> __device__ __forceinline__ void st1<b16>(b16* p, long i, float v) {
 }
 
 // ---- chunked form --------------------------------------------------------------------------------------------------------------------------
-// C tokens at a time (fp32: 32, bf16: 64), positions i, j inside the chunk, e = 1 forward and 0 from the end:
+// C tokens at a time (fp32: 32, bf16: 64; half of it for Dk > 64), positions i, j inside the chunk, e = 1 forward and 0 from the end:
 //     o_i = e^{g (i + e)} q_i S + sum_{j <= i} e^{g (i - j)} (q_i k_j) v_j,        S <- e^{g C} S + sum_j e^{g (C - e - j)} k_j v_j^T
 // A workgroup owns a (batch row, head, segment of the time axis); its waves split the columns of v, each keeps its Dk x DVW slice of S in MFMA
 // accumulators for the whole segment.  The accumulator layout (column = lane & 15, row = 4 (lane >> 4) + i) is that of an operand whose k runs along
@@ -50,7 +56,7 @@ typedef __attribute__((address_space(3))) s16x4_t* lds4_t;
 template <typename T> struct Mma;
 template <> struct Mma<float> {
     typedef f32x4 Frag;
-    static constexpr int C = 32, KB = 16, PADK = 16, NS = 1, NV = 1;      // chunk, k per fragment, LDS row padding, pieces of S / scores and of v
+    static constexpr int CMAX = 32, KB = 16, PADK = 16, NS = 1, NV = 1;      // longest chunk, k per fragment, LDS row padding, pieces of S / scores and of v
     // row m of a score tile is token 4 (m & 3) + (m >> 2): the column reads below then take four neighbouring rows at once, without bank conflicts
     __device__ __forceinline__ static int srow(int g, int i) { return 4 * i + g; }
     __device__ __forceinline__ static int krow(int m) { return 4 * (m & 3) + (m >> 2); }
@@ -74,7 +80,7 @@ template <> struct Mma<float> {
 };
 template <> struct Mma<b16> {
     typedef bf16x8_t Frag;
-    static constexpr int C = 64, KB = 32, PADK = 16, NS = 2, NV = 3;
+    static constexpr int CMAX = 64, KB = 32, PADK = 16, NS = 2, NV = 3;
     __device__ __forceinline__ static int srow(int g, int i) { return 4 * g + i; }
     __device__ __forceinline__ static int krow(int m) { return m; }
     __device__ __forceinline__ static f32x4 mma(Frag a, Frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
@@ -111,82 +117,94 @@ template <> struct Mma<b16> {
     }
 };
 
-// 16 bytes of a row: `left` elements of it exist; `vec`: rows are whole 16-byte pieces
-template <typename T> __device__ __forceinline__ u32x4_t load16(const T* p, bool vec, int left) {
+// 16 bytes of a row of which `left` elements exist; VEC: rows are whole 16-byte pieces
+template <typename T, bool VEC> __device__ __forceinline__ u32x4_t load16(const T* p, int left) {
     constexpr int E = 16 / sizeof(T);
     u32x4_t r = {0u, 0u, 0u, 0u};
-    if (left <= 0) return r;
-    if (vec) return *reinterpret_cast<const u32x4_t*>(p);
+    if constexpr (VEC) {
+        if (left > 0) r = *reinterpret_cast<const u32x4_t*>(p);
+    } else {
 #pragma unroll
-    for (int j = 0; j < E; ++j)
-        if (j < left) {
-            if constexpr (sizeof(T) == 4) r[j] = __float_as_uint(p[j]);
-            else r[j >> 1] |= (unsigned)p[j] << (16 * (j & 1));
-        }
+        for (int j = 0; j < E; ++j)
+            if (j < left) {
+                if constexpr (sizeof(T) == 4) r[j] = __float_as_uint(p[j]);
+                else r[j >> 1] |= (unsigned)p[j] << (16 * (j & 1));
+            }
+    }
     return r;
 }
 
-template <typename T, int D, int NT> struct Stage {            // a chunk of one operand: registers on the way from memory to LDS
-    static constexpr int E = 16 / sizeof(T), V = D / E, N = Mma<T>::C * V / NT, LD = D + Mma<T>::PADK;
-    static_assert(N * NT == Mma<T>::C * V, "a chunk is a whole number of pieces per thread");
+template <typename T, int D, int C, int NT, bool VEC> struct Stage {     // a chunk of one operand: registers on the way from memory to LDS
+    static constexpr int E = 16 / sizeof(T), V = D / E, N = C * V / NT, LD = D + Mma<T>::PADK, RS = NT / V;
+    static_assert(N * NT == C * V && RS * V == NT, "a chunk is a whole number of pieces per thread, a pass over the threads whole rows");
     u32x4_t r[N];
     // rows: token `first` and on in steps of `step` elements (negative from the end); n of them exist
-    __device__ __forceinline__ void load(const T* first, long step, int n, int dim, bool vec) {
+    __device__ __forceinline__ void load(const T* first, long step, int n, int dim) {
+        const int row = threadIdx.x / V, c = threadIdx.x % V * E, left = dim - c;
+        const T* p = first + row * step + c;
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const int x = threadIdx.x + j * NT, row = x / V, c = x % V * E;
-            r[j] = load16(first + row * step + c, vec, row < n ? dim - c : 0);
-        }
+        for (int j = 0; j < N; ++j) r[j] = load16<T, VEC>(p + (long)(j * RS) * step, row + j * RS < n ? left : 0);
     }
     __device__ __forceinline__ void store(T* lds) const {
+        T* p = lds + threadIdx.x / V * LD + threadIdx.x % V * E;
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const int x = threadIdx.x + j * NT;
-            *reinterpret_cast<u32x4_t*>(lds + x / V * LD + x % V * E) = r[j];
-        }
+        for (int j = 0; j < N; ++j) *reinterpret_cast<u32x4_t*>(p + j * RS * LD) = r[j];
     }
-};
-
-struct ChunkArgs {
-    LinAttnArgs a;
-    float* seg_state;            // [B * H][nseg - 1][Dk * Dv]: a segment's own contribution, after the scan the state that enters the next one
-    int nseg, seg_len;           // segments of seg_len tokens (a multiple of the chunk)
-    int vq, vk, vv, vo;          // 16-byte accesses possible
 };
 
 __device__ __forceinline__ float decay_power(float g, int n) { return n == 0 ? 1.f : expf(g * (float)n); }
+__device__ __forceinline__ int row_length(const LinAttnArgs& a, int b) { return a.lengths ? min(max(a.lengths[b], 0), a.T) : a.T; }
 
-// STATE_ONLY: the segment's own contribution to the state (from zero), nothing is read of q and no o is written
-template <typename T, typename TO, int DKP, int DVP, bool STATE_ONLY>
-__global__ __launch_bounds__((DVP < 64 ? DVP / 16 : 4) * 64) void linattn_chunk_kernel(const ChunkArgs ca) {
+// The workgroups of one XCD (every eighth) take neighbouring heads of the same tokens: rows of all heads lie together in memory, and heads that
+// share q, k or v find them in that XCD's L2.
+__device__ __forceinline__ long xcd_order(long i, long n) { return n % 8 == 0 ? i % 8 * (n / 8) + i / 8 : i; }
+
+constexpr int waves_of(int DVP) { return DVP < 64 ? DVP / 16 : 4; }
+// With Dk > 64 the state takes 64 registers of a wave: a chunk half as long leaves two waves per SIMD without spilling, and needs fewer score products.
+template <typename T> constexpr int chunk_of(int DKP) { return DKP > 64 ? Mma<T>::CMAX / 2 : Mma<T>::CMAX; }
+
+// STATE_ONLY: the segment's own contribution to the state (from zero), nothing is read of q and no o is written.  Two waves per SIMD at least:
+// one alone leaves matrix and vector units waiting for each other.
+template <typename T, int DKP, int DVP, bool STATE_ONLY, bool VEC>
+__global__ __launch_bounds__(waves_of(DVP) * 64, 2) void linattn_chunk_kernel(const LinAttnArgs a) {
     typedef Mma<T> M;
-    constexpr int NW = DVP < 64 ? DVP / 16 : 4, NT = NW * 64, DVW = DVP / NW, C = M::C, KB = M::KB, TPF = KB / 16;
+    constexpr int NW = waves_of(DVP), NT = NW * 64, DVW = DVP / NW, C = chunk_of<T>(DKP), KB = M::KB, TPF = KB / 16;
     constexpr int KT = DKP / 16, KF = DKP / KB, VT = DVW / 16, CT = C / 16, CF = C / KB;
-    const LinAttnArgs& a = ca.a;
-    typedef Stage<T, DKP, NT> SK;
-    typedef Stage<T, DVP, NT> SV;
+    const Job& J = a.job[blockIdx.y];
+    typedef Stage<T, DKP, C, NT, VEC> SK;
+    typedef Stage<T, DVP, C, NT, VEC> SV;
     __shared__ __attribute__((aligned(16))) T qs[STATE_ONLY ? 8 : C * SK::LD];
     __shared__ __attribute__((aligned(16))) T ks[C * SK::LD];
     __shared__ __attribute__((aligned(16))) T vs[C * SV::LD];
     const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4, v0 = (threadIdx.x >> 6) * DVW;
-    const int seg = blockIdx.x % ca.nseg, bh = blockIdx.x / ca.nseg, h = bh % a.H, b = bh / a.H;
-    const int n = a.lengths ? min(max(a.lengths[b], 0), a.T) : a.T;
-    const int beg = seg * ca.seg_len, end = min(n, beg + ca.seg_len);
-    if (STATE_ONLY && beg + ca.seg_len >= n) return;           // no token follows: the scan does not read it
+    const long wg = xcd_order(blockIdx.x, gridDim.x);
+    const int h = (int)(wg % a.H), seg = (int)(wg / a.H % a.nseg), b = (int)(wg / a.H / a.nseg);
+    const long bh = (long)b * a.H + h, D2 = (long)J.Dk * J.Dv;
+    const int n = row_length(a, b), beg = seg * a.seg_len, end = min(n, beg + a.seg_len);
+    if (STATE_ONLY && beg + a.seg_len >= n) return;             // no token follows: the scan does not read it
     const float g = a.g[h];
-    const int e = a.rev ? 0 : 1;
-    const long dir = a.rev ? -1 : 1, t0 = a.rev ? n - 1 : 0;    // position p is token t0 + dir p
-    const T* q = (const T*)a.q + (long)b * a.qb + (long)(h / a.rq) * a.qh + t0 * a.qt;
-    const T* k = (const T*)a.k + (long)b * a.kb + (long)(h / a.rk) * a.kh + t0 * a.kt;
-    const T* v = (const T*)a.v + (long)b * a.vb + (long)(h / a.rv) * a.vh + t0 * a.vt;
-    TO* o = (TO*)a.o + (long)b * a.ob + (long)h * a.oh;
-    const long qt = dir * a.qt, kt = dir * a.kt, vt = dir * a.vt;
+    const int e = J.rev ? 0 : 1;
+    const long dir = J.rev ? -1 : 1, t0 = J.rev ? n - 1 : 0;     // position p is token t0 + dir p
+    const T* q = (const T*)J.q.p + (long)b * J.q.b + (long)(h / J.q.r) * J.q.h + t0 * J.q.t;
+    const T* k = (const T*)J.k.p + (long)b * J.k.b + (long)(h / J.k.r) * J.k.h + t0 * J.k.t;
+    const T* v = (const T*)J.v.p + (long)b * J.v.b + (long)(h / J.v.r) * J.v.h + t0 * J.v.t;
+    const long qt = dir * J.q.t, kt = dir * J.k.t, vt = dir * J.v.t, obase = (long)b * J.ob + (long)h * J.oh;
+    const int Dk = J.Dk, Dv = J.Dv;
 
+    SK rq, rk;
+    SV rv;
+    if (beg < end) {
+        if constexpr (!STATE_ONLY) rq.load(q + beg * qt, qt, end - beg, Dk);
+        rk.load(k + beg * kt, kt, end - beg, Dk);
+        rv.load(v + beg * vt, vt, end - beg, Dv);
+    }
     f32x4 S[KT][VT];
-    const float* s_in = STATE_ONLY ? nullptr : (seg == 0 ? a.s_in : ca.seg_state + ((long)bh * (ca.nseg - 1) + seg - 1) * a.Dk * a.Dv);
-    const int si = seg == 0 ? a.si : a.Dv, sj = seg == 0 ? a.sj : 1;
-    if (s_in && seg == 0) s_in += (long)bh * a.Dk * a.Dv;
-    if (beg >= n && seg > 0) s_in = nullptr;                     // an empty segment: nothing is computed from it
+    const float* s_in = nullptr;
+    int si = J.si, sj = J.sj;
+    if constexpr (!STATE_ONLY) {
+        if (seg == 0) s_in = J.s_in ? J.s_in + bh * D2 : nullptr;
+        else if (beg < n) { s_in = J.seg + (bh * (a.nseg - 1) + seg - 1) * D2; si = J.gi; sj = J.gj; }      // an empty segment computes nothing from it
+    }
 #pragma unroll
     for (int x = 0; x < KT; ++x)
 #pragma unroll
@@ -194,38 +212,31 @@ __global__ __launch_bounds__((DVP < 64 ? DVP / 16 : 4) * 64) void linattn_chunk_
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int d = 16 * x + 4 * grp + i, j = v0 + 16 * y + col;
-                S[x][y][i] = (s_in && d < a.Dk && j < a.Dv) ? s_in[(long)d * si + (long)j * sj] : 0.f;
+                S[x][y][i] = (s_in && d < Dk && j < Dv) ? s_in[(long)d * si + (long)j * sj] : 0.f;
             }
 
-    // powers of the decay: inside a tile (t - s >= 0, else nothing), one tile further (t - s + 16 >= 1), and per tile
-    float pd[4], pb[4], ptile[CT], wst[CF][KB / 4], pi = 0.f;
+    // powers of the decay: inside a tile (t - s >= 0, else nothing), x tiles further (t - s + 16 x >= 1), in front of a tile of tokens, to the chunk's end
+    float pw[CT][4], pin[CT], wst[CF][KB / 4];
     if constexpr (!STATE_ONLY) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int d = col - M::srow(grp, i);
-            pd[i] = d >= 0 ? a.uscale * decay_power(g, d) : 0.f;
-            pb[i] = a.uscale * decay_power(g, 16 + d);
-        }
+        for (int x = 0; x < CT; ++x) {
 #pragma unroll
-        for (int x = 0; x < CT; ++x) ptile[x] = decay_power(g, 16 * x);
-        pi = decay_power(g, col + e);
+            for (int i = 0; i < 4; ++i) {
+                const int d = col - M::srow(grp, i) + 16 * x;
+                pw[x][i] = d >= 0 ? J.uscale * J.oscale * decay_power(g, d) : 0.f;
+            }
+            pin[x] = J.oscale * decay_power(g, col + 16 * x + e);
+        }
     }
     auto weights = [&](int L) {
 #pragma unroll
         for (int u = 0; u < CF; ++u)
 #pragma unroll
-            for (int j = 0; j < KB / 4; ++j) wst[u][j] = a.uscale * decay_power(g, max(0, L - e - (KB * u + 16 * (j >> 2) + M::srow(grp, j & 3))));
+            for (int j = 0; j < KB / 4; ++j) wst[u][j] = J.uscale * decay_power(g, max(0, L - e - (KB * u + 16 * (j >> 2) + M::srow(grp, j & 3))));
     };
     weights(C);
-    const float em1 = expm1f(g * (float)C);
+    float m1 = expm1f(g * (float)C);
 
-    SK rq, rk;
-    SV rv;
-    if (beg < end) {
-        if constexpr (!STATE_ONLY) rq.load(q + beg * qt, qt, end - beg, a.Dk, ca.vq);
-        rk.load(k + beg * kt, kt, end - beg, a.Dk, ca.vk);
-        rv.load(v + beg * vt, vt, end - beg, a.Dv, ca.vv);
-    }
     for (int c0 = beg; c0 < end; c0 += C) {
         __syncthreads();
         if constexpr (!STATE_ONLY) rq.store(qs);
@@ -234,9 +245,9 @@ __global__ __launch_bounds__((DVP < 64 ? DVP / 16 : 4) * 64) void linattn_chunk_
         __syncthreads();
         const int L = min(C, end - c0), c1 = c0 + C;
         if (c1 < end) {
-            if constexpr (!STATE_ONLY) rq.load(q + c1 * qt, qt, end - c1, a.Dk, ca.vq);
-            rk.load(k + c1 * kt, kt, end - c1, a.Dk, ca.vk);
-            rv.load(v + c1 * vt, vt, end - c1, a.Dv, ca.vv);
+            if constexpr (!STATE_ONLY) rq.load(q + c1 * qt, qt, end - c1, Dk);
+            rk.load(k + c1 * kt, kt, end - c1, Dk);
+            rv.load(v + c1 * vt, vt, end - c1, Dv);
         }
         typename M::Frag vf[CF][VT];
 #pragma unroll
@@ -271,18 +282,15 @@ __global__ __launch_bounds__((DVP < 64 ? DVP / 16 : 4) * 64) void linattn_chunk_
             }
 #pragma unroll
             for (int x = 0; x < CT; ++x) {
-                if (16 * x >= L) break;
-                const float f = pi * ptile[x];
 #pragma unroll
                 for (int y = 0; y < VT; ++y)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) acc[x][y][i] *= f;
+                    for (int i = 0; i < 4; ++i) acc[x][y][i] *= pin[x];
                 typename M::Frag qf[KF];
 #pragma unroll
                 for (int u = 0; u < KF; ++u) qf[u] = M::row(qs, SK::LD, 16 * x + col, u, grp);
 #pragma unroll
-                for (int u = 0; u < CF; ++u) {
-                    if (u * TPF > x) break;
+                for (int u = 0; u * TPF <= x; ++u) {
                     f32x4 t[TPF];
 #pragma unroll
                     for (int p = 0; p < TPF; ++p) {
@@ -292,7 +300,7 @@ __global__ __launch_bounds__((DVP < 64 ? DVP / 16 : 4) * 64) void linattn_chunk_
 #pragma unroll
                         for (int w = 0; w < KF; ++w) t[p] = M::mma(M::row(ks, SK::LD, 16 * s + M::krow(col), w, grp), qf[w], t[p]);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) t[p][i] *= s == x ? pd[i] : pb[i] * ptile[x - s > 0 ? x - s - 1 : 0];
+                        for (int i = 0; i < 4; ++i) t[p][i] *= pw[x - s][i];
                     }
                     typename M::Frag pf[M::NS];
                     M::template pieces<M::NS>(t, pf);
@@ -303,25 +311,25 @@ __global__ __launch_bounds__((DVP < 64 ? DVP / 16 : 4) * 64) void linattn_chunk_
                 }
                 const int r = 16 * x + col;
                 if (r < L) {
-                    TO* row = o + (t0 + dir * (c0 + r)) * a.ot;
+                    const long row = obase + (t0 + dir * (c0 + r)) * J.ot;
 #pragma unroll
                     for (int y = 0; y < VT; ++y) {
                         const int j = v0 + 16 * y + 4 * grp;
-                        const float4 w = make_float4(acc[x][y][0] * a.oscale, acc[x][y][1] * a.oscale, acc[x][y][2] * a.oscale, acc[x][y][3] * a.oscale);
-                        if (ca.vo) {
-                            if (j < a.Dv) st4(row + j, 0, w);
+                        const float4 w = make_float4(acc[x][y][0], acc[x][y][1], acc[x][y][2], acc[x][y][3]);
+                        if (j >= Dv) continue;
+                        if (J.ovec) {
+                            if (J.o16) st4((b16*)J.o + row + j, 0, w); else st4((float*)J.o + row + j, 0, w);
                         } else {
-                            if (j < a.Dv) st1(row, j, w.x);
-                            if (j + 1 < a.Dv) st1(row, j + 1, w.y);
-                            if (j + 2 < a.Dv) st1(row, j + 2, w.z);
-                            if (j + 3 < a.Dv) st1(row, j + 3, w.w);
+                            const float f[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                if (j + i < Dv) { if (J.o16) st1((b16*)J.o, row + j + i, f[i]); else st1((float*)J.o, row + j + i, f[i]); }
                         }
                     }
                 }
             }
         }
         // the state
-        float m1 = em1;
         if (L < C) {                                               // the last chunk of a row
             weights(L);
             m1 = expm1f(g * (float)L);
@@ -351,17 +359,21 @@ __global__ __launch_bounds__((DVP < 64 ? DVP / 16 : 4) * 64) void linattn_chunk_
             }
         }
     }
-    // behind the row's last token: o is zero
-    if constexpr (!STATE_ONLY) {
-        const int z0 = max(n, beg), z1 = min(a.T, beg + ca.seg_len);
-        for (long x = threadIdx.x; x < (long)max(0, z1 - z0) * a.Dv; x += NT) st1(o, (z0 + x / a.Dv) * a.ot + x % a.Dv, 0.f);
+    float* s_out;
+    int oi = J.si, oj = J.sj;
+    if constexpr (STATE_ONLY) {
+        s_out = J.seg + (bh * (a.nseg - 1) + seg) * D2;
+        oi = J.gi; oj = J.gj;
+    } else {
+        // behind the row's last token: o is zero
+        const int z0 = max(n, beg), zn = max(0, min(a.T, beg + a.seg_len) - z0);
+        for (long x = threadIdx.x; x < (long)zn * Dv; x += NT) {
+            const long at = obase + (z0 + x / Dv) * J.ot + x % Dv;
+            if (J.o16) ((b16*)J.o)[at] = 0; else ((float*)J.o)[at] = 0.f;
+        }
+        if (!J.s_out || seg != (n > 0 ? (n - 1) / a.seg_len : 0)) return;      // the segment with the row's last token
+        s_out = J.s_out + bh * D2;
     }
-    float* s_out = STATE_ONLY ? ca.seg_state + ((long)bh * (ca.nseg - 1) + seg) * a.Dk * a.Dv : a.s_out;
-    if (!STATE_ONLY) {
-        if (!s_out || seg != (n > 0 ? (n - 1) / ca.seg_len : 0)) return;      // the segment with the row's last token
-        s_out += (long)bh * a.Dk * a.Dv;
-    }
-    const int oi = STATE_ONLY ? a.Dv : a.si, oj = STATE_ONLY ? 1 : a.sj;
 #pragma unroll
     for (int x = 0; x < KT; ++x)
 #pragma unroll
@@ -369,27 +381,27 @@ __global__ __launch_bounds__((DVP < 64 ? DVP / 16 : 4) * 64) void linattn_chunk_
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int d = 16 * x + 4 * grp + i, j = v0 + 16 * y + col;
-                if (d < a.Dk && j < a.Dv) s_out[(long)d * oi + (long)j * oj] = S[x][y][i];
+                if (d < Dk && j < Dv) s_out[(long)d * oi + (long)j * oj] = S[x][y][i];
             }
 }
 
-// seg_state[i] <- the state behind segment i: one thread per element, the segments' own contributions loaded eight at a time
-__global__ __launch_bounds__(256) void linattn_segment_scan_kernel(const ChunkArgs ca) {
-    const LinAttnArgs& a = ca.a;
-    const int x = blockIdx.y * 256 + threadIdx.x, D = a.Dk * a.Dv, bh = blockIdx.x;
+// seg[i] <- the state behind segment i: one thread per element, the segments' own contributions loaded eight at a time
+__global__ __launch_bounds__(256) void linattn_segment_scan_kernel(const LinAttnArgs a) {
+    const Job& J = a.job[0];
+    const int x = blockIdx.y * 256 + threadIdx.x, D = J.Dk * J.Dv, bh = blockIdx.x;
     if (x >= D) return;
-    const int n = a.lengths ? min(max(a.lengths[bh / a.H], 0), a.T) : a.T;
+    const int n = row_length(a, bh / a.H);
     const float g = a.g[bh % a.H];
-    float* p = ca.seg_state + (long)bh * (ca.nseg - 1) * D + x;
-    float run = a.s_in ? a.s_in[(long)bh * D + (long)(x / a.Dv) * a.si + (long)(x % a.Dv) * a.sj] : 0.f;
-    const float em1 = expm1f(g * (float)ca.seg_len);
-    for (int i0 = 0; i0 < ca.nseg - 1; i0 += 8) {
+    float* p = J.seg + (long)bh * (a.nseg - 1) * D + x;
+    float run = J.s_in ? J.s_in[(long)bh * D + x] : 0.f;
+    const float em1 = expm1f(g * (float)a.seg_len);
+    for (int i0 = 0; i0 < a.nseg - 1; i0 += 8) {
         float y[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = (i0 + i < ca.nseg - 1 && (long)(i0 + i + 1) * ca.seg_len < n) ? p[(long)(i0 + i) * D] : 0.f;
+        for (int i = 0; i < 8; ++i) y[i] = (i0 + i < a.nseg - 1 && (long)(i0 + i + 1) * a.seg_len < n) ? p[(long)(i0 + i) * D] : 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            if (i0 + i >= ca.nseg - 1 || (long)(i0 + i + 1) * ca.seg_len >= n) return;      // what follows enters no token's segment
+            if (i0 + i >= a.nseg - 1 || (long)(i0 + i + 1) * a.seg_len >= n) return;      // what follows enters no token's segment
             run = __builtin_fmaf(run, em1, run) + y[i];
             p[(long)(i0 + i) * D] = run;
         }
@@ -400,30 +412,31 @@ __global__ __launch_bounds__(256) void linattn_segment_scan_kernel(const ChunkAr
 template <typename T>
 __global__ __launch_bounds__(256) void linattn_step_kernel(const LinAttnArgs a) {
     __shared__ float qs[128], ks[128], red[256];
+    const Job& J = a.job[0];
     const int h = blockIdx.x % a.H, b = blockIdx.x / a.H, tid = threadIdx.x;
-    const T* q = (const T*)a.q + (long)b * a.qb + (long)(h / a.rq) * a.qh;
-    const T* k = (const T*)a.k + (long)b * a.kb + (long)(h / a.rk) * a.kh;
-    const T* v = (const T*)a.v + (long)b * a.vb + (long)(h / a.rv) * a.vh;
-    if (tid < a.Dk) { qs[tid] = ld1(q, tid); ks[tid] = ld1(k, tid); }
+    const T* q = (const T*)J.q.p + (long)b * J.q.b + (long)(h / J.q.r) * J.q.h;
+    const T* k = (const T*)J.k.p + (long)b * J.k.b + (long)(h / J.k.r) * J.k.h;
+    const T* v = (const T*)J.v.p + (long)b * J.v.b + (long)(h / J.v.r) * J.v.h;
+    if (tid < J.Dk) { qs[tid] = ld1(q, tid); ks[tid] = ld1(k, tid); }
     __syncthreads();
     const float lam = expf(a.g[h]);
-    float* S = a.s_out + ((long)b * a.H + h) * a.Dk * a.Dv;
-    const int cols = a.Dv <= 32 ? 32 : (a.Dv <= 64 ? 64 : 128), groups = 256 / cols, j = tid % cols, r0 = tid / cols;
+    float* S = J.s_out + ((long)b * a.H + h) * J.Dk * J.Dv;
+    const int cols = J.Dv <= 32 ? 32 : (J.Dv <= 64 ? 64 : 128), groups = 256 / cols, j = tid % cols, r0 = tid / cols;
     float acc = 0.f;
-    if (j < a.Dv) {
+    if (j < J.Dv) {
         const float vv = ld1(v, j);
-        for (int d = r0; d < a.Dk; d += groups) {
-            const float s = lam * S[(long)d * a.Dv + j] + ks[d] * vv;
-            S[(long)d * a.Dv + j] = s;
+        for (int d = r0; d < J.Dk; d += groups) {
+            const float s = lam * S[(long)d * J.Dv + j] + ks[d] * vv;
+            S[(long)d * J.Dv + j] = s;
             acc += qs[d] * s;
         }
     }
     red[tid] = acc;
     __syncthreads();
-    if (tid < a.Dv) {
+    if (tid < J.Dv) {
         float s = 0.f;
         for (int r = 0; r < groups; ++r) s += red[r * cols + tid];
-        st1((T*)a.o + (long)b * a.ob + (long)h * a.oh, tid, s * a.oscale);
+        st1((T*)J.o + (long)b * J.ob + (long)h * J.oh, tid, s * J.oscale);
     }
 }
 
@@ -442,54 +455,80 @@ __global__ void head_sum_kernel(const float* __restrict__ x, T* __restrict__ out
 
 // Segments of the time axis: one pass over q, k, v where the rows and heads alone give every compute unit a workgroup or more; otherwise the axis is
 // split so that two are there, at no less than four chunks a segment, for a second read of k and v and the segments' states.
-void segments(int B, int T, int H, int b16_in, int* nseg, int* len) {
-    const int C = b16_in ? Mma<b16>::C : Mma<float>::C, chunks = (T + C - 1) / C, cus = hw_cu_count();
+void segments(int B, int T, int H, int b16_io, int* nseg, int* len) {
+    const int C = b16_io ? Mma<b16>::CMAX : Mma<float>::CMAX, chunks = (int)(((long)T + C - 1) / C), cus = hw_cu_count();
     const long rows = (long)B * H;
-    long want = rows >= cus ? 1 : (2L * cus + rows - 1) / (rows > 0 ? rows : 1);
+    long want = rows >= cus || rows < 1 ? 1 : (2L * cus + rows - 1) / rows;
     if (want > chunks / 4) want = chunks / 4;
     if (want < 1) want = 1;
-    const int per = (int)((chunks + want - 1) / want);
-    *nseg = per > 0 ? (chunks + per - 1) / per : 1;
-    if (*nseg < 1) *nseg = 1;
-    *len = (per > 0 ? per : 1) * C;
+    const int per = chunks > 0 ? (int)((chunks + want - 1) / want) : 1;
+    *nseg = chunks > 0 ? (chunks + per - 1) / per : 1;
+    *len = per * C;
 }
 
-template <typename T, typename TO, int DKP, int DVP> void chunk_launch(const ChunkArgs& c, hipStream_t st) {
-    constexpr int NT = (DVP < 64 ? DVP / 16 : 4) * 64;
-    const dim3 grid((unsigned)((long)c.a.B * c.a.H * c.nseg));
-    if (c.nseg > 1) {
-        hipLaunchKernelGGL((linattn_chunk_kernel<T, TO, DKP, DVP, true>), grid, dim3(NT), 0, st, c);
-        hipLaunchKernelGGL(linattn_segment_scan_kernel, dim3(c.a.B * c.a.H, (c.a.Dk * c.a.Dv + 255) / 256), dim3(256), 0, st, c);
+template <typename T, int DKP, int DVP> void chunk_launch(const LinAttnArgs& a, int jobs, bool state_only, hipStream_t st) {
+    const dim3 grid((unsigned)((long)a.B * a.H * a.nseg), jobs), block(waves_of(DVP) * 64);
+    bool vec = true;
+    for (int j = 0; j < jobs; ++j) vec = vec && a.job[j].q.vec && a.job[j].k.vec && a.job[j].v.vec;
+    if (state_only) {
+        if (vec) hipLaunchKernelGGL((linattn_chunk_kernel<T, DKP, DVP, true, true>), grid, block, 0, st, a);
+        else hipLaunchKernelGGL((linattn_chunk_kernel<T, DKP, DVP, true, false>), grid, block, 0, st, a);
+    } else {
+        if (vec) hipLaunchKernelGGL((linattn_chunk_kernel<T, DKP, DVP, false, true>), grid, block, 0, st, a);
+        else hipLaunchKernelGGL((linattn_chunk_kernel<T, DKP, DVP, false, false>), grid, block, 0, st, a);
     }
-    hipLaunchKernelGGL((linattn_chunk_kernel<T, TO, DKP, DVP, false>), grid, dim3(NT), 0, st, c);
 }
-template <typename T, typename TO, int DKP> void chunk_launch_v(const ChunkArgs& c, hipStream_t st) {
-    if (c.a.Dv <= 32) chunk_launch<T, TO, DKP, 32>(c, st);
-    else if (c.a.Dv <= 64) chunk_launch<T, TO, DKP, 64>(c, st);
-    else chunk_launch<T, TO, DKP, 128>(c, st);
+template <typename T, int DKP> void chunk_launch_v(const LinAttnArgs& a, int jobs, bool state_only, hipStream_t st) {
+    if (a.job[0].Dv <= 32) chunk_launch<T, DKP, 32>(a, jobs, state_only, st);
+    else if (a.job[0].Dv <= 64) chunk_launch<T, DKP, 64>(a, jobs, state_only, st);
+    else chunk_launch<T, DKP, 128>(a, jobs, state_only, st);
 }
-template <typename T, typename TO> void chunk_launch_k(const ChunkArgs& c, hipStream_t st) {
-    if (c.a.Dk <= 32) chunk_launch_v<T, TO, 32>(c, st);
-    else if (c.a.Dk <= 64) chunk_launch_v<T, TO, 64>(c, st);
-    else chunk_launch_v<T, TO, 128>(c, st);
+template <typename T> void chunk_launch_k(const LinAttnArgs& a, int jobs, bool state_only, hipStream_t st) {
+    if (a.job[0].Dk <= 32) chunk_launch_v<T, 32>(a, jobs, state_only, st);
+    else if (a.job[0].Dk <= 64) chunk_launch_v<T, 64>(a, jobs, state_only, st);
+    else chunk_launch_v<T, 128>(a, jobs, state_only, st);
 }
+// jobs of one size of Dk and Dv (up to their tiles) share a launch
+int run_chunks(const LinAttnArgs& a, int jobs, bool state_only, int b16_io, hipStream_t st) {
+    if (b16_io) chunk_launch_k<b16>(a, jobs, state_only, st);
+    else chunk_launch_k<float>(a, jobs, state_only, st);
+    HA2G_CHECK_LAUNCH("linattn");
+    return 0;
+}
+int run_scan(const LinAttnArgs& a, hipStream_t st) {
+    hipLaunchKernelGGL(linattn_segment_scan_kernel, dim3(a.B * a.H, (a.job[0].Dk * a.job[0].Dv + 255) / 256), dim3(256), 0, st, a);
+    HA2G_CHECK_LAUNCH("linattn: segments");
+    return 0;
+}
+int tile_of(int d) { return d <= 32 ? 32 : (d <= 64 ? 64 : 128); }
 
 // rows of D elements are whole pieces of `bytes`, also from one row to the next
-bool pieces_ok(const void* p, long b, long t, long h, int D, int elem, int bytes) {
-    return (uintptr_t)p % bytes == 0 && (long)D * elem % bytes == 0 && b * elem % bytes == 0 && t * elem % bytes == 0 && h * elem % bytes == 0;
+bool pieces_ok(const void* p, const long* s, int D, int elem, int bytes) {
+    return (uintptr_t)p % bytes == 0 && (long)D * elem % bytes == 0 && s[0] * elem % bytes == 0 && s[1] * elem % bytes == 0 && s[2] * elem % bytes == 0;
+}
+Operand operand(const void* p, const long* s, int r, int D, int elem) { return {p, s[0], s[1], s[2], r, pieces_ok(p, s, D, elem, 16)}; }
+
+void set_out(Job& j, void* o, const long* s, int o16) {
+    j.o = o; j.ob = s[0]; j.ot = s[1]; j.oh = s[2]; j.o16 = o16;
+    j.ovec = pieces_ok(o, s, j.Dv, o16 ? 2 : 4, o16 ? 8 : 16);
+}
+// one segment's worth of states lies as the forward pass has it, [Dk][Dv]; `turned` where the job's state is that transposed
+void set_state(Job& j, const float* s_in, float* s_out, float* seg, bool turned) {
+    j.s_in = s_in; j.s_out = s_out; j.seg = seg;
+    j.si = j.gi = turned ? 1 : j.Dv;
+    j.sj = j.gj = turned ? j.Dk : 1;
 }
 
-int fill_args(LinAttnArgs& a, const char* what, const void* q, const void* k, const void* v, void* o, const float* g, const long* strides, int B, int T,
-              int H, int rq, int rk, int rv, int Dk, int Dv) {
+int check_args(LinAttnArgs& a, const char* what, const float* g, const int* lengths, int B, int T, int H, int rq, int rk, int rv, int Dk, int Dv, int b16_io,
+               bool operands) {
     HA2G_REQUIRE(B >= 0 && T >= 0 && H >= 1 && Dk >= 1 && Dk <= 128 && Dv >= 1 && Dv <= 128, "%s: B=%d T=%d H=%d Dk=%d Dv=%d (1 <= Dk, Dv <= 128)", what, B,
                  T, H, Dk, Dv);
     HA2G_REQUIRE(rq >= 1 && rk >= 1 && rv >= 1 && H % rq == 0 && H % rk == 0 && H % rv == 0, "%s: %d heads shared by %d / %d / %d", what, H, rq, rk, rv);
-    HA2G_REQUIRE((long)B * H <= 0x7fffffffL, "%s: B * H = %ld", what, (long)B * H);
-    HA2G_REQUIRE(B == 0 || (g && (T == 0 || (q && k && v && o))), "%s: null operand", what);
-    a.q = q; a.k = k; a.v = v; a.o = o; a.g = g;
-    a.qb = strides[0]; a.qt = strides[1]; a.qh = strides[2]; a.kb = strides[3]; a.kt = strides[4]; a.kh = strides[5];
-    a.vb = strides[6]; a.vt = strides[7]; a.vh = strides[8]; a.ob = strides[9]; a.ot = strides[10]; a.oh = strides[11];
-    a.B = B; a.T = T; a.H = H; a.Dk = Dk; a.Dv = Dv; a.rq = rq; a.rk = rk; a.rv = rv;
+    HA2G_REQUIRE(B == 0 || (g && (T == 0 || operands)), "%s: null operand", what);
+    a.g = g; a.lengths = lengths; a.B = B; a.T = T; a.H = H;
+    segments(B, T, H, b16_io, &a.nseg, &a.seg_len);
+    HA2G_REQUIRE((long)B * H * a.nseg <= 0x7fffffffL, "%s: B * H * segments = %ld", what, (long)B * H * a.nseg);
+    HA2G_REQUIRE((long)T + a.seg_len <= 0x7fffffffL, "%s: T = %d", what, T);
     return 0;
 }
 
@@ -497,49 +536,83 @@ int fill_args(LinAttnArgs& a, const char* what, const void* q, const void* k, co
 
 extern "C" {
 
-long ha2g_linattn_workspace_floats(int B, int T, int H, int Dk, int Dv, int b16_in) {
+long ha2g_linattn_workspace_floats(int B, int T, int H, int Dk, int Dv, int b16_io) {
     int nseg, len;
     if (B < 1 || H < 1 || T < 1) return 0;
-    segments(B, T, H, b16_in, &nseg, &len);
+    segments(B, T, H, b16_io, &nseg, &len);
     return (long)B * H * (nseg - 1) * Dk * Dv;
 }
 
-int ha2g_linattn(const void* q, const void* k, const void* v, void* o, const float* log_decay, const float* s_in, float* s_out, const int* lengths,
-                 const long* strides, int B, int T, int H, int rq, int rk, int rv, int Dk, int Dv, int s_transposed, float o_scale, float u_scale,
-                 int reverse, int b16_in, int b16_out, float* ws, void* stream) {
-    ChunkArgs c;
-    LinAttnArgs& a = c.a;
-    if (const int rc = fill_args(a, "linattn", q, k, v, o, log_decay, strides, B, T, H, rq, rk, rv, Dk, Dv)) return rc;
+int ha2g_linattn_fwd(const void* q, const void* k, const void* v, void* o, const float* log_decay, const float* s_in, float* s_out, const int* lengths,
+                     const long* strides, int B, int T, int H, int rq, int rk, int rv, int Dk, int Dv, float scale, int b16_io, float* ws, void* stream) {
+    LinAttnArgs a;
+    if (const int rc = check_args(a, "linattn_fwd", log_decay, lengths, B, T, H, rq, rk, rv, Dk, Dv, b16_io, q && k && v && o)) return rc;
     if (B == 0) return 0;
-    a.s_in = s_in; a.s_out = s_out; a.lengths = lengths;
-    a.si = s_transposed ? 1 : Dv; a.sj = s_transposed ? Dk : 1;
-    a.oscale = o_scale; a.uscale = u_scale; a.rev = reverse;
+    HA2G_REQUIRE(a.nseg == 1 || ws, "linattn_fwd: no workspace (ha2g_linattn_workspace_floats)");
+    const int e = b16_io ? 2 : 4;
+    Job& j = a.job[0];
+    j.q = operand(q, strides, rq, Dk, e); j.k = operand(k, strides + 3, rk, Dk, e); j.v = operand(v, strides + 6, rv, Dv, e);
+    j.Dk = Dk; j.Dv = Dv; j.rev = 0; j.oscale = scale; j.uscale = 1.f;
+    set_out(j, o, strides + 9, b16_io);
+    set_state(j, s_in, s_out, ws, false);
     const hipStream_t st = (hipStream_t)stream;
-    HA2G_REQUIRE(b16_in || !b16_out, "linattn: fp32 operands with a bf16 result");
-    segments(B, T, H, b16_in, &c.nseg, &c.seg_len);
-    HA2G_REQUIRE(c.nseg == 1 || ws, "linattn: no workspace (ha2g_linattn_workspace_floats)");
-    HA2G_REQUIRE((long)B * H * c.nseg <= 0x7fffffffL, "linattn: B * H * segments = %ld", (long)B * H * c.nseg);
-    HA2G_REQUIRE((long)T + c.seg_len <= 0x7fffffffL, "linattn: T = %d", T);
-    c.seg_state = ws;
-    const int e = b16_in ? 2 : 4, eo = b16_out ? 2 : 4;
-    c.vq = pieces_ok(q, a.qb, a.qt, a.qh, Dk, e, 16);
-    c.vk = pieces_ok(k, a.kb, a.kt, a.kh, Dk, e, 16);
-    c.vv = pieces_ok(v, a.vb, a.vt, a.vh, Dv, e, 16);
-    c.vo = pieces_ok(o, a.ob, a.ot, a.oh, Dv, eo, 4 * eo);
-    if (!b16_in) chunk_launch_k<float, float>(c, st);
-    else if (b16_out) chunk_launch_k<b16, b16>(c, st);
-    else chunk_launch_k<b16, float>(c, st);
-    HA2G_CHECK_LAUNCH("linattn");
-    return 0;
+    if (a.nseg > 1) {
+        if (const int rc = run_chunks(a, 1, true, b16_io, st)) return rc;
+        if (const int rc = run_scan(a, st)) return rc;
+    }
+    return run_chunks(a, 1, false, b16_io, st);
+}
+
+int ha2g_linattn_bwd(const void* q, const void* k, const void* v, const void* dout, void* dq, void* dk, void* dv, const float* log_decay, const float* s_in,
+                     const float* ds_out, float* ds_in, const int* lengths, const long* strides, int B, int T, int H, int rq, int rk, int rv, int Dk, int Dv,
+                     float scale, int b16_io, int dq_b16, int dk_b16, int dv_b16, const float* ws_fwd, float* ws, void* stream) {
+    LinAttnArgs a;
+    if (const int rc = check_args(a, "linattn_bwd", log_decay, lengths, B, T, H, rq, rk, rv, Dk, Dv, b16_io, q && k && v && dout)) return rc;
+    HA2G_REQUIRE(B == 0 || dv || !ds_in || T == 0, "linattn_bwd: the gradient of the first state comes with dv");
+    if (B == 0) return 0;
+    HA2G_REQUIRE(a.nseg == 1 || (ws && (ws_fwd || !dq)), "linattn_bwd: no workspace (ha2g_linattn_workspace_floats)");
+    const int e = b16_io ? 2 : 4;
+    const Operand oq_ = operand(q, strides, rq, Dk, e), ok_ = operand(k, strides + 3, rk, Dk, e), ov_ = operand(v, strides + 6, rv, Dv, e),
+                  od_ = operand(dout, strides + 9, 1, Dv, e);
+    Job jv, jk, jq;
+    jv.q = ok_; jv.k = oq_; jv.v = od_; jv.Dk = Dk; jv.Dv = Dv; jv.rev = 1; jv.oscale = 1.f; jv.uscale = scale;
+    set_out(jv, dv, strides + 18, dv_b16);
+    set_state(jv, ds_out, ds_in, ws, false);
+    jk.q = ov_; jk.k = od_; jk.v = oq_; jk.Dk = Dv; jk.Dv = Dk; jk.rev = 1; jk.oscale = 1.f; jk.uscale = scale;
+    set_out(jk, dk, strides + 15, dk_b16);
+    set_state(jk, ds_out, nullptr, ws, true);
+    jq.q = od_; jq.k = ov_; jq.v = ok_; jq.Dk = Dv; jq.Dv = Dk; jq.rev = 0; jq.oscale = scale; jq.uscale = 1.f;
+    set_out(jq, dq, strides + 12, dq_b16);
+    set_state(jq, s_in, nullptr, const_cast<float*>(ws_fwd), true);
+    const hipStream_t st = (hipStream_t)stream;
+    if (a.nseg > 1 && (dv || dk)) {                      // both walk through the same states; dq through the forward pass's
+        a.job[0] = jv;
+        if (const int rc = run_chunks(a, 1, true, b16_io, st)) return rc;
+        if (const int rc = run_scan(a, st)) return rc;
+    }
+    const bool same = tile_of(Dk) == tile_of(Dv);
+    int n = 0;
+    if (dv || ds_in) a.job[n++] = jv;
+    if (!same && n) {
+        if (const int rc = run_chunks(a, n, false, b16_io, st)) return rc;
+        n = 0;
+    }
+    if (dk) a.job[n++] = jk;
+    if (dq) a.job[n++] = jq;
+    return n ? run_chunks(a, n, false, b16_io, st) : 0;
 }
 
 int ha2g_linattn_step(const void* q, const void* k, const void* v, void* o, const float* log_decay, float* state, const long* strides, int B, int H,
-                      int rq, int rk, int rv, int Dk, int Dv, float o_scale, int b16_io, void* stream) {
+                      int rq, int rk, int rv, int Dk, int Dv, float scale, int b16_io, void* stream) {
     LinAttnArgs a;
-    if (const int rc = fill_args(a, "linattn_step", q, k, v, o, log_decay, strides, B, 1, H, rq, rk, rv, Dk, Dv)) return rc;
-    HA2G_REQUIRE(B == 0 || state, "linattn_step: null state");
+    if (const int rc = check_args(a, "linattn_step", log_decay, nullptr, B, 1, H, rq, rk, rv, Dk, Dv, b16_io, q && k && v && o && state)) return rc;
     if (B == 0) return 0;
-    a.s_out = state; a.oscale = o_scale;
+    const int e = b16_io ? 2 : 4;
+    Job& j = a.job[0];
+    j.q = operand(q, strides, rq, Dk, e); j.k = operand(k, strides + 3, rk, Dk, e); j.v = operand(v, strides + 6, rv, Dv, e);
+    j.Dk = Dk; j.Dv = Dv; j.oscale = scale;
+    set_out(j, o, strides + 9, b16_io);
+    j.s_out = state;
     if (b16_io) hipLaunchKernelGGL(linattn_step_kernel<b16>, dim3(B * H), dim3(256), 0, (hipStream_t)stream, a);
     else hipLaunchKernelGGL(linattn_step_kernel<float>, dim3(B * H), dim3(256), 0, (hipStream_t)stream, a);
     HA2G_CHECK_LAUNCH("linattn_step");

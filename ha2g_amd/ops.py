@@ -4,6 +4,7 @@ hand-written backward kernels.  torch is used for device memory, streams and aut
 there is no fallback path -- every op here ends in a libha2g_hip.so call.
 """
 import os
+from array import array
 
 import torch
 
@@ -1911,18 +1912,35 @@ def _need(cond, msg, *args):
         raise ValueError('ha2g_amd: ' + msg % args)
 
 
+class _Here:
+    """no change of device (contextlib.nullcontext costs a microsecond of the call)"""
+
+    def __enter__(self):
+        pass
+
+    def __exit__(self, *exc):
+        pass
+
+
+_here = _Here()
+
+
 def _on(t):
     """launches go to the device their tensors live on, also where another one is current"""
-    return _null() if t.device.index == _cur_device() else torch.cuda.device(t.device)
+    return _here if t.device.index == _cur_device() else torch.cuda.device(t.device)
 
 
 def _inner1(x):
-    return x if x.shape[-1] == 1 or x.stride(-1) == 1 else x.contiguous()
+    return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
 
 
-def _la_check(what, q, k, v, log_decay, state, nd):
+_FLOATS = (torch.float32, torch.bfloat16)
+
+
+def _la_refuse(what, q, k, v, log_decay, state, nd):
+    """names what _la_check found"""
     for n, x in (('q', q), ('k', k), ('v', v)):
-        _need(x.dim() == nd and x.dtype in (torch.float32, torch.bfloat16) and x.dtype == q.dtype and x.device == q.device,
+        _need(x.dim() == nd and x.dtype in _FLOATS and x.dtype == q.dtype and x.device == q.device,
               '%s: %s is %s %s: %d dimensions, fp32 or bf16, all alike', what, n, x.dtype, tuple(x.shape), nd)
     _need(q.shape[:-2] == k.shape[:-2] == v.shape[:-2], '%s: q %s, k %s, v %s', what, tuple(q.shape), tuple(k.shape), tuple(v.shape))
     H, Dk, Dv = log_decay.numel(), q.shape[-1], v.shape[-1]
@@ -1932,81 +1950,87 @@ def _la_check(what, q, k, v, log_decay, state, nd):
     _need(not log_decay.requires_grad, '%s: the decays are constants (no gradient)', what)
     _need(H >= 1 and all(x.shape[-2] >= 1 and H % x.shape[-2] == 0 for x in (q, k, v)), '%s: %d / %d / %d heads do not divide %d decays', what, q.shape[-2],
           k.shape[-2], v.shape[-2], H)
-    if state is not None:
-        _need(state.shape == (q.shape[0], H, Dk, Dv) and state.dtype == torch.float32 and state.device == q.device,
-              '%s: state is fp32 [%d, %d, %d, %d], got %s %s', what, q.shape[0], H, Dk, Dv, state.dtype, tuple(state.shape))
+    _need(state is None or (state.shape == (q.shape[0], H, Dk, Dv) and state.dtype == torch.float32 and state.device == q.device),
+          '%s: state is fp32 [%d, %d, %d, %d]', what, q.shape[0], H, Dk, Dv)
     _need(q.is_cuda, '%s: GPU tensors (there is no CPU path)', what)
-    return H
+    raise AssertionError(what)
 
 
-def _la_strides(*ts):
-    import array
-    return array.array('l', [s for t in ts for s in (t.stride() if t.dim() == 4 else (t.stride(0), 0, t.stride(1)))[:3]])
+def _la_check(what, q, k, v, log_decay, state, nd):
+    """-> H, Dk, Dv.  A call costs as much as a small kernel: one expression for the good case, the reasons apart."""
+    qs, ks, vs, gs, dt, dev = q.shape, k.shape, v.shape, log_decay.shape, q.dtype, q.device
+    if not (len(qs) == len(ks) == len(vs) == nd and len(gs) == 1 and dt in _FLOATS and k.dtype == dt and v.dtype == dt and
+            log_decay.dtype == torch.float32 and k.device == dev and v.device == dev and log_decay.device == dev and q.is_cuda):
+        _la_refuse(what, q, k, v, log_decay, state, nd)
+    H, Dk, Dv = gs[0], qs[-1], vs[-1]
+    if not (qs[:-2] == ks[:-2] == vs[:-2] and ks[-1] == Dk and 1 <= Dk <= 128 and 1 <= Dv <= 128 and H and qs[-2] and ks[-2] and vs[-2] and
+            H % qs[-2] == H % ks[-2] == H % vs[-2] == 0 and log_decay.is_contiguous() and not log_decay.requires_grad and
+            (state is None or (state.shape == (qs[0], H, Dk, Dv) and state.dtype == torch.float32 and state.device == dev))):
+        _la_refuse(what, q, k, v, log_decay, state, nd)
+    return H, Dk, Dv
 
 
-def _la_call(q, k, v, o, log_decay, s_in, s_out, lengths, transposed, o_scale, u_scale, reverse):
-    B, T, H = q.shape[0], q.shape[1], log_decay.numel()
+def _la_forward(q, k, v, log_decay, scale, state, lengths, want_state):
+    B, T, Hq, Dk = q.shape
+    H, Hk, Hv, Dv = log_decay.shape[0], k.shape[2], v.shape[2], v.shape[3]
+    dev, bf = q.device, q.dtype == torch.bfloat16
     q, k, v = _inner1(q), _inner1(k), _inner1(v)
-    bf = int(q.dtype == torch.bfloat16)
-    n = lib.ha2g_linattn_workspace_floats(B, T, H, q.shape[3], v.shape[3], bf)
-    ws = torch.empty(n, dtype=torch.float32, device=q.device) if n else None
-    check(lib.ha2g_linattn(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), log_decay.data_ptr(), _p(s_in), _p(s_out), _p(lengths),
-                           _la_strides(q, k, v, o), B, T, H, H // q.shape[2], H // k.shape[2], H // v.shape[2], q.shape[3], v.shape[3], int(transposed),
-                           o_scale, u_scale, int(reverse), bf, int(o.dtype == torch.bfloat16), _p(ws), _stream()))
-
-
-def _la_grad(like, H, dtype):
-    """gradient buffer of an operand with like.shape[2] heads: per-head sums in fp32 first where several heads read one"""
-    B, T, Hx, D = like.shape
-    return torch.empty(B, T, H, D, dtype=dtype if Hx == H else torch.float32, device=like.device)
+    with _on(q):
+        o = torch.empty((B, T, H, Dv), dtype=q.dtype, device=dev)
+        s = torch.empty((B, H, Dk, Dv), dtype=torch.float32, device=dev) if want_state else None
+        n = lib.ha2g_linattn_workspace_floats(B, T, H, Dk, Dv, bf)
+        ws = torch.empty(n, dtype=torch.float32, device=dev) if n else None
+        check(lib.ha2g_linattn_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), log_decay.data_ptr(), _p(state), _p(s), _p(lengths),
+                                   array('l', q.stride()[:3] + k.stride()[:3] + v.stride()[:3] + (T * H * Dv, H * Dv, Dv)), B, T, H, H // Hq, H // Hk, H // Hv,
+                                   Dk, Dv, scale, bf, _p(ws), _stream()))
+    return o, s, ws
 
 
 def _la_share(d, like):
+    """gradients of heads that share an operand: added up in the order of the heads"""
     B, T, Hx, D = like.shape
-    if d.shape[2] == Hx:
+    if d is None or d.shape[2] == Hx:
         return d
-    out = torch.empty(B, T, Hx, D, dtype=like.dtype, device=like.device)
-    check(lib.ha2g_head_sum(d.data_ptr(), out.data_ptr(), B * T, Hx, d.shape[2] // Hx, D, int(out.dtype == torch.bfloat16), _stream()))
+    out = torch.empty((B, T, Hx, D), dtype=like.dtype, device=like.device)
+    check(lib.ha2g_head_sum(d.data_ptr(), out.data_ptr(), B * T, Hx, d.shape[2] // Hx, D, out.dtype == torch.bfloat16, _stream()))
     return out
 
 
 class LinearAttentionFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, log_decay, scale, state, lengths, want_state):
-        B, T, H = q.shape[0], q.shape[1], log_decay.numel()
         ctx.set_materialize_grads(False)
-        with _on(q):
-            o = torch.empty(B, T, H, v.shape[3], dtype=v.dtype, device=q.device)
-            s = torch.empty(B, H, q.shape[3], v.shape[3], dtype=torch.float32, device=q.device) if want_state else None
-            _la_call(q, k, v, o, log_decay, state, s, lengths, False, scale, 1.0, False)
+        o, s, ws = _la_forward(q, k, v, log_decay, scale, state, lengths, want_state)
         ctx.scale = scale
-        ctx.save_for_backward(q, k, v, log_decay, state, lengths)
+        ctx.save_for_backward(q, k, v, log_decay, state, lengths, ws)
         return o, s
 
     @staticmethod
     def backward(ctx, do, ds):
-        q, k, v, g, state, lengths = ctx.saved_tensors
-        H, scale = g.numel(), ctx.scale
+        q, k, v, g, state, lengths, ws_fwd = ctx.saved_tensors
+        (B, T, Hq, Dk), H, Hk, Hv, Dv = q.shape, g.shape[0], k.shape[2], v.shape[2], v.shape[3]
+        need, dev, dt = ctx.needs_input_grad, q.device, q.dtype
+        bf = dt == torch.bfloat16
         with _on(q):
             if do is None:
-                do = torch.zeros(1, 1, 1, v.shape[3], dtype=v.dtype, device=q.device).expand(q.shape[0], q.shape[1], H, -1)
+                do = torch.zeros((1, 1, 1, Dv), dtype=dt, device=dev).expand(B, T, H, Dv)
             if ds is not None:
                 ds = ds.contiguous()
-            dq = dk = dv = dstate = None
-            if ctx.needs_input_grad[0]:
-                dq = _la_grad(q, H, q.dtype)
-                _la_call(do, v, k, dq, g, state, None, lengths, True, scale, 1.0, False)
-                dq = _la_share(dq, q)
-            if ctx.needs_input_grad[1]:
-                dk = _la_grad(k, H, k.dtype)
-                _la_call(v, do, q, dk, g, ds, None, lengths, True, 1.0, scale, True)
-                dk = _la_share(dk, k)
-            if ctx.needs_input_grad[2] or ctx.needs_input_grad[5]:
-                dv = _la_grad(v, H, v.dtype)
-                if ctx.needs_input_grad[5]:
-                    dstate = torch.empty(q.shape[0], H, q.shape[3], v.shape[3], dtype=torch.float32, device=q.device)
-                _la_call(k, q, do, dv, g, ds, dstate, lengths, False, 1.0, scale, True)
-                dv = _la_share(dv, v) if ctx.needs_input_grad[2] else None
+            q, k, v, do = _inner1(q), _inner1(k), _inner1(v), _inner1(do)
+
+            def grad(Hx, D):                # per-head sums in fp32 first where several heads read one
+                return torch.empty((B, T, H, D), dtype=dt if Hx == H else torch.float32, device=dev)
+            dq = grad(Hq, Dk) if need[0] else None
+            dk = grad(Hk, Dk) if need[1] else None
+            dv = grad(Hv, Dv) if need[2] or need[5] else None
+            dstate = torch.empty((B, H, Dk, Dv), dtype=torch.float32, device=dev) if need[5] else None
+            ws = None if ws_fwd is None else torch.empty_like(ws_fwd)
+            rk, rv = (T * H * Dk, H * Dk, Dk), (T * H * Dv, H * Dv, Dv)
+            check(lib.ha2g_linattn_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), do.data_ptr(), _p(dq), _p(dk), _p(dv), g.data_ptr(), _p(state), _p(ds),
+                                       _p(dstate), _p(lengths), array('l', q.stride()[:3] + k.stride()[:3] + v.stride()[:3] + do.stride()[:3] + rk + rk + rv),
+                                       B, T, H, H // Hq, H // Hk, H // Hv, Dk, Dv, ctx.scale, bf, bf and Hq == H, bf and Hk == H, bf and Hv == H, _p(ws_fwd),
+                                       _p(ws), _stream()))
+            dq, dk, dv = _la_share(dq, q), _la_share(dk, k), _la_share(dv, v) if need[2] else None
         return dq, dk, dv, None, None, dstate, None, None
 
 
@@ -2018,26 +2042,35 @@ def linear_attention(q, k, v, log_decay, scale=None, state=None, lengths=None, r
     state [B, H, Dk, Dv] fp32: what stands before the first token (None: zero).  lengths [B] int32 on the device: row b ends after lengths[b]
     tokens (clipped to 0 .. T); what lies behind is not read, the output and the gradients there are zero.
     Returns o [B, T, H, Dv] in v's type, with return_state also the state behind each row's last token, fp32."""
-    _la_check('linear_attention', q, k, v, log_decay, state, 4)
-    _need(lengths is None or (lengths.shape == (q.shape[0],) and lengths.dtype == torch.int32 and lengths.device == q.device and lengths.is_contiguous()),
-          'linear_attention: lengths is int32 [%d] on the device of q', q.shape[0])
-    scale = float(q.shape[3] ** -0.5 if scale is None else scale)
-    o, s = LinearAttentionFunction.apply(q, k, v, log_decay, scale, None if state is None else state.contiguous(), lengths, bool(return_state))
+    _, Dk, _ = _la_check('linear_attention', q, k, v, log_decay, state, 4)
+    if lengths is not None:
+        _need(lengths.shape == (q.shape[0],) and lengths.dtype == torch.int32 and lengths.device == q.device and lengths.is_contiguous(),
+              'linear_attention: lengths is int32 [%d] on the device of q', q.shape[0])
+    scale = float(Dk ** -0.5 if scale is None else scale)
+    if state is not None:
+        state = state.contiguous()
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (state is not None and state.requires_grad)):
+        o, s = LinearAttentionFunction.apply(q, k, v, log_decay, scale, state, lengths, bool(return_state))
+    else:
+        o, s, _ = _la_forward(q, k, v, log_decay, scale, state, lengths, return_state)
     return (o, s) if return_state else o
 
 
 def linear_attention_step(q, k, v, log_decay, state, scale=None):
     """One token of linear_attention: q [B, Hq, Dk], k [B, Hk, Dk], v [B, Hv, Dv] -> o [B, H, Dv]; `state` (fp32, contiguous) is updated in place.
     For generation: no gradient passes through it."""
-    H = _la_check('linear_attention_step', q, k, v, log_decay, state, 3)
-    _need(state is not None and state.is_contiguous(), 'linear_attention_step: needs a contiguous state')
-    _need(not (torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, state))), 'linear_attention_step: no gradient (use linear_attention)')
+    H, Dk, Dv = _la_check('linear_attention_step', q, k, v, log_decay, state, 3)
+    if state is None or not state.is_contiguous():
+        raise ValueError('ha2g_amd: linear_attention_step: needs a contiguous state')
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad):
+        raise ValueError('ha2g_amd: linear_attention_step: no gradient (use linear_attention)')
     q, k, v = _inner1(q), _inner1(k), _inner1(v)
+    B, (qb, qh, _), (kb, kh, _), (vb, vh, _) = q.shape[0], q.stride(), k.stride(), v.stride()
     with _on(q):
-        o = torch.empty(q.shape[0], H, v.shape[2], dtype=v.dtype, device=q.device)
-        check(lib.ha2g_linattn_step(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), log_decay.data_ptr(), state.data_ptr(), _la_strides(q, k, v, o),
-                                    q.shape[0], H, H // q.shape[1], H // k.shape[1], H // v.shape[1], q.shape[2], v.shape[2],
-                                    float(q.shape[2] ** -0.5 if scale is None else scale), int(q.dtype == torch.bfloat16), _stream()))
+        o = torch.empty((B, H, Dv), dtype=q.dtype, device=q.device)
+        check(lib.ha2g_linattn_step(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), log_decay.data_ptr(), state.data_ptr(),
+                                    array('l', (qb, 0, qh, kb, 0, kh, vb, 0, vh, H * Dv, 0, Dv)), B, H, H // q.shape[1], H // k.shape[1], H // v.shape[1], Dk, Dv,
+                                    float(Dk ** -0.5 if scale is None else scale), q.dtype == torch.bfloat16, _stream()))
     torch.autograd.graph.increment_version(state)
     return o
 
@@ -2049,37 +2082,48 @@ def linear_attention_step(q, k, v, log_decay, state, scale=None):
 _NORMS = ('rms', 'layer')
 
 
+def _tail_forward(y, res, gate, w, b, s, w2, b2, groups, layer, act, alpha, eps, keep):
+    """-> h, z, the contiguous operands, and with `keep` the statistics in one tensor: mu, rs per group, then mu2, rs2 per row (those there are)"""
+    C = y.shape[-1]
+    y, res, gate, w, b, s, w2, b2 = ops = [None if t is None else t.contiguous() for t in (y, res, gate, w, b, s, w2, b2)]
+    rows, dev = y.numel() // C, y.device
+    shared = gate is not None and gate.shape != y.shape
+    outer, inner = (y.shape[0], rows // max(y.shape[0], 1)) if shared else (1, rows)
+    st = None
+    mu = rs = mu2 = rs2 = 0
+    with _on(y):
+        h = torch.empty_like(y)
+        z = None if w2 is None else torch.empty_like(y)
+        if keep and (w is not None or w2 is not None):
+            n1, n2 = (rows * groups if w is not None else 0), (rows if w2 is not None else 0)
+            st = torch.empty((n1 + n2) << layer, dtype=torch.float32, device=dev)
+            mu, rs, mu2, rs2 = _tail_stats(st, n1, n2, layer)
+        check(lib.ha2g_block_tail_fwd(y.data_ptr(), _p(res), _p(gate), _p(w), _p(b), _p(s), _p(w2), _p(b2), h.data_ptr(), _p(z), mu, rs, mu2, rs2, outer, inner,
+                                      shared, C, groups, layer, act, alpha, eps, y.dtype == torch.bfloat16, _stream()))
+    return h, z, ops, st, (outer, inner, shared, C, groups, layer, act, alpha, eps)
+
+
+def _tail_stats(st, n1, n2, layer):
+    """addresses of mu, rs [n1] and mu2, rs2 [n2] in st (0: absent)"""
+    p = st.data_ptr()
+    rs, rs2 = p, p + 4 * n1
+    mu, mu2 = (rs2 + 4 * n2, rs2 + 4 * (n2 + n1)) if layer else (0, 0)
+    return (mu if n1 else 0), (rs if n1 else 0), (mu2 if n2 else 0), (rs2 if n2 else 0)
+
+
 class BlockTailFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, res, gate, w, b, s, w2, b2, groups, layer, act, alpha, eps):
         ctx.set_materialize_grads(False)
-        C = y.shape[-1]
-        c = lambda t: None if t is None else t.contiguous()      # noqa: E731
-        y, res, gate, w, b, s, w2, b2 = (c(t) for t in (y, res, gate, w, b, s, w2, b2))
-        rows = y.numel() // C
-        shared = gate is not None and gate.shape != y.shape
-        outer, inner = (y.shape[0], rows // max(y.shape[0], 1)) if shared else (1, rows)
-        keep = any(ctx.needs_input_grad)
-
-        def stat(n, want=True):
-            return torch.empty(n, dtype=torch.float32, device=y.device) if keep and want else None
-        with _on(y):
-            h = torch.empty_like(y)
-            z = torch.empty_like(y) if w2 is not None else None
-            mu, rs = stat(rows * groups, layer and w is not None), stat(rows * groups, w is not None)
-            mu2, rs2 = stat(rows, layer and w2 is not None), stat(rows, w2 is not None)
-            check(lib.ha2g_block_tail_fwd(y.data_ptr(), _p(res), _p(gate), _p(w), _p(b), _p(s), _p(w2), _p(b2), h.data_ptr(), _p(z), _p(mu), _p(rs),
-                                          _p(mu2), _p(rs2), outer, inner, int(shared), C, groups, int(layer), act, alpha, eps,
-                                          int(y.dtype == torch.bfloat16), _stream()))
-        ctx.shape = outer, inner, shared, C, groups, layer, act, alpha, eps
-        ctx.save_for_backward(y, res, gate, w, b, s, w2, b2, mu, rs, mu2, rs2)
+        h, z, ops, st, ctx.shape = _tail_forward(y, res, gate, w, b, s, w2, b2, groups, layer, act, alpha, eps, True)
+        ctx.save_for_backward(*ops, st)
         return h, z
 
     @staticmethod
     def backward(ctx, dh, dz):
-        y, res, gate, w, b, s, w2, b2, mu, rs, mu2, rs2 = ctx.saved_tensors
+        y, res, gate, w, b, s, w2, b2, st = ctx.saved_tensors
         outer, inner, shared, C, groups, layer, act, alpha, eps = ctx.shape
-        need = ctx.needs_input_grad
+        need, dev, rows = ctx.needs_input_grad, y.device, outer * inner
         dh, dz = (None if t is None else t.contiguous() for t in (dh, dz))
         with _on(y):
             dy = torch.empty_like(y) if need[0] else None
@@ -2087,40 +2131,67 @@ class BlockTailFunction(torch.autograd.Function):
             dgate = torch.empty_like(gate) if gate is not None and (need[2] or shared) else None
             nvec = 2 * (w is not None) + (s is not None) + 2 * (w2 is not None)
             n = lib.ha2g_block_tail_slices(outer, inner, C)
-            ws = torch.empty(max(1, n * outer * (nvec + int(shared)) * C), dtype=torch.float32, device=y.device)
-            # no rows: the sums over them are zero
-            dp = (torch.empty if y.numel() else torch.zeros)(nvec, C, dtype=torch.float32, device=y.device)
-            if y.numel() == 0 and dgate is not None:
-                dgate.zero_()
-            check(lib.ha2g_block_tail_bwd(y.data_ptr(), _p(res), _p(gate), _p(w), _p(b), _p(s), _p(w2), _p(b2), _p(mu), _p(rs), _p(mu2), _p(rs2),
-                                          _p(dh), _p(dz), _p(dy), _p(dres), _p(dgate), ws.data_ptr(), ws.data_ptr() + 4 * n * outer * nvec * C if shared else 0,
-                                          dp.data_ptr(), n, outer, inner, int(shared), C, groups, int(layer), act, alpha, eps,
-                                          int(y.dtype == torch.bfloat16), _stream()))
-        it = iter(dp)
-        dw, db = (next(it), next(it)) if w is not None else (None, None)
-        dsc = next(it) if s is not None else None
-        dw2, db2 = (next(it), next(it)) if w2 is not None else (None, None)
-        return (dy, dres, dgate if need[2] else None, dw, db if b is not None else None, dsc, dw2, db2 if b2 is not None else None) + (None,) * 5
+            slabs = n * outer * C
+            dp = torch.empty(nvec * C, dtype=torch.float32, device=dev)
+            ws = torch.empty(slabs * (nvec + shared) + 4, dtype=torch.float32, device=dev)
+            part = ws.data_ptr()
+            mu, rs, mu2, rs2 = _tail_stats(st, rows * groups if w is not None else 0, rows if w2 is not None else 0, layer) if st is not None else (0, 0, 0, 0)
+            if rows == 0:                # no rows: the sums over them are zero
+                dp.zero_()
+                if dgate is not None:
+                    dgate.zero_()
+            check(lib.ha2g_block_tail_bwd(y.data_ptr(), _p(res), _p(gate), _p(w), _p(b), _p(s), _p(w2), _p(b2), mu, rs, mu2, rs2, _p(dh), _p(dz), _p(dy),
+                                          _p(dres), _p(dgate), part, part + 4 * ((slabs * nvec + 3) // 4 * 4) if shared else 0, dp.data_ptr(), n, outer, inner,
+                                          shared, C, groups, layer, act, alpha, eps, y.dtype == torch.bfloat16, _stream()))
+            grads, at = [None] * 5, 0
+            for i, (t, there) in enumerate(((w, w), (b, w), (s, s), (w2, w2), (b2, w2))):
+                if there is not None:
+                    if t is not None and need[3 + i]:
+                        grads[i] = dp[at:at + C]
+                    at += C
+        return (dy, dres, dgate if need[2] else None, *grads, None, None, None, None, None)
 
 
-def _norm_check(what, y, groups, kind, vectors):
-    _need(y.dim() >= 1 and y.dtype in (torch.float32, torch.bfloat16) and 1 <= y.shape[-1] <= 16384, '%s: fp32 or bf16 rows of 1 to 16384 values, got %s %s',
-          what, y.dtype, tuple(y.shape))
+def _norm_refuse(what, y, groups, kind, vectors):
+    """names what _norm_check found"""
+    _need(y.dim() >= 1 and y.dtype in _FLOATS and 1 <= y.shape[-1] <= 16384, '%s: fp32 or bf16 rows of 1 to 16384 values, got %s %s', what, y.dtype,
+          tuple(y.shape))
     C = y.shape[-1]
     _need(groups >= 1 and C % groups == 0, '%s: %d values in %d groups', what, C, groups)
     _need((C // groups) % 4 == 0 or C <= 8192, '%s: rows of more than 8192 values need groups of a multiple of 4', what)
     _need(kind in _NORMS, '%s: kind %r (one of %s)', what, kind, ', '.join(_NORMS))
-    for n, t in vectors:
-        _need(t is None or (t.shape == (C,) and t.dtype == torch.float32 and t.device == y.device), '%s: %s is fp32 [%d]', what, n, C)
+    for t in vectors:
+        _need(t is None or (t.shape == (C,) and t.dtype == torch.float32 and t.device == y.device), '%s: weights, biases and scales are fp32 [%d]', what, C)
     _need(y.is_cuda, '%s: GPU tensors (there is no CPU path)', what)
+    raise AssertionError(what)
+
+
+def _norm_check(what, y, groups, kind, vectors):
+    shape = y.shape
+    ok = len(shape) >= 1 and y.dtype in _FLOATS and 1 <= shape[-1] <= 16384 and groups >= 1 and shape[-1] % groups == 0 and kind in _NORMS and y.is_cuda and (
+        shape[-1] <= 8192 or shape[-1] // groups % 4 == 0)
+    if ok:
+        C, dev = shape[-1:], y.device
+        for t in vectors:
+            if t is not None and not (t.shape == C and t.dtype == torch.float32 and t.device == dev):
+                ok = False
+    if not ok:
+        _norm_refuse(what, y, groups, kind, vectors)
+
+
+def _tail_call(*args):
+    """args of BlockTailFunction.forward; without a gradient to come no node is built and no statistics are kept"""
+    if torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in args[:8]]):
+        return BlockTailFunction.apply(*args)
+    return _tail_forward(*args, False)[:2]
 
 
 def row_norm(x, weight, bias=None, kind='rms', groups=1, eps=1e-5):
     """The norm in front of a block: x [..., C] (fp32 or bf16) -> norm(x) * weight + bias, normalised over each of `groups` equal parts of a row.
     kind: 'rms' or 'layer' (the mean is removed).  weight, bias [C] fp32.  C up to 16384 (8192 where C / groups is no multiple of 4)."""
     _need(weight is not None, 'row_norm: needs a weight')
-    _norm_check('row_norm', x, groups, kind, (('weight', weight), ('bias', bias)))
-    return BlockTailFunction.apply(x, None, None, weight, bias, None, None, None, groups, kind == 'layer', ACT_NONE, 1.0, float(eps))[0]
+    _norm_check('row_norm', x, groups, kind, (weight, bias))
+    return _tail_call(x, None, None, weight, bias, None, None, None, groups, kind == 'layer', ACT_NONE, 1.0, float(eps))[0]
 
 
 def block_tail(y, residual=None, gate=None, weight=None, bias=None, scale=None, alpha=1.0, kind='rms', groups=1, gate_act=ACT_SILU, next_weight=None,
@@ -2131,14 +2202,18 @@ def block_tail(y, residual=None, gate=None, weight=None, bias=None, scale=None, 
     row (heads), the second over the whole row.  gate: y's shape, or [B, 1, ..., C] = one row per sequence y[b].  gate_act: ACT_NONE, ACT_SIGMOID or
     ACT_SILU.  scale [C] fp32 weights the branch, alpha the residual.  z is taken of h before it is rounded to y's type.
     Returns h, or (h, z) with next_weight."""
-    _norm_check('block_tail', y, groups, kind, (('weight', weight), ('bias', bias), ('scale', scale), ('next_weight', next_weight), ('next_bias', next_bias)))
-    _need(bias is None or weight is not None, 'block_tail: a bias without a weight')
-    _need(next_bias is None or next_weight is not None, 'block_tail: a next_bias without a next_weight')
-    _need(residual is None or (residual.shape == y.shape and residual.dtype == y.dtype and residual.device == y.device), 'block_tail: residual is like y')
-    _need(gate_act in (ACT_NONE, ACT_SIGMOID, ACT_SILU), 'block_tail: gate_act %r', gate_act)
+    _norm_check('block_tail', y, groups, kind, (weight, bias, scale, next_weight, next_bias))
+    if (bias is not None and weight is None) or (next_bias is not None and next_weight is None):
+        raise ValueError('ha2g_amd: block_tail: a bias without its weight')
+    if residual is not None and not (residual.shape == y.shape and residual.dtype == y.dtype and residual.device == y.device):
+        raise ValueError('ha2g_amd: block_tail: residual %s %s for y %s %s' % (residual.dtype, tuple(residual.shape), y.dtype, tuple(y.shape)))
+    if gate_act not in (ACT_NONE, ACT_SIGMOID, ACT_SILU):
+        raise ValueError('ha2g_amd: block_tail: gate_act %r' % (gate_act,))
     if gate is not None:
-        _need(gate.dtype == y.dtype and gate.device == y.device, 'block_tail: gate has the type and device of y')
-        _need(gate.shape == y.shape or (y.dim() >= 2 and gate.shape == (y.shape[0],) + (1,) * (y.dim() - 2) + (y.shape[-1],) and y.shape[0] <= 65535),
-              'block_tail: gate %s for y %s (like y, or one row for each of at most 65535 sequences)', tuple(gate.shape), tuple(y.shape))
-    h, z = BlockTailFunction.apply(y, residual, gate, weight, bias, scale, next_weight, next_bias, groups, kind == 'layer', gate_act, float(alpha), float(eps))
+        one = gate.shape != y.shape
+        if gate.dtype != y.dtype or gate.device != y.device or (one and not (
+                y.dim() >= 2 and gate.shape == (y.shape[0],) + (1,) * (y.dim() - 2) + (y.shape[-1],) and y.shape[0] <= 65535)):
+            raise ValueError('ha2g_amd: block_tail: gate %s %s for y %s %s (like y, or one row for each of at most 65535 sequences)'
+                             % (gate.dtype, tuple(gate.shape), y.dtype, tuple(y.shape)))
+    h, z = _tail_call(y, residual, gate, weight, bias, scale, next_weight, next_bias, groups, kind == 'layer', gate_act, float(alpha), float(eps))
     return h if next_weight is None else (h, z)

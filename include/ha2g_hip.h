@@ -573,21 +573,23 @@ int ha2g_logmel_f32(const float* y, int B, long n_samples, int pad_reflect, cons
                     float* ws, void* stream);
 
 /* ---- linear attention with one decay per head (no reference counterpart; stands beside the GRU recurrence of model/hierarchy_net.py:87-88,144) ----
- *   S_t = e^{log_decay} S_{t-1} + u_scale k_t v_t^T,  o_t = o_scale q_t S_t     per batch row and head, S fp32 [Dk][Dv], 1 <= Dk, Dv <= 128
- * q, k, v, o: strides = HOST array {batch, token, head} x {q, k, v, o} in elements, inner stride 1; fp32, or bf16 with b16_in (o: b16_out).
- * Head h of H reads head h / rq of q, h / rk of k, h / rv of v.  s_in / s_out [B][H][Dk][Dv] (s_transposed: [B][H][Dv][Dk]); s_in NULL = zero,
- * s_out NULL = not wanted.  lengths [B] (device int32, NULL = T): tokens at and behind a row's length are not read, o is zero there.
- * reverse: from the last token to the first, a step adds, reads and THEN decays.  The backward pass is three calls (all strides of the tensors named):
- *   dq = (q, k, v) := (do, v, k), s_in := S_0 transposed;  dk = (v, do, q) reverse, s_in := dS_T transposed, u_scale = scale, o_scale = 1;
- *   dv = (k, q, do) reverse, s_in := dS_T, u_scale = scale, o_scale = 1, s_out = dS_0. */
-int ha2g_linattn(const void* q, const void* k, const void* v, void* o, const float* log_decay, const float* s_in, float* s_out, const int* lengths,
-                 const long* strides, int B, int T, int H, int rq, int rk, int rv, int Dk, int Dv, int s_transposed, float o_scale, float u_scale,
-                 int reverse, int b16_in, int b16_out, float* ws, void* stream);
-/* floats of `ws` (0: may be NULL): the states between the segments of a time axis that is split over the chip */
-long ha2g_linattn_workspace_floats(int B, int T, int H, int Dk, int Dv, int b16_in);
+ *   S_t = e^{log_decay} S_{t-1} + k_t v_t^T,  o_t = scale q_t S_t     per batch row and head, S fp32 [Dk][Dv], 1 <= Dk, Dv <= 128
+ * q, k, v, o: fp32, or (b16_io) bf16; strides = HOST array {batch, token, head} x {q, k, v, o} in elements, inner stride 1.  Head h of H reads head
+ * h / rq of q, h / rk of k, h / rv of v.  s_in / s_out [B][H][Dk][Dv]: states in front of the first and behind the last token (NULL = zero, = not
+ * wanted).  lengths [B] (device int32, NULL = T): tokens at and behind a row's length are not read, o is zero there.
+ * ws: ha2g_linattn_workspace_floats() floats (0: may be NULL), the states between the segments of a time axis that is split over the chip. */
+long ha2g_linattn_workspace_floats(int B, int T, int H, int Dk, int Dv, int b16_io);
+int ha2g_linattn_fwd(const void* q, const void* k, const void* v, void* o, const float* log_decay, const float* s_in, float* s_out, const int* lengths,
+                     const long* strides, int B, int T, int H, int rq, int rk, int rv, int Dk, int Dv, float scale, int b16_io, float* ws, void* stream);
+/* gradients: dout and ds_out (NULL = zero) -> dq, dk, dv (NULL = not wanted), ds_in (NULL; otherwise with dv), each of dq, dk, dv with H heads (heads
+ * that share one are added up by ha2g_head_sum) in fp32 or (.._b16) bf16.  strides: {q, k, v, dout, dq, dk, dv}.  ws_fwd: the forward call's
+ * workspace as it left it (for dq); ws: another one of the same size. */
+int ha2g_linattn_bwd(const void* q, const void* k, const void* v, const void* dout, void* dq, void* dk, void* dv, const float* log_decay, const float* s_in,
+                     const float* ds_out, float* ds_in, const int* lengths, const long* strides, int B, int T, int H, int rq, int rk, int rv, int Dk, int Dv,
+                     float scale, int b16_io, int dq_b16, int dk_b16, int dv_b16, const float* ws_fwd, float* ws, void* stream);
 /* one token: q [B][..][Dk] ..., state updated in place; the token strides are not read */
 int ha2g_linattn_step(const void* q, const void* k, const void* v, void* o, const float* log_decay, float* state, const long* strides, int B, int H,
-                      int rq, int rk, int rv, int Dk, int Dv, float o_scale, int b16_io, void* stream);
+                      int rq, int rk, int rv, int Dk, int Dv, float scale, int b16_io, void* stream);
 /* out [rows][heads][D] = the sum over n consecutive heads of x [rows][heads][n][D] (gradients of shared heads) */
 int ha2g_head_sum(const float* x, void* out, long rows, int heads, int n, int D, int b16_out, void* stream);
 

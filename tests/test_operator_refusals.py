@@ -115,7 +115,7 @@ def test_c_entries_return_errors_instead_of_launching():
     import array
     from ha2g_amd._lib import lib
     st = array.array('l', [0] * 12)
-    la = lambda B, H, rq, Dk, Dv: lib.ha2g_linattn(None, None, None, None, None, None, None, None, st, B, 1, H, rq, 1, 1, Dk, Dv, 0, 1.0, 1.0, 0, 0, 0, None, None)      # noqa: E731
+    la = lambda B, H, rq, Dk, Dv: lib.ha2g_linattn_fwd(None, None, None, None, None, None, None, None, st, B, 1, H, rq, 1, 1, Dk, Dv, 1.0, 0, None, None)      # noqa: E731
     assert la(0, 1, 1, 8, 8) == 0
     for bad in ((1, 1, 1, 8, 8), (0, 3, 2, 8, 8), (0, 1, 1, 129, 8), (0, 1, 1, 8, 0), (0, 0, 1, 8, 8)):
         assert la(*bad) != 0 and lib.ha2g_last_error()
