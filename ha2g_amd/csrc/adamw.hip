@@ -1,6 +1,7 @@
 // AdamW (decoupled weight decay) over many separately allocated tensors in one launch:
 //     m = b1 m + (1 - b1) g;   v = b2 v + (1 - b2) g^2;   p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
-// in fp32 per element, the step's scalars in double, t read from device memory (a captured graph advances it).  States are fp32, or 8 bits:
+// in fp32 per element, the step's scalars in double by one thread that also advances t in device memory (a captured graph does so on each replay;
+// two powers in double by every thread cost more than the elements).  States are fp32, or 8 bits:
 // blocks of 128 consecutive elements of a tensor hold m and r = sqrt(v) as e4m3 codes times one power of two each, the smallest that brings the
 // block's largest finite magnitude to at most 448.  r instead of v halves the range in octaves.  A code has 4 significant bits, so a round to
 // nearest would never let v decay by its 0.1 % a step: the part below a code rounds up with its own probability, by a dither that a counter hash
@@ -9,7 +10,7 @@
 
 namespace {
 
-constexpr int AW_TENSORS = 48;      // per launch: the table travels by value in the kernel's arguments (48 * 60 bytes of the 4 KB)
+constexpr int AW_TENSORS = 64;      // per launch: the table travels by value in the kernel's arguments
 
 struct AdamWTable {
     void *p[AW_TENSORS], *g[AW_TENSORS], *m[AW_TENSORS], *v[AW_TENSORS];
@@ -19,12 +20,21 @@ struct AdamWTable {
     int count, first;               // tensors here, number of the first one (the dither's)
     unsigned long long vec;         // bit i: tensor i's pointers allow wide accesses
 };
-
 struct AdamWScalars {
-    double lr, b1, b2, eps, wd;
+    float b1, b2, omb1, omb2, keep, eps;
     unsigned seed;
-    const int *step, *guard;
+    const float* dev;               // lr / (1 - b1^t), 1 / sqrt(1 - b2^t), t (as an integer)
+    const int* guard;
 };
+static_assert(sizeof(AdamWTable) + sizeof(AdamWScalars) <= 4096, "kernel arguments");
+
+__global__ void adamw_scalars_kernel(int* step, const int* guard, double lr, double b1, double b2, float* out) {
+    if (guard == nullptr || *guard == 0) *step += 1;
+    const double t = (double)*step;
+    out[0] = (float)(lr / (1.0 - pow(b1, t)));
+    out[1] = (float)(1.0 / sqrt(1.0 - pow(b2, t)));
+    reinterpret_cast<int*>(out)[2] = *step;
+}
 
 __device__ __forceinline__ unsigned hash32(unsigned x) {      // factors: 2^32 over the golden ratio, and over the plastic number
     x = (x ^ (x >> 16)) * 0x9e3779b9u;
@@ -32,16 +42,11 @@ __device__ __forceinline__ unsigned hash32(unsigned x) {      // factors: 2^32 o
     return x ^ (x >> 16);
 }
 
-struct StepScalars { float b1, b2, omb1, omb2, keep, step, root, eps; };
-__device__ __forceinline__ StepScalars step_scalars(const AdamWScalars& s) {
-    const double t = (double)*s.step;
-    return {(float)s.b1, (float)s.b2, (float)(1.0 - s.b1), (float)(1.0 - s.b2), (float)(1.0 - s.lr * s.wd), (float)(s.lr / (1.0 - pow(s.b1, t))),
-            (float)(1.0 / sqrt(1.0 - pow(s.b2, t))), (float)s.eps};
-}
-__device__ __forceinline__ void update(const StepScalars& c, float g, float& p, float& m, float& v) {
+__device__ __forceinline__ void update(const AdamWScalars& c, float step, float root, float g, float& p, float& m, float& v, float& r) {
     m = c.b1 * m + c.omb1 * g;
     v = c.b2 * v + (c.omb2 * g) * g;
-    p = p * c.keep - c.step * m / (sqrtf(v) * c.root + c.eps);
+    r = sqrtf(v);
+    p = p * c.keep - step * m / (r * root + c.eps);
 }
 __device__ __forceinline__ void sta(float* p, long i, float x) { p[i] = x; }
 __device__ __forceinline__ void sta(b16* p, long i, float x) { unsigned h, l; split2_bf16(x, 0.f, h, l); p[i] = (b16)(h & 0xffff); }
@@ -56,7 +61,7 @@ __device__ __forceinline__ int find_tensor(const AdamWTable& t, int c) {
     return lo;
 }
 
-constexpr int CHUNK32 = 4096, CHUNK8 = 2048;
+constexpr int CHUNK32 = 4096, CHUNK8 = 4096;
 
 template <typename TP, typename TG>
 __global__ __launch_bounds__(256) void adamw32_kernel(const AdamWTable tab, const AdamWScalars sc) {
@@ -66,16 +71,17 @@ __global__ __launch_bounds__(256) void adamw32_kernel(const AdamWTable tab, cons
     TP* p = (TP*)tab.p[i];
     const TG* g = (const TG*)tab.g[i];
     float *m = (float*)tab.m[i], *v = (float*)tab.v[i];
-    const StepScalars c = step_scalars(sc);
+    const float step = sc.dev[0], root = sc.dev[1];
+    float r;
     if ((tab.vec >> i & 1) && base + CHUNK32 <= n) {
 #pragma unroll
         for (int u = 0; u < CHUNK32 / 1024; ++u) {
             const long at = (base >> 2) + u * 256 + threadIdx.x;
             float4 P = ld4(p, at), G = ld4(g, at), M = ld4(m, at), V = ld4(v, at);
-            update(c, G.x, P.x, M.x, V.x);
-            update(c, G.y, P.y, M.y, V.y);
-            update(c, G.z, P.z, M.z, V.z);
-            update(c, G.w, P.w, M.w, V.w);
+            update(sc, step, root, G.x, P.x, M.x, V.x, r);
+            update(sc, step, root, G.y, P.y, M.y, V.y, r);
+            update(sc, step, root, G.z, P.z, M.z, V.z, r);
+            update(sc, step, root, G.w, P.w, M.w, V.w, r);
             st4(p, at, P); st4(m, at, M); st4(v, at, V);
         }
         return;
@@ -83,15 +89,16 @@ __global__ __launch_bounds__(256) void adamw32_kernel(const AdamWTable tab, cons
     const long end = min(n, base + CHUNK32);
     for (long at = base + threadIdx.x; at < end; at += 256) {
         float P = ld1(p, at), M = m[at], V = v[at];
-        update(c, ld1(g, at), P, M, V);
+        update(sc, step, root, ld1(g, at), P, M, V, r);
         sta(p, at, P); m[at] = M; v[at] = V;
     }
 }
 
-__device__ __forceinline__ float code_value(unsigned code) {                   // one e4m3 code
-    return __builtin_amdgcn_cvt_f32_fp8((int)code, 0);
+// |x| if it is finite, else 0
+__device__ __forceinline__ float finite_abs(float x) {
+    const unsigned u = __float_as_uint(x) & 0x7fffffffu;
+    return __uint_as_float(u < 0x7f800000u ? u : 0u);
 }
-__device__ __forceinline__ bool finite_f(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 // exponent of the block's scale from its largest finite magnitude
 __device__ __forceinline__ int scale_exponent(float top) {
     const unsigned u = __float_as_uint(top);
@@ -99,86 +106,105 @@ __device__ __forceinline__ int scale_exponent(float top) {
     const int e = field - 126 - 9 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
     return (field == 0 || e < -126) ? -126 : e;
 }
-__device__ __forceinline__ unsigned encode(float x, float inv, unsigned dither) {
-    if (!finite_f(x)) return 0x7f;
-    const float a = fabsf(x) * inv;
-    int ue = (int)(__float_as_uint(a) >> 23) - 127;
-    if (ue < -6) ue = -6;
-    const int k = (int)(a * __uint_as_float((unsigned)(130 - ue) << 23) + (float)dither * 0x1p-16f);
-    const int code = (ue + 7) * 8 + k - 8;
-    return (unsigned)(code > 126 ? 126 : code) | (x < 0.f ? 0x80u : 0u);
+// a = |x| / scale <= 448 (x finite): the code of the binade, plus the 4 significant bits of a with the dither added below them
+__device__ __forceinline__ unsigned encode(float x, float inv, float dither) {
+    const float f = finite_abs(x), a = f * inv;
+    const int ue = max((int)(__float_as_uint(a) >> 23), 121);                            // exponent field, at least that of 2^-6
+    const int k = (int)(a * __uint_as_float((unsigned)(257 - ue) << 23) + dither);
+    unsigned code = (unsigned)min((ue - 120) * 8 + k - 8, 126);
+    code = f == fabsf(x) ? code : 0x7fu;                                                // NaN and infinities: the NaN code
+    return code | (x < 0.f ? 0x80u : 0u);
 }
 
-// 16 lanes hold a block of 128 elements, 8 consecutive ones each
+// 16 lanes hold a block of 128 elements, 8 consecutive ones each; a thread does this for CHUNK8 / 2048 places
 template <typename TP, typename TG>
 __global__ __launch_bounds__(256) void adamw8_kernel(const AdamWTable tab, const AdamWScalars sc) {
     if (sc.guard != nullptr && *sc.guard != 0) return;
     const int i = find_tensor(tab, blockIdx.x);
-    const long at = (long)(blockIdx.x - tab.start[i]) * CHUNK8 + threadIdx.x * 8, n = tab.n[i];
+    const long n = tab.n[i];
     TP* p = (TP*)tab.p[i];
     const TG* g = (const TG*)tab.g[i];
     unsigned char *mc = (unsigned char*)tab.m[i], *rc = (unsigned char*)tab.v[i];
-    const StepScalars c = step_scalars(sc);
-    const bool wide = (tab.vec >> i & 1) && at + 8 <= n, any = at < n;
-    float P[8], G[8], M[8], R[8];
-    unsigned char cm[8] = {0}, cr[8] = {0};
-    float sm = 0.f, sr = 0.f;
-    if (any) { sm = tab.sm[i][at >> 7]; sr = tab.sr[i][at >> 7]; }
-    if (wide) {
+    float *smp = tab.sm[i], *srp = tab.sr[i];
+    const float step = sc.dev[0], root = sc.dev[1];
+    const unsigned key = hash32(hash32(hash32(sc.seed) ^ (unsigned)__float_as_int(sc.dev[2])) ^ (unsigned)(tab.first + i));
+    const bool vec = tab.vec >> i & 1;
+#pragma unroll 1
+    for (int u = 0; u < CHUNK8 / 2048; ++u) {
+        const long at = (long)(blockIdx.x - tab.start[i]) * CHUNK8 + u * 2048 + threadIdx.x * 8;
+        const bool wide = vec && at + 8 <= n, any = at < n;
+        float P[8], G[8], M[8], R[8];
+        unsigned cm[2] = {0u, 0u}, cr[2] = {0u, 0u};              // elements behind the end are zeros and stay zeros
+        float sm = 0.f, sr = 0.f;
+        if (any) { sm = smp[at >> 7]; sr = srp[at >> 7]; }
+        if (wide) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const float4 a = ld4(p, (at >> 2) + h), b = ld4(g, (at >> 2) + h);
+                P[4 * h] = a.x; P[4 * h + 1] = a.y; P[4 * h + 2] = a.z; P[4 * h + 3] = a.w;
+                G[4 * h] = b.x; G[4 * h + 1] = b.y; G[4 * h + 2] = b.z; G[4 * h + 3] = b.w;
+            }
+            const uint2 x = *reinterpret_cast<const uint2*>(mc + at), y = *reinterpret_cast<const uint2*>(rc + at);
+            cm[0] = x.x; cm[1] = x.y; cr[0] = y.x; cr[1] = y.y;
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                P[k] = G[k] = 0.f;
+                if (at + k < n) {
+                    P[k] = ld1(p, at + k);
+                    G[k] = ld1(g, at + k);
+                    cm[k >> 2] |= (unsigned)mc[at + k] << (8 * (k & 3));
+                    cr[k >> 2] |= (unsigned)rc[at + k] << (8 * (k & 3));
+                }
+            }
+        }
+        float tm = 0.f, tr = 0.f;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const float4 a = ld4(p, (at >> 2) + h), b = ld4(g, (at >> 2) + h);
-            P[4 * h] = a.x; P[4 * h + 1] = a.y; P[4 * h + 2] = a.z; P[4 * h + 3] = a.w;
-            G[4 * h] = b.x; G[4 * h + 1] = b.y; G[4 * h + 2] = b.z; G[4 * h + 3] = b.w;
+            M[4 * h] = __builtin_amdgcn_cvt_f32_fp8((int)cm[h], 0); M[4 * h + 1] = __builtin_amdgcn_cvt_f32_fp8((int)cm[h], 1);
+            M[4 * h + 2] = __builtin_amdgcn_cvt_f32_fp8((int)cm[h], 2); M[4 * h + 3] = __builtin_amdgcn_cvt_f32_fp8((int)cm[h], 3);
+            R[4 * h] = __builtin_amdgcn_cvt_f32_fp8((int)cr[h], 0); R[4 * h + 1] = __builtin_amdgcn_cvt_f32_fp8((int)cr[h], 1);
+            R[4 * h + 2] = __builtin_amdgcn_cvt_f32_fp8((int)cr[h], 2); R[4 * h + 3] = __builtin_amdgcn_cvt_f32_fp8((int)cr[h], 3);
         }
-        *reinterpret_cast<uint2*>(cm) = *reinterpret_cast<const uint2*>(mc + at);
-        *reinterpret_cast<uint2*>(cr) = *reinterpret_cast<const uint2*>(rc + at);
-    } else {
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            const bool in = at + k < n;
-            P[k] = in ? ld1(p, at + k) : 0.f;
-            G[k] = in ? ld1(g, at + k) : 0.f;
-            if (in) { cm[k] = mc[at + k]; cr[k] = rc[at + k]; }
+            M[k] *= sm;
+            R[k] *= sr;
+            float v = R[k] * R[k];
+            update(sc, step, root, G[k], P[k], M[k], v, R[k]);
+            tm = fmaxf(tm, finite_abs(M[k]));
+            tr = fmaxf(tr, finite_abs(R[k]));
         }
-    }
-    float tm = 0.f, tr = 0.f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-        const float r = code_value(cr[k]) * sr;
-        float v = r * r;
-        M[k] = code_value(cm[k]) * sm;
-        update(c, G[k], P[k], M[k], v);
-        R[k] = sqrtf(v);
-        if (at + k >= n) M[k] = R[k] = 0.f;
-        if (finite_f(M[k])) tm = fmaxf(tm, fabsf(M[k]));
-        if (finite_f(R[k])) tr = fmaxf(tr, R[k]);
-    }
+        for (int o = 8; o > 0; o >>= 1) { tm = fmaxf(tm, __shfl_xor(tm, o, 64)); tr = fmaxf(tr, __shfl_xor(tr, o, 64)); }
+        const int em = scale_exponent(tm), er = scale_exponent(tr);
+        const float im = __uint_as_float((unsigned)(127 - em) << 23), ir = __uint_as_float((unsigned)(127 - er) << 23);
+        const unsigned place = key ^ (unsigned)(at >> 32) * 0x9e3779b9u;                  // at is a multiple of 8: its upper word is the elements'
+        cm[0] = cm[1] = cr[0] = cr[1] = 0u;
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) { tm = fmaxf(tm, __shfl_xor(tm, o, 64)); tr = fmaxf(tr, __shfl_xor(tr, o, 64)); }
-    const int em = scale_exponent(tm), er = scale_exponent(tr);
-    const float im = __uint_as_float((unsigned)(127 - em) << 23), ir = __uint_as_float((unsigned)(127 - er) << 23);
-    const unsigned key = hash32(hash32(hash32(sc.seed) ^ (unsigned)*sc.step) ^ (unsigned)(tab.first + i));
+        for (int k = 0; k < 8; ++k) {
+            const unsigned d = hash32(((unsigned)at + k) ^ place);
+            cm[k >> 2] |= encode(M[k], im, (float)(d >> 16) * 0x1p-16f) << (8 * (k & 3));
+            cr[k >> 2] |= encode(R[k], ir, (float)(d & 0xffffu) * 0x1p-16f) << (8 * (k & 3));
+        }
+        if (wide) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-        const unsigned long long e = (unsigned long long)(at + k);
-        const unsigned d = hash32((unsigned)e ^ (unsigned)(e >> 32) * 0x9e3779b9u ^ key);
-        cm[k] = (unsigned char)encode(M[k], im, d >> 16);
-        cr[k] = (unsigned char)encode(R[k], ir, d & 0xffff);
-    }
-    if (wide) {
+            for (int h = 0; h < 2; ++h) st4(p, (at >> 2) + h, make_float4(P[4 * h], P[4 * h + 1], P[4 * h + 2], P[4 * h + 3]));
+            *reinterpret_cast<uint2*>(mc + at) = make_uint2(cm[0], cm[1]);
+            *reinterpret_cast<uint2*>(rc + at) = make_uint2(cr[0], cr[1]);
+        } else {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) st4(p, (at >> 2) + h, make_float4(P[4 * h], P[4 * h + 1], P[4 * h + 2], P[4 * h + 3]));
-        *reinterpret_cast<uint2*>(mc + at) = *reinterpret_cast<const uint2*>(cm);
-        *reinterpret_cast<uint2*>(rc + at) = *reinterpret_cast<const uint2*>(cr);
-    } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-            if (at + k < n) { sta(p, at + k, P[k]); mc[at + k] = cm[k]; rc[at + k] = cr[k]; }
-    }
-    if (any && (threadIdx.x & 15) == 0) {
-        tab.sm[i][at >> 7] = __uint_as_float((unsigned)(127 + em) << 23);
-        tab.sr[i][at >> 7] = __uint_as_float((unsigned)(127 + er) << 23);
+            for (int k = 0; k < 8; ++k)
+                if (at + k < n) {
+                    sta(p, at + k, P[k]);
+                    mc[at + k] = (unsigned char)(cm[k >> 2] >> (8 * (k & 3)));
+                    rc[at + k] = (unsigned char)(cr[k >> 2] >> (8 * (k & 3)));
+                }
+        }
+        if (any && (threadIdx.x & 15) == 0) {
+            smp[at >> 7] = __uint_as_float((unsigned)(127 + em) << 23);
+            srp[at >> 7] = __uint_as_float((unsigned)(127 + er) << 23);
+        }
     }
 }
 
@@ -192,13 +218,20 @@ template <typename TP, typename TG> void adamw_launch(const AdamWTable& t, const
 
 extern "C" {
 
+int ha2g_adamw_scalars(int* step, const int* guard, double lr, double b1, double b2, float* scalars, void* stream) {
+    HA2G_REQUIRE(step && scalars, "adamw_scalars: null operand");
+    hipLaunchKernelGGL(adamw_scalars_kernel, dim3(1), dim3(1), 0, (hipStream_t)stream, step, guard, lr, b1, b2, scalars);
+    HA2G_CHECK_LAUNCH("adamw_scalars");
+    return 0;
+}
+
 // p, g, m, v (and with 8 bits sm, sr): HOST arrays of n device pointers, len: HOST array of n lengths
 int ha2g_adamw_multi(int n, const long* p, const long* g, const long* m, const long* v, const long* sm, const long* sr, const long* len, int p_b16,
-                     int g_b16, int bits, double lr, double b1, double b2, double eps, double wd, unsigned seed, int first, const int* step,
+                     int g_b16, int bits, double lr, double b1, double b2, double eps, double wd, unsigned seed, int first, const float* scalars,
                      const int* guard, void* stream) {
     HA2G_REQUIRE(bits == 32 || bits == 8, "adamw: states of %d bits", bits);
-    HA2G_REQUIRE(n >= 0 && (n == 0 || (p && g && m && v && len && step && (bits == 32 || (sm && sr)))), "adamw: null table");
-    const AdamWScalars sc = {lr, b1, b2, eps, wd, seed, step, guard};
+    HA2G_REQUIRE(n >= 0 && (n == 0 || (p && g && m && v && len && scalars && (bits == 32 || (sm && sr)))), "adamw: null table");
+    const AdamWScalars sc = {(float)b1, (float)b2, (float)(1.0 - b1), (float)(1.0 - b2), (float)(1.0 - lr * wd), (float)eps, seed, scalars, guard};
     const long chunk = bits == 32 ? CHUNK32 : CHUNK8;
     AdamWTable t;
     t.count = 0;

@@ -408,48 +408,73 @@ __global__ __launch_bounds__(256) void linattn_segment_scan_kernel(const LinAttn
     }
 }
 
-// One token: a block per (batch row, head); thread = (row group, column), the partial sums over the row groups meet in LDS.
-template <typename T>
-__global__ __launch_bounds__(256) void linattn_step_kernel(const LinAttnArgs a) {
-    __shared__ float qs[128], ks[128], red[256];
+// One token: a block per (batch row, head), bound by the state's one read and one write.  Thread = (row group, V neighbouring columns), eight rows in
+// flight each; the partial sums over the row groups meet in LDS.
+template <typename T, int V>
+__global__ __launch_bounds__(256) void linattn_step_kernel(const LinAttnArgs a, int lpr /* threads per row, a power of two with lpr * V >= Dv */) {
+    __shared__ float qs[128], ks[128], red[256 * V];
     const Job& J = a.job[0];
-    const int h = blockIdx.x % a.H, b = blockIdx.x / a.H, tid = threadIdx.x;
+    const int h = blockIdx.x % a.H, b = blockIdx.x / a.H, tid = threadIdx.x, Dk = J.Dk, Dv = J.Dv;
     const T* q = (const T*)J.q.p + (long)b * J.q.b + (long)(h / J.q.r) * J.q.h;
     const T* k = (const T*)J.k.p + (long)b * J.k.b + (long)(h / J.k.r) * J.k.h;
     const T* v = (const T*)J.v.p + (long)b * J.v.b + (long)(h / J.v.r) * J.v.h;
-    if (tid < J.Dk) { qs[tid] = ld1(q, tid); ks[tid] = ld1(k, tid); }
+    const int j = tid % lpr * V, r0 = tid / lpr, groups = 256 / lpr;
+    float* S = J.s_out + ((long)b * a.H + h) * Dk * Dv + j;
+    float vv[V], acc[V];
+#pragma unroll
+    for (int c = 0; c < V; ++c) { vv[c] = j < Dv ? ld1(v, j + c) : 0.f; acc[c] = 0.f; }
+    if (tid < Dk) { qs[tid] = ld1(q, tid); ks[tid] = ld1(k, tid); }
     __syncthreads();
     const float lam = expf(a.g[h]);
-    float* S = J.s_out + ((long)b * a.H + h) * J.Dk * J.Dv;
-    const int cols = J.Dv <= 32 ? 32 : (J.Dv <= 64 ? 64 : 128), groups = 256 / cols, j = tid % cols, r0 = tid / cols;
-    float acc = 0.f;
-    if (j < J.Dv) {
-        const float vv = ld1(v, j);
-        for (int d = r0; d < J.Dk; d += groups) {
-            const float s = lam * S[(long)d * J.Dv + j] + ks[d] * vv;
-            S[(long)d * J.Dv + j] = s;
-            acc += qs[d] * s;
+    if (j < Dv)
+        for (int d0 = r0; d0 < Dk; d0 += 8 * groups) {
+            float s[8][V];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int d = d0 + u * groups;
+                if (d < Dk) {
+                    if constexpr (V == 4) { const float4 x = ld4(S + (long)d * Dv, 0); s[u][0] = x.x; s[u][1] = x.y; s[u][2] = x.z; s[u][3] = x.w; }
+                    else s[u][0] = S[(long)d * Dv];
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int d = d0 + u * groups;
+                if (d < Dk) {
+#pragma unroll
+                    for (int c = 0; c < V; ++c) { s[u][c] = lam * s[u][c] + ks[d] * vv[c]; acc[c] += qs[d] * s[u][c]; }
+                    if constexpr (V == 4) st4(S + (long)d * Dv, 0, make_float4(s[u][0], s[u][1], s[u][2], s[u][3]));
+                    else S[(long)d * Dv] = s[u][0];
+                }
+            }
         }
-    }
-    red[tid] = acc;
+#pragma unroll
+    for (int c = 0; c < V; ++c) red[tid * V + c] = acc[c];
     __syncthreads();
-    if (tid < J.Dv) {
+    if (tid < Dv) {
         float s = 0.f;
-        for (int r = 0; r < groups; ++r) s += red[r * cols + tid];
+        for (int r = 0; r < groups; ++r) s += red[r * lpr * V + tid];
         st1((T*)J.o + (long)b * J.ob + (long)h * J.oh, tid, s * J.oscale);
     }
 }
 
 // out[r][c] = sum over j < n of x[r][c / D][j][c % D]: the gradient of a head that n heads read, in the order of the heads
-template <typename T>
-__global__ void head_sum_kernel(const float* __restrict__ x, T* __restrict__ out, long rows, int heads, int n, int D) {
-    const long total = rows * heads * D;
+template <typename T, int V>
+__global__ __launch_bounds__(256) void head_sum_kernel(const float* __restrict__ x, T* __restrict__ out, long rows, int n, int D) {
+    const long total = rows * (D / V);                    // rows: one per token and shared head
     for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
-        const int d = (int)(i % D);
-        const float* p = x + i / D * n * D + d;
-        float s = p[0];
-        for (int j = 1; j < n; ++j) s += p[(long)j * D];
-        st1(out, i, s);
+        const long r = i / (D / V);
+        const int d = (int)(i - r * (D / V)) * V;
+        const float* p = x + r * n * D + d;
+        if constexpr (V == 4) {
+            float4 s = ld4(p, 0);
+            for (int j = 1; j < n; ++j) { const float4 y = ld4(p + (long)j * D, 0); s.x += y.x; s.y += y.y; s.z += y.z; s.w += y.w; }
+            st4(out + r * D + d, 0, s);
+        } else {
+            float s = p[0];
+            for (int j = 1; j < n; ++j) s += p[(long)j * D];
+            st1(out, r * D + d, s);
+        }
     }
 }
 
@@ -613,8 +638,14 @@ int ha2g_linattn_step(const void* q, const void* k, const void* v, void* o, cons
     j.Dk = Dk; j.Dv = Dv; j.oscale = scale;
     set_out(j, o, strides + 9, b16_io);
     j.s_out = state;
-    if (b16_io) hipLaunchKernelGGL(linattn_step_kernel<b16>, dim3(B * H), dim3(256), 0, (hipStream_t)stream, a);
-    else hipLaunchKernelGGL(linattn_step_kernel<float>, dim3(B * H), dim3(256), 0, (hipStream_t)stream, a);
+    const bool wide = Dv % 4 == 0 && (uintptr_t)state % 16 == 0;
+    int lpr = 1;
+    while (lpr * (wide ? 4 : 1) < Dv) lpr *= 2;
+    const dim3 grid(B * H), block(256);
+    if (b16_io && wide) hipLaunchKernelGGL((linattn_step_kernel<b16, 4>), grid, block, 0, (hipStream_t)stream, a, lpr);
+    else if (b16_io) hipLaunchKernelGGL((linattn_step_kernel<b16, 1>), grid, block, 0, (hipStream_t)stream, a, lpr);
+    else if (wide) hipLaunchKernelGGL((linattn_step_kernel<float, 4>), grid, block, 0, (hipStream_t)stream, a, lpr);
+    else hipLaunchKernelGGL((linattn_step_kernel<float, 1>), grid, block, 0, (hipStream_t)stream, a, lpr);
     HA2G_CHECK_LAUNCH("linattn_step");
     return 0;
 }
@@ -622,10 +653,14 @@ int ha2g_linattn_step(const void* q, const void* k, const void* v, void* o, cons
 int ha2g_head_sum(const float* x, void* out, long rows, int heads, int n, int D, int b16_out, void* stream) {
     HA2G_REQUIRE(rows >= 0 && heads >= 1 && n >= 1 && D >= 1, "head_sum: rows=%ld heads=%d n=%d D=%d", rows, heads, n, D);
     if (rows == 0) return 0;
-    const long total = rows * heads * D, want = (total + 255) / 256;
-    const dim3 grid((unsigned)(want > 16384 ? 16384 : want));
-    if (b16_out) hipLaunchKernelGGL(head_sum_kernel<b16>, grid, dim3(256), 0, (hipStream_t)stream, x, (b16*)out, rows, heads, n, D);
-    else hipLaunchKernelGGL(head_sum_kernel<float>, grid, dim3(256), 0, (hipStream_t)stream, x, (float*)out, rows, heads, n, D);
+    const bool wide = D % 4 == 0 && (uintptr_t)x % 16 == 0 && (uintptr_t)out % (b16_out ? 8 : 16) == 0;
+    const long want = (rows * heads * (wide ? D / 4 : D) + 255) / 256;
+    const dim3 grid((unsigned)(want > 16384 ? 16384 : want)), block(256);
+    const hipStream_t st = (hipStream_t)stream;
+    if (b16_out && wide) hipLaunchKernelGGL((head_sum_kernel<b16, 4>), grid, block, 0, st, x, (b16*)out, rows * heads, n, D);
+    else if (b16_out) hipLaunchKernelGGL((head_sum_kernel<b16, 1>), grid, block, 0, st, x, (b16*)out, rows * heads, n, D);
+    else if (wide) hipLaunchKernelGGL((head_sum_kernel<float, 4>), grid, block, 0, st, x, (float*)out, rows * heads, n, D);
+    else hipLaunchKernelGGL((head_sum_kernel<float, 1>), grid, block, 0, st, x, (float*)out, rows * heads, n, D);
     HA2G_CHECK_LAUNCH("head_sum");
     return 0;
 }

@@ -10,7 +10,7 @@ import array
 import torch
 
 from ._lib import check, lib
-from .ops import _need, _on, _stream, gru_cluster_error_tensor
+from .ops import _FLOATS, _need, _on, _stream, gru_cluster_error_tensor
 
 
 def _storage_span(p):
@@ -140,8 +140,9 @@ def _ptrs(ts):
 
 
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, seed=0, guard=None):
-    """One AdamW step over lists of tensors, in place (kernel ha2g_adamw_multi: 48 tensors per launch).  `step` (int32 [1] on the device) is advanced first.
-    params, grads: fp32 or bf16, one type each, dense and laid out alike.  States in 32 bits: fp32 tensors laid out like the parameters.  In 8 bits:
+    """One AdamW step over lists of tensors, in place (kernel ha2g_adamw_multi: 64 tensors per launch).  `step` (int32 [1] on the device) is advanced first.
+    params, grads: fp32 or bf16, one type each, dense and laid out alike (contiguous tensors: of as many elements).  States in 32 bits: fp32 tensors
+    laid out like the parameters.  In 8 bits:
     pairs (codes, scales) as adamw_state8 makes them, exp_avg_sqs holding the ROOT of the second moment; `seed` (32 bits) varies the rounding's dither.
     No tensor appears twice.  guard: optional int32 device word; while it is not zero the step changes nothing.  Everything lies on one device."""
     n = len(params)
@@ -155,39 +156,59 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9, 
         ms, vs, sm, sr = ([s[i] for s in st] for st, i in ((exp_avgs, 0), (exp_avg_sqs, 0), (exp_avgs, 1), (exp_avg_sqs, 1)))
     else:
         ms, vs, sm, sr = exp_avgs, exp_avg_sqs, (), ()
-    every = [*params, *grads, *ms, *vs, *sm, *sr]
-    _need(all(isinstance(t, torch.Tensor) for t in every), 'adamw_step: lists of tensors (8-bit states: of pairs)')
-    _need({t.device for t in every} <= {step.device}, 'adamw_step: everything lies on the device of step')
-    pt, gt = {t.dtype for t in params}, {t.dtype for t in grads}
-    _need(len(pt) <= 1 and len(gt) <= 1 and pt | gt <= {torch.float32, torch.bfloat16}, 'adamw_step: parameters %s, gradients %s (one of fp32, bf16 each)', pt, gt)
-    # the usual case in a few passes over the lists: everything contiguous, sizes alike
-    num = [p.numel() for p in params]
-    plain = all([t.is_contiguous() for t in every])
-    if not (plain and [t.numel() for t in grads] == num):
-        for p, g in zip(params, grads):
-            _need(_dense(p) and _alike(p, g), 'adamw_step: a gradient %s %s for a parameter %s %s', tuple(g.shape), g.stride(), tuple(p.shape), p.stride())
-    if q8:
-        _need({t.dtype for t in ms} | {t.dtype for t in vs} == {torch.float8_e4m3fn} and {t.dtype for t in sm} | {t.dtype for t in sr} == {torch.float32},
-              'adamw_step: 8-bit states are float8_e4m3fn codes and fp32 scales')
-        blocks = [-(-k // Q8_BLOCK) for k in num]
-        _need(all([t.is_contiguous() for st in (ms, vs, sm, sr) for t in st]) and [t.numel() for t in ms] == num == [t.numel() for t in vs] and
-              [t.numel() for t in sm] == blocks == [t.numel() for t in sr], 'adamw_step: 8-bit states of other sizes than their parameters')
-    else:
-        _need({t.dtype for t in ms} | {t.dtype for t in vs} <= {torch.float32}, 'adamw_step: states are fp32 tensors, or pairs for 8 bits')
-        if not (plain and [t.numel() for t in ms] == num == [t.numel() for t in vs]):
-            for p, m, v in zip(params, ms, vs):
-                _need(_alike(p, m) and _alike(p, v), 'adamw_step: a state %s %s for a parameter %s %s', tuple(m.shape), m.stride(), tuple(p.shape), p.stride())
-    _need(step.is_cuda, 'adamw_step: GPU tensors (there is no CPU path)')
+    dev, f32 = step.device, torch.float32
+    pt, gt = (params[0].dtype, grads[0].dtype) if n else (f32, f32)
+    num = [t.numel() for t in params]
+    # the usual case in passes over the lists, a few of a tensor's properties each (a step of a model has the time of ~50 tensors in the kernel)
+    good = step.is_cuda and pt in _FLOATS and gt in _FLOATS
+    if good:
+        at, mt = step.get_device(), torch.float8_e4m3fn if q8 else f32
+        for ts, dt, want in ((params, pt, num), (grads, gt, num), (ms, mt, num), (vs, mt, num)):
+            for t, k in zip(ts, want):
+                if not (t.dtype is dt and t.numel() == k and t.is_contiguous() and t.get_device() == at):
+                    good = False
+        if q8:
+            for ts in (sm, sr):
+                for t, k in zip(ts, num):
+                    if not (t.dtype is f32 and t.numel() == (k + Q8_BLOCK - 1) // Q8_BLOCK and t.is_contiguous() and t.get_device() == at):
+                        good = False
+    if not good:
+        _adamw_check(params, grads, ms, vs, sm, sr, q8, dev, pt, gt, num)
     if n == 0:
         return
     pp = _ptrs(params)
     _need(len(set(pp)) >= n - num.count(0), 'adamw_step: a parameter is listed twice')
     with _on(step):
         st, gp = _stream(), None if guard is None else guard.data_ptr()
-        check(lib.ha2g_adam_step_inc_guarded(step.data_ptr(), gp, st))
-        check(lib.ha2g_adamw_multi(n, pp, _ptrs(grads), _ptrs(ms), _ptrs(vs), _ptrs(sm) if q8 else None, _ptrs(sr) if q8 else None,
-                                   array.array('l', num), int(torch.bfloat16 in pt), int(torch.bfloat16 in gt), 8 if q8 else 32, float(lr), float(betas[0]),
-                                   float(betas[1]), float(eps), float(weight_decay), int(seed) & 0xffffffff, 0, step.data_ptr(), gp, st))
+        sc = torch.empty(4, dtype=f32, device=dev)
+        sp = sc.data_ptr()
+        b1, b2, lr = float(betas[0]), float(betas[1]), float(lr)
+        check(lib.ha2g_adamw_scalars(step.data_ptr(), gp, lr, b1, b2, sp, st))
+        check(lib.ha2g_adamw_multi(n, pp, _ptrs(grads), _ptrs(ms), _ptrs(vs), _ptrs(sm) if q8 else None, _ptrs(sr) if q8 else None, array.array('l', num),
+                                   pt is torch.bfloat16, gt is torch.bfloat16, 8 if q8 else 32, lr, b1, b2, float(eps), float(weight_decay),
+                                   int(seed) & 0xffffffff, 0, sp, gp, st))
+
+
+def _adamw_check(params, grads, ms, vs, sm, sr, q8, dev, pt, gt, num):
+    """what adamw_step's quick pass did not cover: tensors that are dense in another order of dimensions, and everything that is refused"""
+    every = [*params, *grads, *ms, *vs, *sm, *sr]
+    _need(all(isinstance(t, torch.Tensor) for t in every), 'adamw_step: lists of tensors (8-bit states: of pairs)')
+    _need({t.device for t in every} <= {dev}, 'adamw_step: everything lies on the device of step')
+    _need({pt, gt} <= set(_FLOATS) and all(t.dtype == pt for t in params) and all(t.dtype == gt for t in grads),
+          'adamw_step: parameters %s, gradients %s (one of fp32, bf16 each)', pt, gt)
+    for p, g in zip(params, grads):
+        _need(_dense(p) and _alike(p, g), 'adamw_step: a gradient %s %s for a parameter %s %s', tuple(g.shape), g.stride(), tuple(p.shape), p.stride())
+    if q8:
+        _need(all(t.dtype == torch.float8_e4m3fn for t in (*ms, *vs)) and all(t.dtype == torch.float32 for t in (*sm, *sr)),
+              'adamw_step: 8-bit states are float8_e4m3fn codes and fp32 scales')
+        blocks = [-(-k // Q8_BLOCK) for k in num]
+        _need(all(t.is_contiguous() for st in (ms, vs, sm, sr) for t in st) and [t.numel() for t in ms] == num == [t.numel() for t in vs] and
+              [t.numel() for t in sm] == blocks == [t.numel() for t in sr], 'adamw_step: 8-bit states of other sizes than their parameters')
+    else:
+        _need(all(t.dtype == torch.float32 for t in (*ms, *vs)), 'adamw_step: states are fp32 tensors, or pairs for 8 bits')
+        for p, m, v in zip(params, ms, vs):
+            _need(_alike(p, m) and _alike(p, v), 'adamw_step: a state %s %s for a parameter %s %s', tuple(m.shape), m.stride(), tuple(p.shape), p.stride())
+    _need(dev.type == 'cuda', 'adamw_step: GPU tensors (there is no CPU path)')
 
 
 class FusedAdamW(FusedAdam):
@@ -204,6 +225,7 @@ class FusedAdamW(FusedAdam):
 
     def _make_states(self, ps, offs, total, dev):
         cut = lambda t: [t[o:o + p.numel()] for p, o in zip(ps, offs)]      # noqa: E731
+        self._scalars = torch.zeros(4, dtype=torch.float32, device=dev)
         if self.state_bits == 32:
             super()._make_states(ps, offs, total, dev)
             ms, vs, sm, sr = cut(self.flat_m), cut(self.flat_v), None, None
@@ -227,9 +249,10 @@ class FusedAdamW(FusedAdam):
         with _on(self.flat_p):
             st, guard = _stream(), gru_cluster_error_tensor(self.flat_p.device)
             gp = guard.data_ptr() if guard is not None else None
-            check(lib.ha2g_adam_step_inc_guarded(self.step_t.data_ptr(), gp, st))
+            b1, b2, sp = float(g['betas'][0]), float(g['betas'][1]), self._scalars.data_ptr()
+            check(lib.ha2g_adamw_scalars(self.step_t.data_ptr(), gp, float(g['lr']), b1, b2, sp, st))
             first = 0
             for (n, p, gr, m, v, sm, sr, num), wd in zip(self._tables, (float(g['weight_decay']), 0.0)):
-                check(lib.ha2g_adamw_multi(n, p, gr, m, v, sm, sr, num, 0, 0, self.state_bits, float(g['lr']), float(g['betas'][0]), float(g['betas'][1]),
-                                           float(g['eps']), wd, self.seed & 0xffffffff, first, self.step_t.data_ptr(), gp, st))
+                check(lib.ha2g_adamw_multi(n, p, gr, m, v, sm, sr, num, 0, 0, self.state_bits, float(g['lr']), b1, b2, float(g['eps']), wd,
+                                           self.seed & 0xffffffff, first, sp, gp, st))
                 first += n
