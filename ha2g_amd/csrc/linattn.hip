@@ -42,7 +42,8 @@ template <> __device__ __forceinline__ void st1<b16>(b16* p, long i, float v) {
 // A workgroup owns a (batch row, head, segment of the time axis); its waves split the columns of v, each keeps its Dk x DVW slice of S in MFMA
 // accumulators for the whole segment.  The accumulator layout (column = lane & 15, row = 4 (lane >> 4) + i) is that of an operand whose k runs along
 // the rows, up to an order of k that both operands may share: S and the scores k q^T go from accumulators into the next product without
-// touching LDS.  Every wave forms the scores for itself (a fifth of its products) rather than meet the others at a barrier.
+// touching LDS.  Rows of LDS are padded by 32 bytes: 16-byte reads of 16 rows and transpose reads of 4 x 16 blocks meet every bank once (row reads
+// of 2 x 8 bytes had two thirds of the LDS time in conflicts).  Every wave forms the scores for itself (a fifth of its products) rather than meet the others at a barrier.
 //     o^T = S^T q^T + v^T (k q^T):  a lane ends with 4 consecutive columns of one token.
 // fp32 operands run on the fp32 MFMA.  bf16 operands are exact as they are; what is computed is split into bf16 pieces: S and the scores, which
 // only reach the bf16 result, into two (2^-17), the decayed v that is added to S into three (all 24 bits: S stays fp32-exact).
@@ -72,6 +73,8 @@ template <> struct Mma<float> {
         for (int i = 0; i < 4; ++i) f[i] = p[(16 * u + 4 * i + (lane >> 4)) * ld + c0 + (lane & 15)];
         return f;
     }
+    __device__ __forceinline__ static Frag state_col(const float* p, int ld, int x, int u, int lane) { return col(p, ld, 16 * x, u, lane); }
+    __device__ __forceinline__ static int state_row(int x, int g) { return 16 * x + 4 * g; }
     template <int N> __device__ __forceinline__ static void pieces(const f32x4* x, Frag* out) { out[0] = x[0]; }
     __device__ __forceinline__ static void scaled(Frag f, const float* w, f32x4* x) {
 #pragma unroll
@@ -84,17 +87,19 @@ template <> struct Mma<b16> {
     __device__ __forceinline__ static int srow(int g, int i) { return 4 * g + i; }
     __device__ __forceinline__ static int krow(int m) { return m; }
     __device__ __forceinline__ static f32x4 mma(Frag a, Frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
-    __device__ __forceinline__ static Frag row(const b16* p, int ld, int r, int u, int g) {
-        const s16x4_t a = *reinterpret_cast<const s16x4_t*>(p + r * ld + 32 * u + 4 * g), b = *reinterpret_cast<const s16x4_t*>(p + r * ld + 32 * u + 16 + 4 * g);
-        return __builtin_bit_cast(bf16x8_t, (s16x8_t)__builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
-    }
+    __device__ __forceinline__ static Frag row(const b16* p, int ld, int r, int u, int g) { return *reinterpret_cast<const bf16x8_t*>(p + r * ld + 32 * u + 8 * g); }
     // transpose reads: 16 lanes read a [4 rows][16 columns] block row-major, each gets the 4 rows of its own column
-    __device__ __forceinline__ static Frag col(const b16* p, int ld, int c0, int u, int lane) {
-        const b16* q = p + (32 * u + 4 * (lane >> 4) + ((lane & 15) >> 2)) * ld + c0 + 4 * (lane & 3);
-        const s16x4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4_t)(__attribute__((address_space(3))) const b16*)q);
-        const s16x4_t b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4_t)(__attribute__((address_space(3))) const b16*)(q + 16 * ld));
-        return __builtin_bit_cast(bf16x8_t, (s16x8_t)__builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+    __device__ __forceinline__ static s16x4_t tr(const b16* q) { return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4_t)(__attribute__((address_space(3))) const b16*)q); }
+    __device__ __forceinline__ static Frag cols(const b16* p, int ld, int u, int lane) {
+        const b16* q = p + (32 * u + 4 * (lane >> 4) + ((lane & 15) >> 2)) * ld;
+        return __builtin_bit_cast(bf16x8_t, (s16x8_t)__builtin_shufflevector(tr(q), tr(q + 16 * ld), 0, 1, 2, 3, 4, 5, 6, 7));
     }
+    __device__ __forceinline__ static Frag col(const b16* p, int ld, int c0, int u, int lane) { return cols(p + c0 + 4 * (lane & 3), ld, u, lane); }
+    // the columns of state tile x: tiles 2 y and 2 y + 1 take every other four of 32, so that a lane's rows of both are 8 neighbours, as row() reads them
+    __device__ __forceinline__ static Frag state_col(const b16* p, int ld, int x, int u, int lane) {
+        return cols(p + 32 * (x >> 1) + 4 * (x & 1) + 8 * (lane & 3), ld, u, lane);
+    }
+    __device__ __forceinline__ static int state_row(int x, int g) { return 32 * (x >> 1) + 4 * (x & 1) + 8 * g; }
     template <int N> __device__ __forceinline__ static void pieces(const f32x4* x, Frag* out) {
         u32x4_t w[N];
 #pragma unroll
@@ -211,7 +216,7 @@ __global__ __launch_bounds__(waves_of(DVP) * 64, 2) void linattn_chunk_kernel(co
         for (int y = 0; y < VT; ++y)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int d = 16 * x + 4 * grp + i, j = v0 + 16 * y + col;
+                const int d = M::state_row(x, grp) + i, j = v0 + 16 * y + col;
                 S[x][y][i] = (s_in && d < Dk && j < Dv) ? s_in[(long)d * si + (long)j * sj] : 0.f;
             }
 
@@ -351,7 +356,7 @@ __global__ __launch_bounds__(waves_of(DVP) * 64, 2) void linattn_chunk_kernel(co
             }
 #pragma unroll
             for (int x = 0; x < KT; ++x) {
-                const typename M::Frag kf = M::col(ks, SK::LD, 16 * x, u, lane);
+                const typename M::Frag kf = M::state_col(ks, SK::LD, x, u, lane);
 #pragma unroll
                 for (int y = 0; y < VT; ++y)
 #pragma unroll
@@ -380,7 +385,7 @@ __global__ __launch_bounds__(waves_of(DVP) * 64, 2) void linattn_chunk_kernel(co
         for (int y = 0; y < VT; ++y)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int d = 16 * x + 4 * grp + i, j = v0 + 16 * y + col;
+                const int d = M::state_row(x, grp) + i, j = v0 + 16 * y + col;
                 if (d < Dk && j < Dv) s_out[(long)d * oi + (long)j * oj] = S[x][y][i];
             }
 }
