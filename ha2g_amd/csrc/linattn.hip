@@ -37,13 +37,13 @@ template <> __device__ __forceinline__ void st1<b16>(b16* p, long i, float v) {
 }
 
 // ---- chunked form --------------------------------------------------------------------------------------------------------------------------
-// C tokens at a time (fp32: 32, bf16: 64; half of it for Dk > 64), positions i, j inside the chunk, e = 1 forward and 0 from the end:
+// C tokens at a time (fp32: 32, bf16: 64), positions i, j inside the chunk, e = 1 forward and 0 from the end:
 //     o_i = e^{g (i + e)} q_i S + sum_{j <= i} e^{g (i - j)} (q_i k_j) v_j,        S <- e^{g C} S + sum_j e^{g (C - e - j)} k_j v_j^T
 // A workgroup owns a (batch row, head, segment of the time axis); its waves split the columns of v, each keeps its Dk x DVW slice of S in MFMA
 // accumulators for the whole segment.  The accumulator layout (column = lane & 15, row = 4 (lane >> 4) + i) is that of an operand whose k runs along
 // the rows, up to an order of k that both operands may share: S and the scores k q^T go from accumulators into the next product without
-// touching LDS.  Rows of LDS are padded by 32 bytes: 16-byte reads of 16 rows and transpose reads of 4 x 16 blocks meet every bank once (row reads
-// of 2 x 8 bytes had two thirds of the LDS time in conflicts).  Every wave forms the scores for itself (a fifth of its products) rather than meet the others at a barrier.
+// touching the state's LDS copy.  Rows of LDS are padded by 32 bytes: 16-byte reads of 16 rows and transpose reads of 4 x 16 blocks meet every bank once (row reads
+// of 2 x 8 bytes had two thirds of the LDS time in conflicts).
 //     o^T = S^T q^T + v^T (k q^T):  a lane ends with 4 consecutive columns of one token.
 // fp32 operands run on the fp32 MFMA.  bf16 operands are exact as they are; what is computed is split into bf16 pieces: S and the scores, which
 // only reach the bf16 result, into two (2^-17), the decayed v that is added to S into three (all 24 bits: S stays fp32-exact).
@@ -57,7 +57,7 @@ typedef __attribute__((address_space(3))) s16x4_t* lds4_t;
 template <typename T> struct Mma;
 template <> struct Mma<float> {
     typedef f32x4 Frag;
-    static constexpr int CMAX = 32, KB = 16, PADK = 16, NS = 1, NV = 1;      // longest chunk, k per fragment, LDS row padding, pieces of S / scores and of v
+    static constexpr int C = 32, KB = 16, PADK = 16, NS = 1, NV = 1;      // longest chunk, k per fragment, LDS row padding, pieces of S / scores and of v
     // row m of a score tile is token 4 (m & 3) + (m >> 2): the column reads below then take four neighbouring rows at once, without bank conflicts
     __device__ __forceinline__ static int srow(int g, int i) { return 4 * i + g; }
     __device__ __forceinline__ static int krow(int m) { return 4 * (m & 3) + (m >> 2); }
@@ -76,6 +76,9 @@ template <> struct Mma<float> {
     __device__ __forceinline__ static Frag state_col(const float* p, int ld, int x, int u, int lane) { return col(p, ld, 16 * x, u, lane); }
     __device__ __forceinline__ static int state_row(int x, int g) { return 16 * x + 4 * g; }
     template <int N> __device__ __forceinline__ static void pieces(const f32x4* x, Frag* out) { out[0] = x[0]; }
+    typedef f32x4 Tile;                // a score tile's four values of a lane, one per piece
+    __device__ __forceinline__ static void put(Tile* p, f32x4 z) { p[0] = z; }
+    __device__ __forceinline__ static Frag get(const Tile* p, bool) { return p[0]; }
     __device__ __forceinline__ static void scaled(Frag f, const float* w, f32x4* x) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) x[0][i] = f[i] * w[i];
@@ -83,7 +86,7 @@ template <> struct Mma<float> {
 };
 template <> struct Mma<b16> {
     typedef bf16x8_t Frag;
-    static constexpr int CMAX = 64, KB = 32, PADK = 16, NS = 2, NV = 3;
+    static constexpr int C = 64, KB = 32, PADK = 16, NS = 2, NV = 3;
     __device__ __forceinline__ static int srow(int g, int i) { return 4 * g + i; }
     __device__ __forceinline__ static int krow(int m) { return m; }
     __device__ __forceinline__ static f32x4 mma(Frag a, Frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
@@ -111,6 +114,20 @@ template <> struct Mma<b16> {
         }
 #pragma unroll
         for (int n = 0; n < N; ++n) out[n] = __builtin_bit_cast(bf16x8_t, w[n]);
+    }
+    typedef uint2 Tile;
+    __device__ __forceinline__ static void put(Tile* p, f32x4 z) {           // pieces 64 places apart
+        unsigned a[2], b[2];
+        splitn_bf16<2>(z[0], z[1], a);
+        splitn_bf16<2>(z[2], z[3], b);
+        p[0] = make_uint2(a[0], b[0]);
+        p[64] = make_uint2(a[1], b[1]);
+    }
+    __device__ __forceinline__ static Frag get(const Tile* p, bool two) {    // a tile and the next one
+        const uint2 a = p[0];
+        uint2 b = make_uint2(0u, 0u);
+        if (two) b = p[64 * NS];
+        return __builtin_bit_cast(bf16x8_t, u32x4_t{a.x, a.y, b.x, b.y});
     }
     __device__ __forceinline__ static void scaled(Frag f, const float* w, f32x4* x) {
         const u32x4_t u = __builtin_bit_cast(u32x4_t, f);
@@ -143,12 +160,26 @@ template <typename T, int D, int C, int NT, bool VEC> struct Stage {     // a ch
     static constexpr int E = 16 / sizeof(T), V = D / E, N = C * V / NT, LD = D + Mma<T>::PADK, RS = NT / V;
     static_assert(N * NT == C * V && RS * V == NT, "a chunk is a whole number of pieces per thread, a pass over the threads whole rows");
     u32x4_t r[N];
-    // rows: token `first` and on in steps of `step` elements (negative from the end); n of them exist
-    __device__ __forceinline__ void load(const T* first, long step, int n, int dim) {
-        const int row = threadIdx.x / V, c = threadIdx.x % V * E, left = dim - c;
-        const T* p = first + row * step + c;
+    // An address is what all threads share (64 bits, in scalar registers: chunk, row pass) plus 32 bits of the thread's own (row of the pass, piece).
+    const char* base;            // lowest row of the next chunk's first pass
+    unsigned off;
+    long pass, chunk;            // bytes from one row pass to the next, and from one chunk
+    int row, left;               // first row, elements of it from here on
+    // rows: token `first` and on in steps of `step` elements (negative from the end; less than 2^22)
+    __device__ __forceinline__ void start(const T* first, long step, int dim) {
+        row = threadIdx.x / V;
+        const int c = threadIdx.x % V * E, low = step < 0 ? RS - 1 - row : row;
+        left = dim - c;
+        base = (const char*)(first + (step < 0 ? (RS - 1) * step : 0));
+        off = (unsigned)(low * (int)(step < 0 ? -step : step) + c) * sizeof(T);
+        pass = RS * step * (long)sizeof(T);
+        chunk = C * step * (long)sizeof(T);
+    }
+    // the next chunk, of which n rows exist
+    __device__ __forceinline__ void load(int n) {
 #pragma unroll
-        for (int j = 0; j < N; ++j) r[j] = load16<T, VEC>(p + (long)(j * RS) * step, row + j * RS < n ? left : 0);
+        for (int j = 0; j < N; ++j) r[j] = load16<T, VEC>((const T*)(base + j * pass + off), row + j * RS < n ? left : 0);
+        base += chunk;
     }
     __device__ __forceinline__ void store(T* lds) const {
         T* p = lds + threadIdx.x / V * LD + threadIdx.x % V * E;
@@ -164,24 +195,30 @@ __device__ __forceinline__ int row_length(const LinAttnArgs& a, int b) { return 
 // share q, k or v find them in that XCD's L2.
 __device__ __forceinline__ long xcd_order(long i, long n) { return n % 8 == 0 ? i % 8 * (n / 8) + i / 8 : i; }
 
-constexpr int waves_of(int DVP) { return DVP < 64 ? DVP / 16 : 4; }
-// With Dk > 64 the state takes 64 registers of a wave: a chunk half as long leaves two waves per SIMD without spilling, and needs fewer score products.
-template <typename T> constexpr int chunk_of(int DKP) { return DKP > 64 ? Mma<T>::CMAX / 2 : Mma<T>::CMAX; }
+// Waves of a workgroup: 16 columns of v each, 32 where Dk and v are both long (or Dk is too short for eight waves to share its rows).  Dk = 64 with
+// 128 columns fits 128 registers, so that two workgroups of eight waves run on a compute unit (ragged prompts: 45 us, 50 with four waves);
+// Dk = 128 does not, and eight waves of one workgroup in step with each other are slower than two workgroups of four (164 us, 137).
+constexpr int waves_of(int DKP, int DVP) { return DVP < 64 ? DVP / 16 : (DKP == 64 && DVP == 128 ? 8 : 4); }
+constexpr int occupancy_of(int DKP, int DVP) { return waves_of(DKP, DVP) == 8 ? 4 : 2; }
+// With Dk > 64 the state takes up to 64 registers of a wave: a chunk half as long leaves room for two waves per SIMD.
+template <typename T> constexpr int chunk_of(int DKP) { return DKP > 64 ? Mma<T>::C / 2 : Mma<T>::C; }
 
 // STATE_ONLY: the segment's own contribution to the state (from zero), nothing is read of q and no o is written.  Two waves per SIMD at least:
 // one alone leaves matrix and vector units waiting for each other.
 template <typename T, int DKP, int DVP, bool STATE_ONLY, bool VEC>
-__global__ __launch_bounds__(waves_of(DVP) * 64, 2) void linattn_chunk_kernel(const LinAttnArgs a) {
+__global__ __launch_bounds__(waves_of(DKP, DVP) * 64, occupancy_of(DKP, DVP)) void linattn_chunk_kernel(const LinAttnArgs a) {
     typedef Mma<T> M;
-    constexpr int NW = waves_of(DVP), NT = NW * 64, DVW = DVP / NW, C = chunk_of<T>(DKP), KB = M::KB, TPF = KB / 16;
+    constexpr int NW = waves_of(DKP, DVP), NT = NW * 64, DVW = DVP / NW, C = chunk_of<T>(DKP), KB = M::KB, TPF = KB / 16;
     constexpr int KT = DKP / 16, KF = DKP / KB, VT = DVW / 16, CT = C / 16, CF = C / KB;
+    constexpr int TILES = CT * (CT + 1) / 2, MINE = (TILES + NW - 1) / NW;      // score tiles of a chunk (s <= t), and of a wave
     const Job& J = a.job[blockIdx.y];
     typedef Stage<T, DKP, C, NT, VEC> SK;
     typedef Stage<T, DVP, C, NT, VEC> SV;
     __shared__ __attribute__((aligned(16))) T qs[STATE_ONLY ? 8 : C * SK::LD];
     __shared__ __attribute__((aligned(16))) T ks[C * SK::LD];
     __shared__ __attribute__((aligned(16))) T vs[C * SV::LD];
-    const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4, v0 = (threadIdx.x >> 6) * DVW;
+    __shared__ __attribute__((aligned(16))) typename M::Tile ps[STATE_ONLY ? 1 : TILES * M::NS * 64];
+    const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4, wave = threadIdx.x >> 6, v0 = wave * DVW;
     const long wg = xcd_order(blockIdx.x, gridDim.x);
     const int h = (int)(wg % a.H), seg = (int)(wg / a.H % a.nseg), b = (int)(wg / a.H / a.nseg);
     const long bh = (long)b * a.H + h, D2 = (long)J.Dk * J.Dv;
@@ -199,9 +236,11 @@ __global__ __launch_bounds__(waves_of(DVP) * 64, 2) void linattn_chunk_kernel(co
     SK rq, rk;
     SV rv;
     if (beg < end) {
-        if constexpr (!STATE_ONLY) rq.load(q + beg * qt, qt, end - beg, Dk);
-        rk.load(k + beg * kt, kt, end - beg, Dk);
-        rv.load(v + beg * vt, vt, end - beg, Dv);
+        if constexpr (!STATE_ONLY) { rq.start(q + beg * qt, qt, Dk); rq.load(end - beg); }
+        rk.start(k + beg * kt, kt, Dk);
+        rk.load(end - beg);
+        rv.start(v + beg * vt, vt, Dv);
+        rv.load(end - beg);
     }
     f32x4 S[KT][VT];
     const float* s_in = nullptr;
@@ -210,39 +249,56 @@ __global__ __launch_bounds__(waves_of(DVP) * 64, 2) void linattn_chunk_kernel(co
         if (seg == 0) s_in = J.s_in ? J.s_in + bh * D2 : nullptr;
         else if (beg < n) { s_in = J.seg + (bh * (a.nseg - 1) + seg - 1) * D2; si = J.gi; sj = J.gj; }      // an empty segment computes nothing from it
     }
+    const int d_lane = M::state_row(0, grp), j_lane = v0 + col;        // this lane's first element; the others lie at offsets that all lanes share
+    const int at_lane = d_lane * si + j_lane * sj;
 #pragma unroll
     for (int x = 0; x < KT; ++x)
 #pragma unroll
         for (int y = 0; y < VT; ++y)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int d = M::state_row(x, grp) + i, j = v0 + 16 * y + col;
-                S[x][y][i] = (s_in && d < Dk && j < Dv) ? s_in[(long)d * si + (long)j * sj] : 0.f;
+                const int d = M::state_row(x, 0) + i, j = 16 * y;
+                S[x][y][i] = (s_in && d_lane + d < Dk && j_lane + j < Dv) ? (s_in + (d * si + j * sj))[at_lane] : 0.f;
             }
 
-    // powers of the decay: inside a tile (t - s >= 0, else nothing), x tiles further (t - s + 16 x >= 1), in front of a tile of tokens, to the chunk's end
-    float pw[CT][4], pin[CT], wst[CF][KB / 4];
+    // powers of the decay: between the tokens of this wave's score tiles (nothing where s > t), in front of a tile of tokens, to the chunk's end
+    float pw[MINE][4], pin[CT], wst[CF][KB / 4];
+    int tx[MINE], ts[MINE];
     if constexpr (!STATE_ONLY) {
 #pragma unroll
-        for (int x = 0; x < CT; ++x) {
+        for (int m = 0; m < MINE; ++m) {
+            const int id = wave + m * NW;
+            tx[m] = (id >= 1) + (id >= 3) + (id >= 6);
+            ts[m] = id - tx[m] * (tx[m] + 1) / 2;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int d = col - M::srow(grp, i) + 16 * x;
-                pw[x][i] = d >= 0 ? J.uscale * J.oscale * decay_power(g, d) : 0.f;
+                const int d = 16 * (tx[m] - ts[m]) + col - M::srow(grp, i);
+                pw[m][i] = d >= 0 ? J.uscale * J.oscale * decay_power(g, d) : 0.f;
             }
-            pin[x] = J.oscale * decay_power(g, col + 16 * x + e);
         }
     }
-    auto weights = [&](int L) {
+    float pt[CT];                                                    // whole tiles of tokens
 #pragma unroll
-        for (int u = 0; u < CF; ++u)
+    for (int x = 0; x < CT; ++x) pt[x] = decay_power(g, 16 * x);
+    if constexpr (!STATE_ONLY) {
+        const float p0 = J.oscale * decay_power(g, col + e);
 #pragma unroll
-            for (int j = 0; j < KB / 4; ++j) wst[u][j] = J.uscale * decay_power(g, max(0, L - e - (KB * u + 16 * (j >> 2) + M::srow(grp, j & 3))));
-    };
-    weights(C);
+        for (int x = 0; x < CT; ++x) pin[x] = p0 * pt[x];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float p0 = J.uscale * decay_power(g, 16 - e - M::srow(grp, i));
+#pragma unroll
+        for (int x = 0; x < CT; ++x) wst[x / TPF][4 * (x % TPF) + i] = p0 * pt[CT - 1 - x];
+    }
     float m1 = expm1f(g * (float)C);
 
-    for (int c0 = beg; c0 < end; c0 += C) {
+    // o likewise: the lowest row of 16 tokens, and this lane's place from there
+    const int osize = J.o16 ? 2 : 4;
+    const long ostep = dir * J.ot * osize;
+    char* obase16 = (char*)J.o + (obase + (t0 + dir * beg + (J.rev ? -15 : 0)) * J.ot) * osize;
+    const unsigned olane = (unsigned)((J.rev ? 15 - col : col) * (int)J.ot + v0 + 4 * grp) * osize;
+    for (int c0 = beg; c0 < end; c0 += C, obase16 += C * ostep) {
         __syncthreads();
         if constexpr (!STATE_ONLY) rq.store(qs);
         rk.store(ks);
@@ -250,9 +306,9 @@ __global__ __launch_bounds__(waves_of(DVP) * 64, 2) void linattn_chunk_kernel(co
         __syncthreads();
         const int L = min(C, end - c0), c1 = c0 + C;
         if (c1 < end) {
-            if constexpr (!STATE_ONLY) rq.load(q + c1 * qt, qt, end - c1, Dk);
-            rk.load(k + c1 * kt, kt, end - c1, Dk);
-            rv.load(v + c1 * vt, vt, end - c1, Dv);
+            if constexpr (!STATE_ONLY) rq.load(end - c1);
+            rk.load(end - c1);
+            rv.load(end - c1);
         }
         typename M::Frag vf[CF][VT];
 #pragma unroll
@@ -260,6 +316,18 @@ __global__ __launch_bounds__(waves_of(DVP) * 64, 2) void linattn_chunk_kernel(co
 #pragma unroll
             for (int y = 0; y < VT; ++y) vf[u][y] = M::col(vs, SV::LD, v0 + 16 * y, u, lane);
         if constexpr (!STATE_ONLY) {
+            // this wave's score tiles, for all
+#pragma unroll
+            for (int m = 0; m < MINE; ++m)
+                if (wave + m * NW < TILES) {
+                    f32x4 z = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int w = 0; w < KF; ++w)
+                        z = M::mma(M::row(ks, SK::LD, 16 * ts[m] + M::krow(col), w, grp), M::row(qs, SK::LD, 16 * tx[m] + col, w, grp), z);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) z[i] *= pw[m][i];
+                    M::put(ps + (wave + m * NW) * (M::NS * 64) + lane, z);
+                }
             f32x4 acc[CT][VT];
 #pragma unroll
             for (int x = 0; x < CT; ++x)
@@ -286,49 +354,40 @@ __global__ __launch_bounds__(waves_of(DVP) * 64, 2) void linattn_chunk_kernel(co
                 }
             }
 #pragma unroll
-            for (int x = 0; x < CT; ++x) {
+            for (int x = 0; x < CT; ++x)
 #pragma unroll
                 for (int y = 0; y < VT; ++y)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) acc[x][y][i] *= pin[x];
-                typename M::Frag qf[KF];
+            __syncthreads();                                     // the scores are there
 #pragma unroll
-                for (int u = 0; u < KF; ++u) qf[u] = M::row(qs, SK::LD, 16 * x + col, u, grp);
+            for (int x = 0; x < CT; ++x) {
 #pragma unroll
                 for (int u = 0; u * TPF <= x; ++u) {
-                    f32x4 t[TPF];
+                    const typename M::Tile* t = ps + (x * (x + 1) / 2 + u * TPF) * (M::NS * 64) + lane;
 #pragma unroll
-                    for (int p = 0; p < TPF; ++p) {
-                        const int s = u * TPF + p;
-                        t[p] = f32x4{0.f, 0.f, 0.f, 0.f};
-                        if (s > x) continue;
+                    for (int p = M::NS - 1; p >= 0; --p) {
+                        const typename M::Frag pf = M::get(t + 64 * p, u * TPF + 1 <= x);
 #pragma unroll
-                        for (int w = 0; w < KF; ++w) t[p] = M::mma(M::row(ks, SK::LD, 16 * s + M::krow(col), w, grp), qf[w], t[p]);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) t[p][i] *= pw[x - s][i];
+                        for (int y = 0; y < VT; ++y) acc[x][y] = M::mma(vf[u][y], pf, acc[x][y]);
                     }
-                    typename M::Frag pf[M::NS];
-                    M::template pieces<M::NS>(t, pf);
-#pragma unroll
-                    for (int y = 0; y < VT; ++y)
-#pragma unroll
-                        for (int p = M::NS - 1; p >= 0; --p) acc[x][y] = M::mma(vf[u][y], pf[p], acc[x][y]);
                 }
                 const int r = 16 * x + col;
                 if (r < L) {
-                    const long row = obase + (t0 + dir * (c0 + r)) * J.ot;
+                    char* const row = obase16 + 16 * x * ostep;
 #pragma unroll
                     for (int y = 0; y < VT; ++y) {
                         const int j = v0 + 16 * y + 4 * grp;
-                        const float4 w = make_float4(acc[x][y][0], acc[x][y][1], acc[x][y][2], acc[x][y][3]);
                         if (j >= Dv) continue;
+                        char* const at = row + 16 * y * osize + olane;
+                        const float4 w = make_float4(acc[x][y][0], acc[x][y][1], acc[x][y][2], acc[x][y][3]);
                         if (J.ovec) {
-                            if (J.o16) st4((b16*)J.o + row + j, 0, w); else st4((float*)J.o + row + j, 0, w);
+                            if (J.o16) st4((b16*)at, 0, w); else st4((float*)at, 0, w);
                         } else {
                             const float f[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
                             for (int i = 0; i < 4; ++i)
-                                if (j + i < Dv) { if (J.o16) st1((b16*)J.o, row + j + i, f[i]); else st1((float*)J.o, row + j + i, f[i]); }
+                                if (j + i < Dv) { if (J.o16) st1((b16*)at, i, f[i]); else st1((float*)at, i, f[i]); }
                         }
                     }
                 }
@@ -336,7 +395,11 @@ __global__ __launch_bounds__(waves_of(DVP) * 64, 2) void linattn_chunk_kernel(co
         }
         // the state
         if (L < C) {                                               // the last chunk of a row
-            weights(L);
+#pragma unroll
+            for (int u = 0; u < CF; ++u)
+#pragma unroll
+                for (int j = 0; j < KB / 4; ++j)
+                    wst[u][j] = J.uscale * decay_power(g, max(0, L - e - (KB * u + 16 * (j >> 2) + M::srow(grp, j & 3))));
             m1 = expm1f(g * (float)L);
         }
 #pragma unroll
@@ -379,14 +442,15 @@ __global__ __launch_bounds__(waves_of(DVP) * 64, 2) void linattn_chunk_kernel(co
         if (!J.s_out || seg != (n > 0 ? (n - 1) / a.seg_len : 0)) return;      // the segment with the row's last token
         s_out = J.s_out + bh * D2;
     }
+    const int out_lane = d_lane * oi + j_lane * oj;
 #pragma unroll
     for (int x = 0; x < KT; ++x)
 #pragma unroll
         for (int y = 0; y < VT; ++y)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int d = M::state_row(x, grp) + i, j = v0 + 16 * y + col;
-                if (d < Dk && j < Dv) s_out[(long)d * oi + (long)j * oj] = S[x][y][i];
+                const int d = M::state_row(x, 0) + i, j = 16 * y;
+                if (d_lane + d < Dk && j_lane + j < Dv) (s_out + (d * oi + j * oj))[out_lane] = S[x][y][i];
             }
 }
 
@@ -486,7 +550,7 @@ __global__ __launch_bounds__(256) void head_sum_kernel(const float* __restrict__
 // Segments of the time axis: one pass over q, k, v where the rows and heads alone give every compute unit a workgroup or more; otherwise the axis is
 // split so that two are there, at no less than four chunks a segment, for a second read of k and v and the segments' states.
 void segments(int B, int T, int H, int b16_io, int* nseg, int* len) {
-    const int C = b16_io ? Mma<b16>::CMAX : Mma<float>::CMAX, chunks = (int)(((long)T + C - 1) / C), cus = hw_cu_count();
+    const int C = b16_io ? Mma<b16>::C : Mma<float>::C, chunks = (int)(((long)T + C - 1) / C), cus = hw_cu_count();
     const long rows = (long)B * H;
     long want = rows >= cus || rows < 1 ? 1 : (2L * cus + rows - 1) / rows;
     if (want > chunks / 4) want = chunks / 4;
@@ -497,7 +561,7 @@ void segments(int B, int T, int H, int b16_io, int* nseg, int* len) {
 }
 
 template <typename T, int DKP, int DVP> void chunk_launch(const LinAttnArgs& a, int jobs, bool state_only, hipStream_t st) {
-    const dim3 grid((unsigned)((long)a.B * a.H * a.nseg), jobs), block(waves_of(DVP) * 64);
+    const dim3 grid((unsigned)((long)a.B * a.H * a.nseg), jobs), block(waves_of(DKP, DVP) * 64);
     bool vec = true;
     for (int j = 0; j < jobs; ++j) vec = vec && a.job[j].q.vec && a.job[j].k.vec && a.job[j].v.vec;
     if (state_only) {
@@ -531,6 +595,8 @@ int run_scan(const LinAttnArgs& a, hipStream_t st) {
     return 0;
 }
 int tile_of(int d) { return d <= 32 ? 32 : (d <= 64 ? 64 : 128); }
+
+constexpr long STRIDE_LIMIT = 1L << 22;      // of a token, in elements: a workgroup's rows lie within 32 bits of each other
 
 // rows of D elements are whole pieces of `bytes`, also from one row to the next
 bool pieces_ok(const void* p, const long* s, int D, int elem, int bytes) {
@@ -578,6 +644,8 @@ int ha2g_linattn_fwd(const void* q, const void* k, const void* v, void* o, const
     LinAttnArgs a;
     if (const int rc = check_args(a, "linattn_fwd", log_decay, lengths, B, T, H, rq, rk, rv, Dk, Dv, b16_io, q && k && v && o)) return rc;
     if (B == 0) return 0;
+    for (int i = 1; i < 12; i += 3)
+        HA2G_REQUIRE(strides[i] >= 0 && strides[i] < STRIDE_LIMIT, "linattn_fwd: a token stride of %ld elements (0 to %ld)", strides[i], STRIDE_LIMIT - 1);
     HA2G_REQUIRE(a.nseg == 1 || ws, "linattn_fwd: no workspace (ha2g_linattn_workspace_floats)");
     const int e = b16_io ? 2 : 4;
     Job& j = a.job[0];
@@ -600,6 +668,8 @@ int ha2g_linattn_bwd(const void* q, const void* k, const void* v, const void* do
     if (const int rc = check_args(a, "linattn_bwd", log_decay, lengths, B, T, H, rq, rk, rv, Dk, Dv, b16_io, q && k && v && dout)) return rc;
     HA2G_REQUIRE(B == 0 || dv || !ds_in || T == 0, "linattn_bwd: the gradient of the first state comes with dv");
     if (B == 0) return 0;
+    for (int i = 1; i < 21; i += 3)
+        HA2G_REQUIRE(strides[i] >= 0 && strides[i] < STRIDE_LIMIT, "linattn_bwd: a token stride of %ld elements (0 to %ld)", strides[i], STRIDE_LIMIT - 1);
     HA2G_REQUIRE(a.nseg == 1 || (ws && (ws_fwd || !dq)), "linattn_bwd: no workspace (ha2g_linattn_workspace_floats)");
     const int e = b16_io ? 2 : 4;
     const Operand oq_ = operand(q, strides, rq, Dk, e), ok_ = operand(k, strides + 3, rk, Dk, e), ov_ = operand(v, strides + 6, rv, Dv, e),

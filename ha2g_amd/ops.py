@@ -1934,6 +1934,12 @@ def _inner1(x):
     return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
 
 
+def _rows(x):
+    """[B, T, H, D] as the kernels read it: unit inner stride, tokens less than 2^22 elements apart"""
+    st = x.stride()
+    return x if (st[3] == 1 or x.shape[3] == 1) and st[1] < 4194304 else x.contiguous()
+
+
 _FLOATS = (torch.float32, torch.bfloat16)
 
 
@@ -1974,7 +1980,7 @@ def _la_forward(q, k, v, log_decay, scale, state, lengths, want_state):
     B, T, Hq, Dk = q.shape
     H, Hk, Hv, Dv = log_decay.shape[0], k.shape[2], v.shape[2], v.shape[3]
     dev, bf = q.device, q.dtype == torch.bfloat16
-    q, k, v = _inner1(q), _inner1(k), _inner1(v)
+    q, k, v = _rows(q), _rows(k), _rows(v)
     with _on(q):
         o = torch.empty((B, T, H, Dv), dtype=q.dtype, device=dev)
         s = torch.empty((B, H, Dk, Dv), dtype=torch.float32, device=dev) if want_state else None
@@ -2016,7 +2022,7 @@ class LinearAttentionFunction(torch.autograd.Function):
                 do = torch.zeros((1, 1, 1, Dv), dtype=dt, device=dev).expand(B, T, H, Dv)
             if ds is not None:
                 ds = ds.contiguous()
-            q, k, v, do = _inner1(q), _inner1(k), _inner1(v), _inner1(do)
+            q, k, v, do = _rows(q), _rows(k), _rows(v), _rows(do)
 
             def grad(Hx, D):                # per-head sums in fp32 first where several heads read one
                 return torch.empty((B, T, H, D), dtype=dt if Hx == H else torch.float32, device=dev)

@@ -6,6 +6,7 @@ weights stay OHWI) and installs `.grad` views into a matching flat gradient buff
 HBM-streaming kernel, and data-parallel gradient exchange is ONE RCCL all-reduce per module (ha2g_amd/ddp.py).
 """
 import array
+import operator
 
 import torch
 
@@ -115,6 +116,9 @@ class FusedAdam(torch.optim.Optimizer):
         return ddp.average_(self.flat_g, group, async_op)
 
 
+# a tensor's properties as functions: passes over the lists of a model's tensors run in map()
+_numel, _address, _contiguous, _device = torch.Tensor.numel, torch.Tensor.data_ptr, torch.Tensor.is_contiguous, torch.Tensor.get_device
+_dtype = operator.attrgetter('dtype')
 Q8_BLOCK = 128            # consecutive elements of a tensor that share a scale of an 8-bit state
 
 
@@ -136,7 +140,7 @@ def _dense(t):
 
 
 def _ptrs(ts):
-    return array.array('l', [t.data_ptr() for t in ts])
+    return array.array('l', map(_address, ts))
 
 
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, seed=0, guard=None):
@@ -158,20 +162,17 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9, 
         ms, vs, sm, sr = exp_avgs, exp_avg_sqs, (), ()
     dev, f32 = step.device, torch.float32
     pt, gt = (params[0].dtype, grads[0].dtype) if n else (f32, f32)
-    num = [t.numel() for t in params]
+    num = list(map(_numel, params))
     # the usual case in passes over the lists, a few of a tensor's properties each (a step of a model has the time of ~50 tensors in the kernel)
     good = step.is_cuda and pt in _FLOATS and gt in _FLOATS
     if good:
         at, mt = step.get_device(), torch.float8_e4m3fn if q8 else f32
-        for ts, dt, want in ((params, pt, num), (grads, gt, num), (ms, mt, num), (vs, mt, num)):
-            for t, k in zip(ts, want):
-                if not (t.dtype is dt and t.numel() == k and t.is_contiguous() and t.get_device() == at):
-                    good = False
+        lists = [(params, pt, num), (grads, gt, num), (ms, mt, num), (vs, mt, num)]
         if q8:
-            for ts in (sm, sr):
-                for t, k in zip(ts, num):
-                    if not (t.dtype is f32 and t.numel() == (k + Q8_BLOCK - 1) // Q8_BLOCK and t.is_contiguous() and t.get_device() == at):
-                        good = False
+            blocks = [(k + Q8_BLOCK - 1) // Q8_BLOCK for k in num]
+            lists += [(sm, f32, blocks), (sr, f32, blocks)]
+        for ts, dt, want in lists:
+            good = good and list(map(_numel, ts)) == want and set(map(_dtype, ts)) <= {dt} and all(map(_contiguous, ts)) and set(map(_device, ts)) <= {at}
     if not good:
         _adamw_check(params, grads, ms, vs, sm, sr, q8, dev, pt, gt, num)
     if n == 0:
