@@ -8,7 +8,7 @@
 
 namespace {
 
-struct Operand { const void* p; long b, t, h; int r, vec; };      // element strides of batch row, token, head; head h reads head h / r; 16-byte pieces possible
+struct Operand { const void* p; long b, t, h; int r; };      // element strides of batch row, token, head; head h reads head h / r
 
 // one recurrence: reads q k v, adds k v^T, writes o
 struct Job {
@@ -18,7 +18,7 @@ struct Job {
     const float* s_in;           // states in front of the first token, one after another for (b, h), element (i, j) at i * si + j * sj; nullptr = zero
     float* s_out;                // those behind the last one, laid out alike, or nullptr
     float* seg;                  // [B * H][nseg - 1] states between the segments, element (i, j) at i * gi + j * gj
-    int si, sj, gi, gj, Dk, Dv, rev, o16, ovec;
+    int si, sj, gi, gj, Dk, Dv, rev, o16;
     float oscale, uscale;        // on what is read, on what is added
 };
 struct LinAttnArgs {
@@ -139,24 +139,34 @@ template <> struct Mma<b16> {
     }
 };
 
-// 16 bytes of a row of which `left` elements exist; VEC: rows are whole 16-byte pieces
-template <typename T, bool VEC> __device__ __forceinline__ u32x4_t load16(const T* p, int left) {
+// 16 bytes of a row, at any address, of which `left` elements exist; WHOLE: all or none
+typedef u32x4_t u32x4_a2 __attribute__((aligned(2)));
+typedef unsigned u32x2_a2 __attribute__((ext_vector_type(2), aligned(2)));
+template <typename T, bool WHOLE> __device__ __forceinline__ u32x4_t load16(const T* p, int left) {
     constexpr int E = 16 / sizeof(T);
     u32x4_t r = {0u, 0u, 0u, 0u};
-    if constexpr (VEC) {
-        if (left > 0) r = *reinterpret_cast<const u32x4_t*>(p);
-    } else {
+    if (WHOLE ? left > 0 : left >= E) r = *reinterpret_cast<const u32x4_a2*>(p);
+    else if constexpr (!WHOLE) {
+        if (left > 0)
 #pragma unroll
-        for (int j = 0; j < E; ++j)
-            if (j < left) {
-                if constexpr (sizeof(T) == 4) r[j] = __float_as_uint(p[j]);
-                else r[j >> 1] |= (unsigned)p[j] << (16 * (j & 1));
-            }
+            for (int j = 0; j < E - 1; ++j)
+                if (j < left) {
+                    if constexpr (sizeof(T) == 4) r[j] = __float_as_uint(p[j]);
+                    else r[j >> 1] |= (unsigned)p[j] << (16 * (j & 1));
+                }
     }
     return r;
 }
+__device__ __forceinline__ void store4(float* p, const f32x4& v) { *reinterpret_cast<u32x4_a2*>(p) = __builtin_bit_cast(u32x4_t, v); }
+__device__ __forceinline__ void store4(b16* p, const f32x4& v) {
+    unsigned a, b, l;
+    split2_bf16(v[0], v[1], a, l);
+    split2_bf16(v[2], v[3], b, l);
+    const u32x2_a2 w = {a, b};
+    *reinterpret_cast<u32x2_a2*>(p) = w;
+}
 
-template <typename T, int D, int C, int NT, bool VEC> struct Stage {     // a chunk of one operand: registers on the way from memory to LDS
+template <typename T, int D, int C, int NT, bool WHOLE> struct Stage {     // a chunk of one operand: registers on the way from memory to LDS
     static constexpr int E = 16 / sizeof(T), V = D / E, N = C * V / NT, LD = D + Mma<T>::PADK, RS = NT / V;
     static_assert(N * NT == C * V && RS * V == NT, "a chunk is a whole number of pieces per thread, a pass over the threads whole rows");
     u32x4_t r[N];
@@ -178,7 +188,7 @@ template <typename T, int D, int C, int NT, bool VEC> struct Stage {     // a ch
     // the next chunk, of which n rows exist
     __device__ __forceinline__ void load(int n) {
 #pragma unroll
-        for (int j = 0; j < N; ++j) r[j] = load16<T, VEC>((const T*)(base + j * pass + off), row + j * RS < n ? left : 0);
+        for (int j = 0; j < N; ++j) r[j] = load16<T, WHOLE>((const T*)(base + j * pass + off), row + j * RS < n ? left : 0);
         base += chunk;
     }
     __device__ __forceinline__ void store(T* lds) const {
@@ -205,15 +215,15 @@ template <typename T> constexpr int chunk_of(int DKP) { return DKP > 64 ? Mma<T>
 
 // STATE_ONLY: the segment's own contribution to the state (from zero), nothing is read of q and no o is written.  Two waves per SIMD at least:
 // one alone leaves matrix and vector units waiting for each other.
-template <typename T, int DKP, int DVP, bool STATE_ONLY, bool VEC>
+template <typename T, int DKP, int DVP, bool STATE_ONLY, bool WHOLE>
 __global__ __launch_bounds__(waves_of(DKP, DVP) * 64, occupancy_of(DKP, DVP)) void linattn_chunk_kernel(const LinAttnArgs a) {
     typedef Mma<T> M;
     constexpr int NW = waves_of(DKP, DVP), NT = NW * 64, DVW = DVP / NW, C = chunk_of<T>(DKP), KB = M::KB, TPF = KB / 16;
     constexpr int KT = DKP / 16, KF = DKP / KB, VT = DVW / 16, CT = C / 16, CF = C / KB;
     constexpr int TILES = CT * (CT + 1) / 2, MINE = (TILES + NW - 1) / NW;      // score tiles of a chunk (s <= t), and of a wave
     const Job& J = a.job[blockIdx.y];
-    typedef Stage<T, DKP, C, NT, VEC> SK;
-    typedef Stage<T, DVP, C, NT, VEC> SV;
+    typedef Stage<T, DKP, C, NT, WHOLE> SK;
+    typedef Stage<T, DVP, C, NT, WHOLE> SV;
     __shared__ __attribute__((aligned(16))) T qs[STATE_ONLY ? 8 : C * SK::LD];
     __shared__ __attribute__((aligned(16))) T ks[C * SK::LD];
     __shared__ __attribute__((aligned(16))) T vs[C * SV::LD];
@@ -380,14 +390,12 @@ __global__ __launch_bounds__(waves_of(DKP, DVP) * 64, occupancy_of(DKP, DVP)) vo
                         const int j = v0 + 16 * y + 4 * grp;
                         if (j >= Dv) continue;
                         char* const at = row + 16 * y * osize + olane;
-                        const float4 w = make_float4(acc[x][y][0], acc[x][y][1], acc[x][y][2], acc[x][y][3]);
-                        if (J.ovec) {
-                            if (J.o16) st4((b16*)at, 0, w); else st4((float*)at, 0, w);
+                        if (j + 4 <= Dv) {
+                            if (J.o16) store4((b16*)at, acc[x][y]); else store4((float*)at, acc[x][y]);
                         } else {
-                            const float f[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                if (j + i < Dv) { if (J.o16) st1((b16*)at, i, f[i]); else st1((float*)at, i, f[i]); }
+                            for (int i = 0; i < 3; ++i)
+                                if (j + i < Dv) { if (J.o16) st1((b16*)at, i, acc[x][y][i]); else st1((float*)at, i, acc[x][y][i]); }
                         }
                     }
                 }
@@ -562,13 +570,14 @@ void segments(int B, int T, int H, int b16_io, int* nseg, int* len) {
 
 template <typename T, int DKP, int DVP> void chunk_launch(const LinAttnArgs& a, int jobs, bool state_only, hipStream_t st) {
     const dim3 grid((unsigned)((long)a.B * a.H * a.nseg), jobs), block(waves_of(DKP, DVP) * 64);
-    bool vec = true;
-    for (int j = 0; j < jobs; ++j) vec = vec && a.job[j].q.vec && a.job[j].k.vec && a.job[j].v.vec;
+    const int piece = 16 / (int)sizeof(T);
+    bool whole = true;                   // rows of whole 16-byte pieces
+    for (int j = 0; j < jobs; ++j) whole = whole && a.job[j].Dk % piece == 0 && a.job[j].Dv % piece == 0;
     if (state_only) {
-        if (vec) hipLaunchKernelGGL((linattn_chunk_kernel<T, DKP, DVP, true, true>), grid, block, 0, st, a);
+        if (whole) hipLaunchKernelGGL((linattn_chunk_kernel<T, DKP, DVP, true, true>), grid, block, 0, st, a);
         else hipLaunchKernelGGL((linattn_chunk_kernel<T, DKP, DVP, true, false>), grid, block, 0, st, a);
     } else {
-        if (vec) hipLaunchKernelGGL((linattn_chunk_kernel<T, DKP, DVP, false, true>), grid, block, 0, st, a);
+        if (whole) hipLaunchKernelGGL((linattn_chunk_kernel<T, DKP, DVP, false, true>), grid, block, 0, st, a);
         else hipLaunchKernelGGL((linattn_chunk_kernel<T, DKP, DVP, false, false>), grid, block, 0, st, a);
     }
 }
@@ -598,15 +607,10 @@ int tile_of(int d) { return d <= 32 ? 32 : (d <= 64 ? 64 : 128); }
 
 constexpr long STRIDE_LIMIT = 1L << 22;      // of a token, in elements: a workgroup's rows lie within 32 bits of each other
 
-// rows of D elements are whole pieces of `bytes`, also from one row to the next
-bool pieces_ok(const void* p, const long* s, int D, int elem, int bytes) {
-    return (uintptr_t)p % bytes == 0 && (long)D * elem % bytes == 0 && s[0] * elem % bytes == 0 && s[1] * elem % bytes == 0 && s[2] * elem % bytes == 0;
-}
-Operand operand(const void* p, const long* s, int r, int D, int elem) { return {p, s[0], s[1], s[2], r, pieces_ok(p, s, D, elem, 16)}; }
+Operand operand(const void* p, const long* s, int r) { return {p, s[0], s[1], s[2], r}; }
 
 void set_out(Job& j, void* o, const long* s, int o16) {
     j.o = o; j.ob = s[0]; j.ot = s[1]; j.oh = s[2]; j.o16 = o16;
-    j.ovec = pieces_ok(o, s, j.Dv, o16 ? 2 : 4, o16 ? 8 : 16);
 }
 // one segment's worth of states lies as the forward pass has it, [Dk][Dv]; `turned` where the job's state is that transposed
 void set_state(Job& j, const float* s_in, float* s_out, float* seg, bool turned) {
@@ -647,9 +651,8 @@ int ha2g_linattn_fwd(const void* q, const void* k, const void* v, void* o, const
     for (int i = 1; i < 12; i += 3)
         HA2G_REQUIRE(strides[i] >= 0 && strides[i] < STRIDE_LIMIT, "linattn_fwd: a token stride of %ld elements (0 to %ld)", strides[i], STRIDE_LIMIT - 1);
     HA2G_REQUIRE(a.nseg == 1 || ws, "linattn_fwd: no workspace (ha2g_linattn_workspace_floats)");
-    const int e = b16_io ? 2 : 4;
     Job& j = a.job[0];
-    j.q = operand(q, strides, rq, Dk, e); j.k = operand(k, strides + 3, rk, Dk, e); j.v = operand(v, strides + 6, rv, Dv, e);
+    j.q = operand(q, strides, rq); j.k = operand(k, strides + 3, rk); j.v = operand(v, strides + 6, rv);
     j.Dk = Dk; j.Dv = Dv; j.rev = 0; j.oscale = scale; j.uscale = 1.f;
     set_out(j, o, strides + 9, b16_io);
     set_state(j, s_in, s_out, ws, false);
@@ -671,9 +674,8 @@ int ha2g_linattn_bwd(const void* q, const void* k, const void* v, const void* do
     for (int i = 1; i < 21; i += 3)
         HA2G_REQUIRE(strides[i] >= 0 && strides[i] < STRIDE_LIMIT, "linattn_bwd: a token stride of %ld elements (0 to %ld)", strides[i], STRIDE_LIMIT - 1);
     HA2G_REQUIRE(a.nseg == 1 || (ws && (ws_fwd || !dq)), "linattn_bwd: no workspace (ha2g_linattn_workspace_floats)");
-    const int e = b16_io ? 2 : 4;
-    const Operand oq_ = operand(q, strides, rq, Dk, e), ok_ = operand(k, strides + 3, rk, Dk, e), ov_ = operand(v, strides + 6, rv, Dv, e),
-                  od_ = operand(dout, strides + 9, 1, Dv, e);
+    const Operand oq_ = operand(q, strides, rq), ok_ = operand(k, strides + 3, rk), ov_ = operand(v, strides + 6, rv),
+                  od_ = operand(dout, strides + 9, 1);
     Job jv, jk, jq;
     jv.q = ok_; jv.k = oq_; jv.v = od_; jv.Dk = Dk; jv.Dv = Dv; jv.rev = 1; jv.oscale = 1.f; jv.uscale = scale;
     set_out(jv, dv, strides + 18, dv_b16);
@@ -707,9 +709,8 @@ int ha2g_linattn_step(const void* q, const void* k, const void* v, void* o, cons
     LinAttnArgs a;
     if (const int rc = check_args(a, "linattn_step", log_decay, nullptr, B, 1, H, rq, rk, rv, Dk, Dv, b16_io, q && k && v && o && state)) return rc;
     if (B == 0) return 0;
-    const int e = b16_io ? 2 : 4;
     Job& j = a.job[0];
-    j.q = operand(q, strides, rq, Dk, e); j.k = operand(k, strides + 3, rk, Dk, e); j.v = operand(v, strides + 6, rv, Dv, e);
+    j.q = operand(q, strides, rq); j.k = operand(k, strides + 3, rk); j.v = operand(v, strides + 6, rv);
     j.Dk = Dk; j.Dv = Dv; j.oscale = scale;
     set_out(j, o, strides + 9, b16_io);
     j.s_out = state;

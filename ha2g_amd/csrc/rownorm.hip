@@ -5,6 +5,8 @@
 // gradients are rounded once where they are stored, and z is the norm of h BEFORE that rounding, in the backward pass as in the forward one
 // (h is formed again from y, res and gate there: the same bytes as reading h, and the parameters' gradients stay fp32-exact).
 // Bound by HBM: a row lives in the registers of TPR threads (NI chunks of VEC values each) between its one read and its one write.
+// Groups of a multiple of 16 bytes at aligned addresses are the straight case; otherwise (RAG: heads of 71, rows of 5 270) a chunk is four values at any
+// address -- memory takes unaligned 16 bytes -- that may belong to two groups, and the row's last one may be short.
 #include "common.h"
 
 namespace {
@@ -24,14 +26,32 @@ struct TailArgs {
     float alpha, eps;
 };
 
-// VEC values as they lie in memory, 16 bytes at most
+// VEC values as they lie in memory, 16 bytes at most; ALIGN: at any multiple of a value's size
+typedef unsigned u32x4u_t __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2u_t __attribute__((ext_vector_type(2)));
+typedef u32x4u_t u32x4_a2 __attribute__((aligned(2)));
+typedef u32x2u_t u32x2_a2 __attribute__((aligned(2)));
 template <typename T, int VEC> struct Raw { unsigned u[(VEC * sizeof(T) + 3) / 4]; };
 template <typename T, int VEC> __device__ __forceinline__ Raw<T, VEC> load_raw(const T* p, long at) {
     Raw<T, VEC> r;
-    if constexpr (VEC * sizeof(T) == 16) { const uint4 v = *reinterpret_cast<const uint4*>(p + at); r.u[0] = v.x; r.u[1] = v.y; r.u[2] = v.z; r.u[3] = v.w; }
-    else if constexpr (VEC * sizeof(T) == 8) { const uint2 v = *reinterpret_cast<const uint2*>(p + at); r.u[0] = v.x; r.u[1] = v.y; }
+    if constexpr (VEC * sizeof(T) == 16) { const u32x4_a2 v = *reinterpret_cast<const u32x4_a2*>(p + at); r.u[0] = v[0]; r.u[1] = v[1]; r.u[2] = v[2]; r.u[3] = v[3]; }
+    else if constexpr (VEC * sizeof(T) == 8) { const u32x2_a2 v = *reinterpret_cast<const u32x2_a2*>(p + at); r.u[0] = v[0]; r.u[1] = v[1]; }
     else if constexpr (sizeof(T) == 4) r.u[0] = __float_as_uint(p[at]);
     else r.u[0] = p[at];
+    return r;
+}
+// of which the first n exist (1 <= n <= VEC), zeros behind
+template <typename T, int VEC> __device__ __forceinline__ Raw<T, VEC> load_raw(const T* p, long at, int n) {
+    if (VEC == 1 || n == VEC) return load_raw<T, VEC>(p, at);
+    Raw<T, VEC> r;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+        if constexpr (sizeof(T) == 4) r.u[j] = j < n ? __float_as_uint(p[at + j]) : 0u;
+        else {
+            if (j % 2 == 0) r.u[j / 2] = 0u;
+            if (j < n) r.u[j / 2] |= (unsigned)p[at + j] << (16 * (j & 1));
+        }
+    }
     return r;
 }
 template <int VEC> __device__ __forceinline__ void unpack(const Raw<float, VEC>& r, float* x) {
@@ -42,30 +62,61 @@ template <int VEC> __device__ __forceinline__ void unpack(const Raw<b16, VEC>& r
 #pragma unroll
     for (int j = 0; j < VEC; ++j) x[j] = __uint_as_float((j & 1) ? r.u[j >> 1] & 0xffff0000u : r.u[j >> 1] << 16);
 }
-template <int VEC> __device__ __forceinline__ void store_row(float* p, long at, const float* x) {
-    if constexpr (VEC >= 4) {
+template <int VEC> __device__ __forceinline__ void store_row(float* p, long at, const float* x, int n = VEC) {
+    if constexpr (VEC == 1) p[at] = x[0];
+    else if (n == VEC) {
 #pragma unroll
-        for (int j = 0; j < VEC; j += 4) *reinterpret_cast<float4*>(p + at + j) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
-    } else p[at] = x[0];
+        for (int j = 0; j < VEC; j += 4) {
+            const u32x4u_t v = {__float_as_uint(x[j]), __float_as_uint(x[j + 1]), __float_as_uint(x[j + 2]), __float_as_uint(x[j + 3])};
+            *reinterpret_cast<u32x4_a2*>(p + at + j) = v;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+            if (j < n) p[at + j] = x[j];
+    }
 }
-template <int VEC> __device__ __forceinline__ void store_row(b16* p, long at, const float* x) {
+template <int VEC> __device__ __forceinline__ void store_row(b16* p, long at, const float* x, int n = VEC) {
     unsigned h[(VEC + 1) / 2], l;
 #pragma unroll
     for (int j = 0; j < VEC; j += 2) split2_bf16(x[j], VEC > 1 ? x[j + (VEC > 1)] : 0.f, h[j >> 1], l);
-    if constexpr (VEC == 8) *reinterpret_cast<uint4*>(p + at) = make_uint4(h[0], h[1], h[2], h[3]);
-    else if constexpr (VEC == 4) *reinterpret_cast<uint2*>(p + at) = make_uint2(h[0], h[1]);
-    else p[at] = (b16)(h[0] & 0xffff);
-}
-template <int VEC> __device__ __forceinline__ void load_vec(const float* p, long at, float* x) {
-    if constexpr (VEC >= 4) {
+    if constexpr (VEC == 1) p[at] = (b16)(h[0] & 0xffff);
+    else if (n == VEC) {
+        if constexpr (VEC == 8) { const u32x4u_t v = {h[0], h[1], h[2], h[3]}; *reinterpret_cast<u32x4_a2*>(p + at) = v; }
+        else { const u32x2u_t v = {h[0], h[1]}; *reinterpret_cast<u32x2_a2*>(p + at) = v; }
+    } else {
 #pragma unroll
-        for (int j = 0; j < VEC; j += 4) { const float4 v = *reinterpret_cast<const float4*>(p + at + j); x[j] = v.x; x[j + 1] = v.y; x[j + 2] = v.z; x[j + 3] = v.w; }
-    } else x[0] = p[at];
+        for (int j = 0; j < VEC; ++j)
+            if (j < n) p[at + j] = (b16)(h[j >> 1] >> (16 * (j & 1)));
+    }
+}
+template <int VEC> __device__ __forceinline__ void load_vec(const float* p, long at, float* x, int n) {
+    if constexpr (VEC == 8) { unpack<4>(load_raw<float, 4>(p, at), x); unpack<4>(load_raw<float, 4>(p, at + 4), x + 4); }
+    else unpack<VEC>(load_raw<float, VEC>(p, at, n), x);
 }
 template <int VEC> __device__ __forceinline__ void fill(float* x, float v) {
 #pragma unroll
     for (int j = 0; j < VEC; ++j) x[j] = v;
 }
+
+// Where a thread's chunks lie: values of chunk i that exist (n), its group, and how many of its values belong to that group (k; the rest to the next)
+template <int TPR, int NI, int VEC, bool RAG> struct Place {
+    int g[NI], k_[NI], n_[NI];
+    __device__ __forceinline__ void init(const TailArgs& a, int lane) {
+        const int D = a.C / a.G;
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            const int at = (lane + i * TPR) * VEC;
+            g[i] = at / D;
+            if constexpr (RAG) {
+                n_[i] = max(0, min(VEC, a.C - at));
+                k_[i] = min(VEC, (g[i] + 1) * D - at);
+            }
+        }
+    }
+    __device__ __forceinline__ int n(int i) const { if constexpr (RAG) return n_[i]; else return VEC; }
+    __device__ __forceinline__ int k(int i) const { if constexpr (RAG) return k_[i]; else return VEC; }
+};
 
 // the gate's activation and its derivative
 __device__ __forceinline__ void gate_act(float g, int act, float& a, float& d) {
@@ -75,13 +126,14 @@ __device__ __forceinline__ void gate_act(float g, int act, float& a, float& d) {
     d = act == 3 ? s * (1.f - s) : s * (1.f + g * (1.f - s));
 }
 
-// Sums over the row's TPR threads of one value per chunk: r[i] = the sum over the group chunk i belongs to.  The whole row: a butterfly, and beyond a
-// wave one meeting in LDS (two places in turn).  Groups of 2^n <= 64 chunks: a butterfly over their lanes.  Others (heads of 60): every chunk's
-// value goes to LDS, 16 lanes add up a group, its sum is read back from the group's first place.  A row of one wave needs no barrier.
+// Sums over the row's TPR threads of a value per chunk (RAG: of its two parts): r = the sum over the group the chunk (its part) belongs to.  The whole
+// row: a butterfly, and beyond a wave one meeting in LDS (two places in turn).  Groups of 2^n <= 64 chunks: a butterfly over their lanes.  Others
+// (heads of 60): every chunk's value goes to LDS, a team of lanes adds up a group, its sum is read back.  A row of one wave needs no barrier.
 // Every thread of the block calls it the same number of times.
-template <int TPR, int NI> struct RowSum {
-    float *lds, *meet;           // this row's TPR * NI floats; two times TPR / 64
-    int lane, G, cpg, nch, phase;      // thread of the row, groups, chunks per group, chunks
+template <int TPR, int NI, int VEC, bool RAG> struct RowSum {
+    static constexpr int PARTS = RAG ? 2 : 1, PLACES = TPR * NI * PARTS + (RAG ? TPR * NI * VEC / 3 + 1 : 0);      // groups of 3 or more values
+    float *lds, *meet;           // this row's PLACES floats; two times TPR / 64
+    int lane, G, D, nch, phase;  // thread of the row, groups, values per group, chunks
     __device__ __forceinline__ static void sync() {
         if constexpr (TPR > 64) __syncthreads();
         else { __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront"); __builtin_amdgcn_wave_barrier(); __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront"); }
@@ -99,81 +151,106 @@ template <int TPR, int NI> struct RowSum {
         }
         return s;
     }
-    __device__ __forceinline__ void groups(const float (&p)[NI], float (&r)[NI]) {
+    __device__ __forceinline__ void groups(const Place<TPR, NI, VEC, RAG>& pl, const float (&p)[NI][PARTS], float (&r)[NI][PARTS]) {
         if (G == 1) {
             float s = 0.f;
 #pragma unroll
-            for (int i = 0; i < NI; ++i) s += p[i];
+            for (int i = 0; i < NI; ++i) s += p[i][0];
             s = all(s);
 #pragma unroll
-            for (int i = 0; i < NI; ++i) r[i] = s;
+            for (int i = 0; i < NI; ++i) r[i][0] = r[i][PARTS - 1] = s;
             return;
         }
-        if (cpg <= 64 && (cpg & (cpg - 1)) == 0) {
+        const int cpg = D / VEC;
+        if constexpr (!RAG)
+            if (cpg <= 64 && (cpg & (cpg - 1)) == 0) {
 #pragma unroll
-            for (int i = 0; i < NI; ++i) r[i] = p[i];
-            for (int o = cpg >> 1; o > 0; o >>= 1)
+                for (int i = 0; i < NI; ++i) r[i][0] = p[i][0];
+                for (int o = cpg >> 1; o > 0; o >>= 1)
 #pragma unroll
-                for (int i = 0; i < NI; ++i) r[i] += __shfl_xor(r[i], o, 64);
-            return;
-        }
+                    for (int i = 0; i < NI; ++i) r[i][0] += __shfl_xor(r[i][0], o, 64);
+                return;
+            }
         sync();
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
             const int c = lane + i * TPR;
-            if (c < nch) lds[c] = p[i];
+            if (c < nch)
+#pragma unroll
+                for (int q = 0; q < PARTS; ++q) lds[c * PARTS + q] = p[i][q];
         }
         sync();
-        for (int g = lane >> 4; g < G; g += TPR / 16) {
+        const int team = G * 32 <= TPR ? 64 : 16;
+        float* const sums = RAG ? lds + TPR * NI * PARTS : lds;
+        for (int g = lane / team; g < G; g += TPR / team) {
+            const int c0 = g * D / VEC, c1 = ((g + 1) * D + VEC - 1) / VEC;
             float s = 0.f;
-            for (int c = lane & 15; c < cpg; c += 16) s += lds[g * cpg + c];
-#pragma unroll
-            for (int o = 8; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-            if ((lane & 15) == 0) lds[g * cpg] = s;
+            for (int c = c0 + lane % team; c < c1; c += team) s += lds[c * PARTS + (RAG && c * VEC < g * D ? 1 : 0)];
+            for (int o = team >> 1; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+            if (lane % team == 0) sums[RAG ? g : c0] = s;
         }
         sync();
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
             const int c = lane + i * TPR;
-            r[i] = c < nch ? lds[c / cpg * cpg] : 0.f;
+            if constexpr (RAG) {
+                r[i][0] = c < nch ? sums[pl.g[i]] : 0.f;
+                r[i][1] = c < nch && pl.k(i) < pl.n(i) ? sums[pl.g[i] + 1] : 0.f;
+            } else r[i][0] = c < nch ? sums[pl.g[i] * cpg] : 0.f;
         }
     }
 };
+// a chunk's value j: which of its parts
+template <bool RAG> __device__ __forceinline__ int part_of(int j, int k) { return RAG && j >= k ? 1 : 0; }
+template <bool RAG, int PARTS> __device__ __forceinline__ float pick(const float (&r)[PARTS], int j, int k) {
+    if constexpr (RAG) return j >= k ? r[1] : r[0];
+    else return r[0];
+}
+template <bool RAG, int PARTS> __device__ __forceinline__ void add_to(float (&p)[PARTS], int j, int k, bool whole, float v) {
+    if constexpr (RAG) { if (whole || j < k) p[0] += v; else p[1] += v; }
+    else p[0] += v;
+}
 
-// x -> x^ in place; m / r: mean and 1 / std per chunk
-template <int TPR, int NI, int VEC>
-__device__ __forceinline__ void normalise(RowSum<TPR, NI>& rsum, float (&x)[NI][VEC], float (&m)[NI], float (&r)[NI], bool layer, float inv, float eps) {
-    float p[NI];
+// x -> x^ in place; m / r: mean and 1 / std per chunk and part.  Values that do not exist are zeros and stay zeros.
+template <int TPR, int NI, int VEC, bool RAG>
+__device__ __forceinline__ void normalise(RowSum<TPR, NI, VEC, RAG>& rsum, const Place<TPR, NI, VEC, RAG>& pl, float (&x)[NI][VEC],
+                                          float (&m)[NI][RowSum<TPR, NI, VEC, RAG>::PARTS], float (&r)[NI][RowSum<TPR, NI, VEC, RAG>::PARTS], bool layer,
+                                          float inv, float eps) {
+    constexpr int PARTS = RowSum<TPR, NI, VEC, RAG>::PARTS;
+    const bool whole = rsum.G == 1;
+    float p[NI][PARTS];
 #pragma unroll
-    for (int i = 0; i < NI; ++i) m[i] = 0.f;
+    for (int i = 0; i < NI; ++i) fill<PARTS>(m[i], 0.f);
     if (layer) {
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
-            p[i] = 0.f;
+            fill<PARTS>(p[i], 0.f);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) p[i] += x[i][j];
+            for (int j = 0; j < VEC; ++j) add_to<RAG>(p[i], j, pl.k(i), whole, x[i][j]);
         }
-        rsum.groups(p, m);
+        rsum.groups(pl, p, m);
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
-            m[i] *= inv;
+#pragma unroll
+            for (int q = 0; q < PARTS; ++q) m[i][q] *= inv;
             const bool in = rsum.lane + i * TPR < rsum.nch;
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) x[i][j] = in ? x[i][j] - m[i] : 0.f;
+            for (int j = 0; j < VEC; ++j) x[i][j] = in && j < pl.n(i) ? x[i][j] - pick<RAG>(m[i], j, pl.k(i)) : 0.f;
         }
     }
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-        p[i] = 0.f;
+        fill<PARTS>(p[i], 0.f);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) p[i] += x[i][j] * x[i][j];
+        for (int j = 0; j < VEC; ++j) add_to<RAG>(p[i], j, pl.k(i), whole, x[i][j] * x[i][j]);
     }
-    rsum.groups(p, r);
+    rsum.groups(pl, p, r);
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-        r[i] = 1.0f / sqrtf(r[i] * inv + eps);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) x[i][j] *= r[i];
+        for (int q = 0; q < PARTS; ++q) r[i][q] = 1.0f / sqrtf(r[i][q] * inv + eps);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) x[i][j] *= pick<RAG>(r[i], j, pl.k(i));
     }
 }
 
@@ -183,39 +260,43 @@ template <int TPR> constexpr int block_of() { return TPR > 256 ? TPR : 256; }
 template <int NI, int VEC> struct Columns {
     static constexpr bool KEEP = NI == 1;
     float w[VEC], b[VEC], s[VEC], w2[VEC], b2[VEC];
-    __device__ __forceinline__ void load(const TailArgs& a, long at, bool in) {
+    __device__ __forceinline__ void load(const TailArgs& a, long at, bool in, int n) {
         fill<VEC>(w, 1.f); fill<VEC>(b, 0.f); fill<VEC>(s, 1.f); fill<VEC>(w2, 0.f); fill<VEC>(b2, 0.f);
         if (!in) return;
-        if (a.w) load_vec<VEC>(a.w, at, w);
-        if (a.b) load_vec<VEC>(a.b, at, b);
-        if (a.s) load_vec<VEC>(a.s, at, s);
-        if (a.w2) load_vec<VEC>(a.w2, at, w2);
-        if (a.b2) load_vec<VEC>(a.b2, at, b2);
+        if (a.w) load_vec<VEC>(a.w, at, w, n);
+        if (a.b) load_vec<VEC>(a.b, at, b, n);
+        if (a.s) load_vec<VEC>(a.s, at, s, n);
+        if (a.w2) load_vec<VEC>(a.w2, at, w2, n);
+        if (a.b2) load_vec<VEC>(a.b2, at, b2, n);
     }
 };
 
-template <typename T, int TPR, int NI, int VEC>
+template <typename T, int TPR, int NI, int VEC, bool RAG>
 __global__ __launch_bounds__(block_of<TPR>()) void tail_fwd_kernel(const TailArgs a) {
+    typedef RowSum<TPR, NI, VEC, RAG> Sum;
     constexpr int RPB = block_of<TPR>() / TPR;
-    __shared__ float lds[RPB * TPR * NI], meet[2][2 * (TPR / 64)];
-    const int sub = threadIdx.x / TPR, lane = threadIdx.x % TPR, nch = a.C / VEC;
+    __shared__ float lds[RPB * Sum::PLACES], meet[2][2 * (TPR / 64)];
+    const int sub = threadIdx.x / TPR, lane = threadIdx.x % TPR, nch = (a.C + VEC - 1) / VEC;
     const long rows = a.inner * a.outer;
-    RowSum<TPR, NI> gsum{lds + sub * TPR * NI, meet[0], lane, a.G, nch / a.G, nch, 0}, rsum{lds + sub * TPR * NI, meet[1], lane, 1, nch, nch, 0};
+    float* const mine = lds + sub * Sum::PLACES;
+    Sum gsum{mine, meet[0], lane, a.G, a.C / a.G, nch, 0}, rsum{mine, meet[1], lane, 1, a.C, nch, 0};
+    Place<TPR, NI, VEC, RAG> pl;
+    pl.init(a, lane);
     Columns<NI, VEC> col;
-    if constexpr (Columns<NI, VEC>::KEEP) col.load(a, (long)lane * VEC, lane < nch);
+    if constexpr (Columns<NI, VEC>::KEEP) col.load(a, (long)lane * VEC, lane < nch, pl.n(0));
     for (long r0 = (long)blockIdx.x * RPB; r0 < rows; r0 += (long)gridDim.x * RPB) {
         const long row = r0 + sub;
         const bool in = row < rows;
         const long at = row * a.C, gat = a.gate_shared ? row / a.inner * a.C : at;
         Raw<T, VEC> ry[NI], rg[NI], rr[NI];
-        float x[NI][VEC], m[NI], r[NI];
+        float x[NI][VEC], m[NI][Sum::PARTS], r[NI][Sum::PARTS];
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
             const int c = lane + i * TPR;
             if (in && c < nch) {
-                ry[i] = load_raw<T, VEC>((const T*)a.y, at + (long)c * VEC);
-                if (a.gate) rg[i] = load_raw<T, VEC>((const T*)a.gate, gat + (long)c * VEC);
-                if (a.res) rr[i] = load_raw<T, VEC>((const T*)a.res, at + (long)c * VEC);
+                ry[i] = load_raw<T, VEC>((const T*)a.y, at + (long)c * VEC, pl.n(i));
+                if (a.gate) rg[i] = load_raw<T, VEC>((const T*)a.gate, gat + (long)c * VEC, pl.n(i));
+                if (a.res) rr[i] = load_raw<T, VEC>((const T*)a.res, at + (long)c * VEC, pl.n(i));
             }
         }
 #pragma unroll
@@ -225,14 +306,19 @@ __global__ __launch_bounds__(block_of<TPR>()) void tail_fwd_kernel(const TailArg
             if (in && c < nch) unpack<VEC>(ry[i], x[i]);
         }
         if (a.w) {
-            normalise<TPR, NI, VEC>(gsum, x, m, r, a.layer, (float)a.G / a.C, a.eps);
+            normalise(gsum, pl, x, m, r, a.layer, (float)a.G / a.C, a.eps);
             if (a.rs && in) {
 #pragma unroll
                 for (int i = 0; i < NI; ++i) {
-                    const int c = lane + i * TPR, g = c / gsum.cpg;
-                    if (c < nch && c == g * gsum.cpg) {
-                        a.rs[row * a.G + g] = r[i];
-                        if (a.layer) a.mu[row * a.G + g] = m[i];
+                    const int c = lane + i * TPR;
+                    const long at = row * a.G + pl.g[i];              // a group's statistics are kept by the chunk it begins in
+                    if (c < nch && c * VEC == pl.g[i] * gsum.D) {
+                        a.rs[at] = r[i][0];
+                        if (a.layer) a.mu[at] = m[i][0];
+                    }
+                    if (RAG && c < nch && pl.k(i) < pl.n(i)) {
+                        a.rs[at + 1] = r[i][Sum::PARTS - 1];
+                        if (a.layer) a.mu[at + 1] = m[i][Sum::PARTS - 1];
                     }
                 }
             }
@@ -241,7 +327,7 @@ __global__ __launch_bounds__(block_of<TPR>()) void tail_fwd_kernel(const TailArg
         for (int i = 0; i < NI; ++i) {
             const int c = lane + i * TPR;
             if (!(in && c < nch)) continue;
-            if constexpr (!Columns<NI, VEC>::KEEP) col.load(a, (long)c * VEC, true);
+            if constexpr (!Columns<NI, VEC>::KEEP) col.load(a, (long)c * VEC, true, pl.n(i));
             float t[VEC];
             if (a.w) {
 #pragma unroll
@@ -261,49 +347,60 @@ __global__ __launch_bounds__(block_of<TPR>()) void tail_fwd_kernel(const TailArg
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) x[i][j] = a.alpha * t[j] + x[i][j];
             }
-            store_row<VEC>((T*)a.h, at + (long)c * VEC, x[i]);
+            if constexpr (RAG)
+#pragma unroll
+                for (int j = 0; j < VEC; ++j)
+                    if (j >= pl.n(i)) x[i][j] = 0.f;
+            store_row<VEC>((T*)a.h, at + (long)c * VEC, x[i], pl.n(i));
         }
         if (a.w2) {
-            normalise<TPR, NI, VEC>(rsum, x, m, r, a.layer, 1.0f / a.C, a.eps);
+            normalise(rsum, pl, x, m, r, a.layer, 1.0f / a.C, a.eps);
             if (a.rs2 && in && lane == 0) {
-                a.rs2[row] = r[0];
-                if (a.layer) a.mu2[row] = m[0];
+                a.rs2[row] = r[0][0];
+                if (a.layer) a.mu2[row] = m[0][0];
             }
 #pragma unroll
             for (int i = 0; i < NI; ++i) {
                 const int c = lane + i * TPR;
                 if (!(in && c < nch)) continue;
-                if constexpr (!Columns<NI, VEC>::KEEP) col.load(a, (long)c * VEC, true);
+                if constexpr (!Columns<NI, VEC>::KEEP) col.load(a, (long)c * VEC, true, pl.n(i));
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) x[i][j] = x[i][j] * col.w2[j] + col.b2[j];
-                store_row<VEC>((T*)a.z, at + (long)c * VEC, x[i]);
+                store_row<VEC>((T*)a.z, at + (long)c * VEC, x[i], pl.n(i));
             }
         }
     }
 }
 
 // One row's operands on their way: loaded a row ahead, so that a row's sums and barriers lie under the next row's loads
-template <typename T, int NI, int VEC, bool FULL> struct RowIn {
+template <typename T, int TPR, int NI, int VEC, bool RAG, bool FULL> struct RowIn {
+    static constexpr int PARTS = RAG ? 2 : 1;
     Raw<T, VEC> y[NI], dh[NI], dz[FULL ? NI : 1], gate[FULL ? NI : 1], res[FULL ? NI : 1];
-    float mu[NI], rs[NI], mu2, rs2;
-    __device__ __forceinline__ void load(const TailArgs& a, long row, long gat, bool in, int lane, int tpr, int nch, const int* grp) {
+    float mu[NI][PARTS], rs[NI][PARTS], mu2, rs2;
+    __device__ __forceinline__ void load(const TailArgs& a, long row, long gat, bool in, int lane, int nch, const Place<TPR, NI, VEC, RAG>& pl) {
         mu2 = rs2 = 0.f;
         const long at = row * a.C;
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
-            const int c = lane + i * tpr;
-            mu[i] = rs[i] = 0.f;
+            const int c = lane + i * TPR;
+            fill<PARTS>(mu[i], 0.f);
+            fill<PARTS>(rs[i], 0.f);
             if (!(in && c < nch)) continue;
-            y[i] = load_raw<T, VEC>((const T*)a.y, at + (long)c * VEC);
-            if (a.dh) dh[i] = load_raw<T, VEC>((const T*)a.dh, at + (long)c * VEC);
+            y[i] = load_raw<T, VEC>((const T*)a.y, at + (long)c * VEC, pl.n(i));
+            if (a.dh) dh[i] = load_raw<T, VEC>((const T*)a.dh, at + (long)c * VEC, pl.n(i));
             if (a.w) {
-                rs[i] = a.rs[row * a.G + grp[i]];
-                if (a.layer) mu[i] = a.mu[row * a.G + grp[i]];
+                const long g = row * a.G + pl.g[i];
+#pragma unroll
+                for (int q = 0; q < PARTS; ++q)
+                    if (q == 0 || pl.k(i) < pl.n(i)) {
+                        rs[i][q] = a.rs[g + q];
+                        if (a.layer) mu[i][q] = a.mu[g + q];
+                    }
             }
             if constexpr (FULL) {
-                if (a.dz) dz[i] = load_raw<T, VEC>((const T*)a.dz, at + (long)c * VEC);
-                if (a.gate) gate[i] = load_raw<T, VEC>((const T*)a.gate, gat + (long)c * VEC);
-                if (a.res && a.w2) res[i] = load_raw<T, VEC>((const T*)a.res, at + (long)c * VEC);
+                if (a.dz) dz[i] = load_raw<T, VEC>((const T*)a.dz, at + (long)c * VEC, pl.n(i));
+                if (a.gate) gate[i] = load_raw<T, VEC>((const T*)a.gate, gat + (long)c * VEC, pl.n(i));
+                if (a.res && a.w2) res[i] = load_raw<T, VEC>((const T*)a.res, at + (long)c * VEC, pl.n(i));
             }
         }
         if constexpr (FULL) {
@@ -317,32 +414,35 @@ template <typename T, int NI, int VEC, bool FULL> struct RowIn {
 
 // A block walks through the rows of its slice of a sequence and keeps the columns' sums in registers; its partial sums leave it once.
 // FULL: with gate, scale, residual or second norm; otherwise the norm alone (w, b).
-template <typename T, int TPR, int NI, int VEC, bool FULL>
+template <typename T, int TPR, int NI, int VEC, bool RAG, bool FULL>
 __global__ __launch_bounds__(block_of<TPR>()) void tail_bwd_kernel(const TailArgs a) {
     constexpr int RPB = block_of<TPR>() / TPR, NV = FULL ? 6 : 2;      // w, b, s, w2, b2, gate
-    __shared__ float lds[RPB * TPR * NI * (RPB > 1 ? VEC : 1)], meet[2][2 * (TPR / 64)];
-    const int sub = threadIdx.x / TPR, lane = threadIdx.x % TPR, nch = a.C / VEC;
-    float* const mine = lds + sub * TPR * NI;
-    RowSum<TPR, NI> gsum{mine, meet[0], lane, a.G, nch / a.G, nch, 0}, rsum{mine, meet[1], lane, 1, nch, nch, 0};
+    typedef RowSum<TPR, NI, VEC, RAG> Sum;
+    constexpr int COLS = RPB > 1 ? RPB * TPR * NI * VEC : 1;
+    __shared__ __attribute__((aligned(16))) float lds[RPB * Sum::PLACES > COLS ? RPB * Sum::PLACES : COLS];
+    __shared__ float meet[2][2 * (TPR / 64)];
+    const int sub = threadIdx.x / TPR, lane = threadIdx.x % TPR, nch = (a.C + VEC - 1) / VEC;
+    float* const mine = lds + sub * Sum::PLACES;
+    Sum gsum{mine, meet[0], lane, a.G, a.C / a.G, nch, 0}, rsum{mine, meet[1], lane, 1, a.C, nch, 0};
+    Place<TPR, NI, VEC, RAG> pl;
+    pl.init(a, lane);
+    const bool whole = a.G == 1;
     const long per = (a.inner + gridDim.x - 1) / gridDim.x, beg = blockIdx.x * per, end = min(a.inner, beg + per);
     const float inv = (float)a.G / a.C, inv2 = 1.0f / a.C;
     const long row0 = (long)blockIdx.y * a.inner, gat0 = (long)blockIdx.y * a.C;
-    int grp[NI];
-#pragma unroll
-    for (int i = 0; i < NI; ++i) grp[i] = (lane + i * TPR) / gsum.cpg;
     float acc[NV][NI][VEC];
 #pragma unroll
     for (int n = 0; n < NV; ++n)
 #pragma unroll
         for (int i = 0; i < NI; ++i) fill<VEC>(acc[n][i], 0.f);
     Columns<NI, VEC> col;
-    if constexpr (Columns<NI, VEC>::KEEP) col.load(a, (long)lane * VEC, lane < nch);
-    RowIn<T, NI, VEC, FULL> cur, nxt;
-    cur.load(a, row0 + beg + sub, a.gate_shared ? gat0 : (row0 + beg + sub) * a.C, beg + sub < end, lane, TPR, nch, grp);
+    if constexpr (Columns<NI, VEC>::KEEP) col.load(a, (long)lane * VEC, lane < nch, pl.n(0));
+    RowIn<T, TPR, NI, VEC, RAG, FULL> cur, nxt;
+    cur.load(a, row0 + beg + sub, a.gate_shared ? gat0 : (row0 + beg + sub) * a.C, beg + sub < end, lane, nch, pl);
     for (long q0 = beg; q0 < end; q0 += RPB) {
         const bool in = q0 + sub < end;
         const long row = row0 + q0 + sub, at = row * a.C;
-        nxt.load(a, row + RPB, a.gate_shared ? gat0 : (row + RPB) * a.C, q0 + RPB + sub < end, lane, TPR, nch, grp);
+        nxt.load(a, row + RPB, a.gate_shared ? gat0 : (row + RPB) * a.C, q0 + RPB + sub < end, lane, nch, pl);
         float xh[NI][VEC], n[NI][VEC], d[NI][VEC], ga[FULL ? NI : 1][VEC], gd[FULL ? NI : 1][VEC];
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
@@ -350,12 +450,12 @@ __global__ __launch_bounds__(block_of<TPR>()) void tail_bwd_kernel(const TailArg
             fill<VEC>(xh[i], 0.f); fill<VEC>(n[i], 0.f); fill<VEC>(d[i], 0.f);
             if constexpr (FULL) { fill<VEC>(ga[i], 1.f); fill<VEC>(gd[i], 0.f); }
             if (!(in && c < nch)) continue;
-            if constexpr (!Columns<NI, VEC>::KEEP) col.load(a, (long)c * VEC, true);
+            if constexpr (!Columns<NI, VEC>::KEEP) col.load(a, (long)c * VEC, true, pl.n(i));
             unpack<VEC>(cur.y[i], xh[i]);
             if (a.dh) unpack<VEC>(cur.dh[i], d[i]);
             if (a.w) {
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) xh[i][j] = (xh[i][j] - cur.mu[i]) * cur.rs[i];
+                for (int j = 0; j < VEC; ++j) xh[i][j] = (xh[i][j] - pick<RAG>(cur.mu[i], j, pl.k(i))) * pick<RAG>(cur.rs[i], j, pl.k(i));
             }
             if constexpr (FULL) {
 #pragma unroll
@@ -376,7 +476,7 @@ __global__ __launch_bounds__(block_of<TPR>()) void tail_bwd_kernel(const TailArg
                     const int c = lane + i * TPR;
                     fill<VEC>(hh[i], 0.f); fill<VEC>(e[i], 0.f);
                     if (!(in && c < nch)) continue;
-                    if constexpr (!Columns<NI, VEC>::KEEP) col.load(a, (long)c * VEC, true);
+                    if constexpr (!Columns<NI, VEC>::KEEP) col.load(a, (long)c * VEC, true, pl.n(i));
                     float t[VEC];
                     fill<VEC>(t, 0.f);
                     if (a.res) unpack<VEC>(cur.res[i], t);
@@ -386,7 +486,7 @@ __global__ __launch_bounds__(block_of<TPR>()) void tail_bwd_kernel(const TailArg
                         float h = n[i][j] * ga[i][j];
                         if (a.s) h *= col.s[j];
                         if (a.res) h = a.alpha * t[j] + h;
-                        hh[i][j] = (h - cur.mu2) * cur.rs2;
+                        hh[i][j] = j < pl.n(i) ? (h - cur.mu2) * cur.rs2 : 0.f;
                         acc[3][i][j] += e[i][j] * hh[i][j];
                         acc[4][i][j] += e[i][j];
                         e[i][j] *= col.w2[j];
@@ -403,19 +503,24 @@ __global__ __launch_bounds__(block_of<TPR>()) void tail_bwd_kernel(const TailArg
             }
         }
         // d = the whole gradient of h (of n, where there is nothing behind it) -> d(x^)
-        float p1[NI], p2[NI];
+        float p1[NI][Sum::PARTS], p2[NI][Sum::PARTS];
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
             const int c = lane + i * TPR;
-            p1[i] = p2[i] = 0.f;
+            fill<Sum::PARTS>(p1[i], 0.f);
+            fill<Sum::PARTS>(p2[i], 0.f);
+            if constexpr (RAG)
+#pragma unroll
+                for (int j = 0; j < VEC; ++j)
+                    if (j >= pl.n(i)) d[i][j] = 0.f;
             if (!(in && c < nch)) { fill<VEC>(d[i], 0.f); continue; }
-            if constexpr (!Columns<NI, VEC>::KEEP) col.load(a, (long)c * VEC, true);
+            if constexpr (!Columns<NI, VEC>::KEEP) col.load(a, (long)c * VEC, true, pl.n(i));
             if constexpr (FULL) {
                 float t[VEC];
                 if (a.dres) {
 #pragma unroll
                     for (int j = 0; j < VEC; ++j) t[j] = a.alpha * d[i][j];
-                    store_row<VEC>((T*)a.dres, at + (long)c * VEC, t);
+                    store_row<VEC>((T*)a.dres, at + (long)c * VEC, t, pl.n(i));
                 }
                 if (a.s) {
 #pragma unroll
@@ -428,7 +533,7 @@ __global__ __launch_bounds__(block_of<TPR>()) void tail_bwd_kernel(const TailArg
                         acc[5][i][j] += t[j];
                         d[i][j] *= ga[i][j];
                     }
-                    if (a.dgate && !a.gate_shared) store_row<VEC>((T*)a.dgate, at + (long)c * VEC, t);
+                    if (a.dgate && !a.gate_shared) store_row<VEC>((T*)a.dgate, at + (long)c * VEC, t, pl.n(i));
                 }
             }
             if (a.w) {
@@ -437,25 +542,26 @@ __global__ __launch_bounds__(block_of<TPR>()) void tail_bwd_kernel(const TailArg
                     acc[0][i][j] += d[i][j] * xh[i][j];
                     acc[1][i][j] += d[i][j];
                     d[i][j] *= col.w[j];
-                    p1[i] += d[i][j] * xh[i][j];
-                    p2[i] += d[i][j];
+                    add_to<RAG>(p1[i], j, pl.k(i), whole, d[i][j] * xh[i][j]);
+                    add_to<RAG>(p2[i], j, pl.k(i), whole, d[i][j]);
                 }
             }
         }
         if (a.w) {
-            float c1[NI], c2[NI];
-            gsum.groups(p1, c1);
-            if (a.layer) gsum.groups(p2, c2);
+            float c1[NI][Sum::PARTS], c2[NI][Sum::PARTS];
+            gsum.groups(pl, p1, c1);
+            if (a.layer) gsum.groups(pl, p2, c2);
 #pragma unroll
             for (int i = 0; i < NI; ++i)
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) d[i][j] = cur.rs[i] * (d[i][j] - xh[i][j] * (c1[i] * inv) - (a.layer ? c2[i] * inv : 0.f));
+                for (int j = 0; j < VEC; ++j)
+                    d[i][j] = pick<RAG>(cur.rs[i], j, pl.k(i)) * (d[i][j] - xh[i][j] * (pick<RAG>(c1[i], j, pl.k(i)) * inv) - (a.layer ? pick<RAG>(c2[i], j, pl.k(i)) * inv : 0.f));
         }
         if (a.dy) {
 #pragma unroll
             for (int i = 0; i < NI; ++i) {
                 const int c = lane + i * TPR;
-                if (in && c < nch) store_row<VEC>((T*)a.dy, at + (long)c * VEC, d[i]);
+                if (in && c < nch) store_row<VEC>((T*)a.dy, at + (long)c * VEC, d[i], pl.n(i));
             }
         }
         cur = nxt;
@@ -475,7 +581,9 @@ __global__ __launch_bounds__(block_of<TPR>()) void tail_bwd_kernel(const TailArg
 #pragma unroll
             for (int i = 0; i < NI; ++i) {
                 const int c = lane + i * TPR;
-                if (c < nch) store_row<VEC>(lds, (long)(sub * NI * TPR + c) * VEC, acc[q][i]);
+                if (c < nch)
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) lds[(sub * NI * TPR + c) * VEC + j] = acc[q][i][j];
             }
             __syncthreads();
             for (int c = threadIdx.x; c < a.C; c += RPB * TPR) {
@@ -488,7 +596,7 @@ __global__ __launch_bounds__(block_of<TPR>()) void tail_bwd_kernel(const TailArg
 #pragma unroll
             for (int i = 0; i < NI; ++i) {
                 const int c = lane + i * TPR;
-                if (c < nch) store_row<VEC>(out, (long)c * VEC, acc[q][i]);
+                if (c < nch) store_row<VEC>(out, (long)c * VEC, acc[q][i], pl.n(i));
             }
         }
     }
@@ -521,60 +629,61 @@ __global__ __launch_bounds__(1024) void slab_sum_kernel(const float* __restrict_
 }
 
 // Threads per row and chunks per thread: a wave alone up to 128 chunks, then one chunk per thread as far as 256 threads go, then two; the widest rows
-// take what the registers of 1 024 threads hold.
-#define TAIL_SHAPES(VEC, CASE)                                                                                                                     \
+// take what the registers of 1 024 threads hold.  Groups of one or two values (VEC = 1) are taken one by one.
+#define TAIL_SHAPES(VEC, RAG, CASE)                                                                                                                \
     {                                                                                                                                              \
-        const int nch = a.C / VEC;                                                                                                                 \
-        if (nch <= 64) CASE(64, 1, VEC)                                                                                                            \
-        else if (nch <= 128) CASE(64, 2, VEC)                                                                                                      \
-        else if (nch <= 256) CASE(256, 1, VEC)                                                                                                     \
-        else if (nch <= 512) CASE(256, 2, VEC)                                                                                                     \
-        else if (nch <= 1024) CASE(512, 2, VEC)                                                                                                    \
-        else if (nch <= 2048 || VEC == 8) CASE(1024, 2, VEC)                                                                                       \
-        else if (nch <= 4096 || VEC == 4) CASE(1024, 4, VEC == 8 ? 4 : VEC)                                                                        \
-        else CASE(1024, 8, 1)                                                                                                                      \
+        const int nch = (a.C + VEC - 1) / VEC;                                                                                                     \
+        if (nch <= 64) CASE(64, 1, VEC, RAG)                                                                                                       \
+        else if (nch <= 128) CASE(64, 2, VEC, RAG)                                                                                                 \
+        else if (nch <= 256) CASE(256, 1, VEC, RAG)                                                                                                \
+        else if (nch <= 512) CASE(256, 2, VEC, RAG)                                                                                                \
+        else if (nch <= 1024) CASE(512, 2, VEC, RAG)                                                                                               \
+        else if (nch <= 2048) CASE(1024, 2, VEC, RAG)                                                                                              \
+        else CASE(1024, (VEC == 8 ? 2 : 4), VEC, RAG)                                                                                              \
+    }
+#define TAIL_ONES(CASE)                                                                                                                            \
+    {                                                                                                                                              \
+        if (a.C <= 1024) CASE(256, 4, 1, false)                                                                                                    \
+        else CASE(1024, 16, 1, false)                                                                                                              \
     }
 #define TAIL_VECS(CASE)                                                                                                                            \
-    if constexpr (sizeof(T) == 2) {                                                                                                                \
-        if (vec == 8) TAIL_SHAPES(8, CASE)                                                                                                         \
-        else if (vec == 4) TAIL_SHAPES(4, CASE)                                                                                                    \
-        else TAIL_SHAPES(1, CASE)                                                                                                                  \
-    } else {                                                                                                                                       \
-        if (vec == 4) TAIL_SHAPES(4, CASE)                                                                                                         \
-        else TAIL_SHAPES(1, CASE)                                                                                                                  \
-    }
+    if (vec == 1) TAIL_ONES(CASE)                                                                                                                  \
+    else if (rag) TAIL_SHAPES(4, true, CASE)                                                                                                       \
+    else if constexpr (sizeof(T) == 2) {                                                                                                           \
+        if (vec == 8) TAIL_SHAPES(8, false, CASE)                                                                                                  \
+        else TAIL_SHAPES(4, false, CASE)                                                                                                           \
+    } else TAIL_SHAPES(4, false, CASE)
 
-template <typename T> void tail_fwd_launch(const TailArgs& a, int vec, hipStream_t st) {
+template <typename T> void tail_fwd_launch(const TailArgs& a, int vec, bool rag, hipStream_t st) {
     const long rows = a.inner * a.outer;
-#define FWD_CASE(TPR, NI, VEC)                                                                                             \
+#define FWD_CASE(TPR, NI, VEC, RAG)                                                                                        \
     {                                                                                                                      \
         constexpr int rpb = block_of<TPR>() / TPR;                                                                         \
         const long want = (rows + rpb - 1) / rpb, cap = 8L * hw_cu_count();                                                \
-        hipLaunchKernelGGL((tail_fwd_kernel<T, TPR, NI, VEC>), dim3((unsigned)(want < cap ? want : cap)), dim3(block_of<TPR>()), 0, st, a); \
+        hipLaunchKernelGGL((tail_fwd_kernel<T, TPR, NI, VEC, RAG>), dim3((unsigned)(want < cap ? want : cap)), dim3(block_of<TPR>()), 0, st, a); \
     }
     TAIL_VECS(FWD_CASE)
 #undef FWD_CASE
 }
-template <typename T> void tail_bwd_launch(const TailArgs& a, int vec, int slices, hipStream_t st) {
+template <typename T> void tail_bwd_launch(const TailArgs& a, int vec, bool rag, int slices, hipStream_t st) {
     const bool full = a.res || a.gate || a.s || a.w2 || !a.w;
-#define BWD_CASE(TPR, NI, VEC)                                                                                                                  \
+#define BWD_CASE(TPR, NI, VEC, RAG)                                                                                                             \
     {                                                                                                                                           \
-        if (full) hipLaunchKernelGGL((tail_bwd_kernel<T, TPR, NI, VEC, true>), dim3(slices, a.outer), dim3(block_of<TPR>()), 0, st, a);         \
-        else hipLaunchKernelGGL((tail_bwd_kernel<T, TPR, NI, VEC, false>), dim3(slices, a.outer), dim3(block_of<TPR>()), 0, st, a);             \
+        if (full) hipLaunchKernelGGL((tail_bwd_kernel<T, TPR, NI, VEC, RAG, true>), dim3(slices, a.outer), dim3(block_of<TPR>()), 0, st, a);    \
+        else hipLaunchKernelGGL((tail_bwd_kernel<T, TPR, NI, VEC, RAG, false>), dim3(slices, a.outer), dim3(block_of<TPR>()), 0, st, a);        \
     }
     TAIL_VECS(BWD_CASE)
 #undef BWD_CASE
 }
 
-// values per access: 16 bytes' worth where groups and addresses allow it (bf16: or 8 bytes'), one otherwise
-int tail_vec(const TailArgs& a, int b16_io) {
-    const uintptr_t io = (uintptr_t)a.y | (uintptr_t)a.res | (uintptr_t)a.gate | (uintptr_t)a.h | (uintptr_t)a.z | (uintptr_t)a.dh | (uintptr_t)a.dz |
-                         (uintptr_t)a.dy | (uintptr_t)a.dres | (uintptr_t)a.dgate;
-    const uintptr_t par = (uintptr_t)a.w | (uintptr_t)a.b | (uintptr_t)a.s | (uintptr_t)a.w2 | (uintptr_t)a.b2 | (uintptr_t)a.part | (uintptr_t)a.gpart;
+// values per access (16 bytes' worth, bf16 also 8; 1 for groups of one or two values), and whether chunks may straddle groups or end short
+int tail_vec(const TailArgs& a, int b16_io, bool* rag) {
     const int D = a.C / a.G;
-    if (par % 16 || D % 4) return 1;
-    if (b16_io) return D % 8 == 0 && io % 16 == 0 ? 8 : (io % 8 == 0 ? 4 : 1);
-    return io % 16 == 0 ? 4 : 1;
+    *rag = false;
+    if (a.G > 1 && D < 3) return 1;
+    if (b16_io && D % 8 == 0) return 8;
+    *rag = D % 4 != 0;
+    return 4;
 }
 
 int tail_check(const char* what, const TailArgs& a) {
@@ -607,10 +716,10 @@ int ha2g_block_tail_fwd(const void* y, const void* res, const void* gate, const 
     if (const int rc = tail_check("block_tail_fwd", a)) return rc;
     if (outer == 0 || inner == 0) return 0;
     HA2G_REQUIRE(y && h && (!w2 || z) && (!layer || !rs || mu) && (!layer || !rs2 || mu2), "block_tail_fwd: null operand");
-    const int vec = tail_vec(a, b16_io);
-    HA2G_REQUIRE(vec > 1 || C <= 8192, "block_tail_fwd: C=%d > 8192 needs groups of a multiple of 4 and 16-byte aligned operands", C);
-    if (b16_io) tail_fwd_launch<b16>(a, vec, (hipStream_t)stream);
-    else tail_fwd_launch<float>(a, vec, (hipStream_t)stream);
+    bool rag;
+    const int vec = tail_vec(a, b16_io, &rag);
+    if (b16_io) tail_fwd_launch<b16>(a, vec, rag, (hipStream_t)stream);
+    else tail_fwd_launch<float>(a, vec, rag, (hipStream_t)stream);
     HA2G_CHECK_LAUNCH("block_tail_fwd");
     return 0;
 }
@@ -630,11 +739,11 @@ int ha2g_block_tail_bwd(const void* y, const void* res, const void* gate, const 
     const int nvec = (w ? 2 : 0) + (s ? 1 : 0) + (w2 ? 2 : 0);
     HA2G_REQUIRE(y && (!w || rs) && (!w2 || rs2) && (!layer || !w || mu) && (!layer || !w2 || mu2) && (nvec == 0 || (part && dparams)) &&
                  (!(gate && gate_shared) || (gpart && dgate)), "block_tail_bwd: null operand");
-    const int vec = tail_vec(a, b16_io);
-    HA2G_REQUIRE(vec > 1 || C <= 8192, "block_tail_bwd: C=%d > 8192 needs groups of a multiple of 4 and 16-byte aligned operands", C);
+    bool rag;
+    const int vec = tail_vec(a, b16_io, &rag);
     const hipStream_t st = (hipStream_t)stream;
-    if (b16_io) tail_bwd_launch<b16>(a, vec, slices, st);
-    else tail_bwd_launch<float>(a, vec, slices, st);
+    if (b16_io) tail_bwd_launch<b16>(a, vec, rag, slices, st);
+    else tail_bwd_launch<float>(a, vec, rag, slices, st);
     HA2G_CHECK_LAUNCH("block_tail_bwd");
     if (nvec) {
         hipLaunchKernelGGL(slab_sum_kernel<float>, dim3((nvec * C + 63) / 64), dim3(1024), 0, st, part, dparams, slices * outer, nvec * C);

@@ -2164,7 +2164,6 @@ def _norm_refuse(what, y, groups, kind, vectors):
           tuple(y.shape))
     C = y.shape[-1]
     _need(groups >= 1 and C % groups == 0, '%s: %d values in %d groups', what, C, groups)
-    _need((C // groups) % 4 == 0 or C <= 8192, '%s: rows of more than 8192 values need groups of a multiple of 4', what)
     _need(kind in _NORMS, '%s: kind %r (one of %s)', what, kind, ', '.join(_NORMS))
     for t in vectors:
         _need(t is None or (t.shape == (C,) and t.dtype == torch.float32 and t.device == y.device), '%s: weights, biases and scales are fp32 [%d]', what, C)
@@ -2174,8 +2173,7 @@ def _norm_refuse(what, y, groups, kind, vectors):
 
 def _norm_check(what, y, groups, kind, vectors):
     shape = y.shape
-    ok = len(shape) >= 1 and y.dtype in _FLOATS and 1 <= shape[-1] <= 16384 and groups >= 1 and shape[-1] % groups == 0 and kind in _NORMS and y.is_cuda and (
-        shape[-1] <= 8192 or shape[-1] // groups % 4 == 0)
+    ok = len(shape) >= 1 and y.dtype in _FLOATS and 1 <= shape[-1] <= 16384 and groups >= 1 and shape[-1] % groups == 0 and kind in _NORMS and y.is_cuda
     if ok:
         C, dev = shape[-1:], y.device
         for t in vectors:
@@ -2194,7 +2192,7 @@ def _tail_call(*args):
 
 def row_norm(x, weight, bias=None, kind='rms', groups=1, eps=1e-5):
     """The norm in front of a block: x [..., C] (fp32 or bf16) -> norm(x) * weight + bias, normalised over each of `groups` equal parts of a row.
-    kind: 'rms' or 'layer' (the mean is removed).  weight, bias [C] fp32.  C up to 16384 (8192 where C / groups is no multiple of 4)."""
+    kind: 'rms' or 'layer' (the mean is removed).  weight, bias [C] fp32.  C up to 16384."""
     _need(weight is not None, 'row_norm: needs a weight')
     _norm_check('row_norm', x, groups, kind, (weight, bias))
     return _tail_call(x, None, None, weight, bias, None, None, None, groups, kind == 'layer', ACT_NONE, 1.0, float(eps))[0]

@@ -598,7 +598,7 @@ int ha2g_head_sum(const float* x, void* out, long rows, int heads, int n, int D,
  *   n = norm(y) w + b in G groups of C / G (layer != 0: mean removed; otherwise RMS), u = n act(gate), h = alpha res + s u, z = norm(h) w2 + b2 over C.
  * y, res, gate, h, z: rows of C values, fp32 or (b16_io) bf16; parameters [C] fp32; w, b, gate, s, res, w2, b2 may be NULL (w NULL: no norm; w2 NULL:
  * no z).  rows = outer * inner; gate_shared: one gate row per `inner` rows.  act: 0 none, 3 sigmoid, 4 SiLU.  mu, rs [rows * G], mu2, rs2 [rows]:
- * kept for the backward pass (NULL = not kept; mu, mu2 only for layer).  C <= 16384; C <= 8192 where C / G % 4 != 0 or an operand is not aligned to 16.
+ * kept for the backward pass (NULL = not kept; mu, mu2 only for layer).  C <= 16384.
  * bwd: dh, dz (NULL = zero) -> dy, dres, dgate (NULL = not wanted; with gate_shared required), and dparams = [dw][db][ds][dw2][db2] (those whose
  * weight is there; db with w, db2 with w2); part = slices * outer * (their number) * C floats, gpart = slices * outer * C (gate_shared), slices =
  * ha2g_block_tail_slices().  Every sum has a fixed order. */

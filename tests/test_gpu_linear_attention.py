@@ -122,8 +122,21 @@ def test_shared_heads_and_their_gradients(heads, dt):
 
 @pytest.mark.parametrize('dt', (torch.float32, torch.bfloat16), ids=('fp32', 'bf16'))
 @pytest.mark.parametrize('layout', ('fused', 'heads_first', 'inner', 'odd'))
-def test_layouts(layout, dt):
-    check_all(*make(2, 37, 4, 4, 2, 4, 20, 28, dt, seed=4, layout=layout))
+@pytest.mark.parametrize('Dk,Dv', ((20, 28), (25, 35), (64, 128)))
+def test_layouts(layout, Dk, Dv, dt):
+    check_all(*make(2, 37, 4, 4, 2, 4, Dk, Dv, dt, seed=4, layout=layout))
+
+
+def test_tokens_far_apart():
+    """token strides past what a workgroup's 32-bit addresses cover are copied; batch and head strides may be anything"""
+    q, k, v, g, state, do, ds = make(2, 5, 2, 2, 2, 2, 8, 8, torch.float32, seed=14)
+    big = torch.zeros(5 * 4194304 + 64, device=DEV)
+    x = big.as_strided((2, 5, 2, 8), (16, 4194304, 8, 1))
+    x.copy_(q)
+    want = ops.linear_attention(q, k, v, g, state=state)
+    assert torch.equal(ops.linear_attention(x, k, v, g, state=state), want)
+    y = q.transpose(0, 1).contiguous().transpose(0, 1)
+    assert torch.equal(ops.linear_attention(y, k, v, g, state=state), want)
 
 
 @pytest.mark.parametrize('dt', (torch.float32, torch.bfloat16), ids=('fp32', 'bf16'))

@@ -136,7 +136,8 @@ DTS = pytest.mark.parametrize('dt', (torch.float32, torch.bfloat16), ids=('fp32'
 @DTS
 @pytest.mark.parametrize('kind', ('rms', 'layer'))
 @pytest.mark.parametrize('C,G', ((1, 1), (3, 1), (4, 1), (16, 4), (27, 3), (64, 1), (126, 2), (300, 1), (300, 5), (300, 100), (300, 300), (1024, 8), (1025, 1), (1028, 1),
-                                 (2000, 8), (2048, 16), (4100, 1), (5000, 5), (8191, 1), (16384, 128)))
+                                 (2000, 8), (2048, 16), (4100, 1), (5000, 5), (8191, 1), (16384, 128), (284, 4), (5270, 2), (16383, 3), (16384, 8192),
+                                 (1026, 513), (9, 3), (2815, 5), (12, 4), (6000, 1000)))
 def test_row_norm_sizes_and_groups(C, G, kind, dt):
     check_all((13, C), dt, kind=kind, G=G, row_norm=True, seed=C)
 
@@ -158,9 +159,9 @@ def test_every_part_alone_and_together(parts, gate, dt):
 
 @DTS
 @pytest.mark.parametrize('act', (ops.ACT_NONE, ops.ACT_SIGMOID, ops.ACT_SILU))
-@pytest.mark.parametrize('C', (40, 300, 1500, 2048, 4100, 5001))
+@pytest.mark.parametrize('C', (40, 300, 1500, 2048, 4100, 5001, 9999))
 def test_gates_and_widths(C, act, dt):
-    check_all((2, 9, C), dt, kind='layer', parts=('w', 'b', 'res', 'scale', 'w2', 'b2'), gate='token', act=act, seed=C)
+    check_all((2, 9, C), dt, kind='layer', G=3 if C % 3 == 0 else 1, parts=('w', 'b', 'res', 'scale', 'w2', 'b2'), gate='token', act=act, seed=C)
 
 
 @DTS
