@@ -555,13 +555,14 @@ __global__ __launch_bounds__(256) void head_sum_kernel(const float* __restrict__
     }
 }
 
-// Segments of the time axis: one pass over q, k, v where the rows and heads alone give every compute unit a workgroup or more; otherwise the axis is
-// split so that two are there, at no less than four chunks a segment, for a second read of k and v and the segments' states.
-void segments(int B, int T, int H, int b16_io, int* nseg, int* len) {
-    const int C = b16_io ? Mma<b16>::C : Mma<float>::C, chunks = (int)(((long)T + C - 1) / C), cus = hw_cu_count();
+// Segments of the time axis: one pass over q, k, v where the rows and heads alone give every compute unit half of the eight waves it should have;
+// otherwise the axis is split so that the eight are there, at no less than two chunks a segment, for a second read of k and v and the segments'
+// states.  (Twelve or sixteen waves: the scan over the states grows by what the chunks save.)
+void segments(int B, int T, int H, int Dv, int b16_io, int* nseg, int* len) {
+    const int C = b16_io ? Mma<b16>::C : Mma<float>::C, chunks = (int)(((long)T + C - 1) / C), groups = hw_cu_count() * (Dv <= 32 ? 4 : 2);
     const long rows = (long)B * H;
-    long want = rows >= cus || rows < 1 ? 1 : (2L * cus + rows - 1) / rows;
-    if (want > chunks / 4) want = chunks / 4;
+    long want = 2 * rows >= groups || rows < 1 ? 1 : (groups + rows - 1) / rows;
+    if (want > chunks / 2) want = chunks / 2;
     if (want < 1) want = 1;
     const int per = chunks > 0 ? (int)((chunks + want - 1) / want) : 1;
     *nseg = chunks > 0 ? (chunks + per - 1) / per : 1;
@@ -626,7 +627,7 @@ int check_args(LinAttnArgs& a, const char* what, const float* g, const int* leng
     HA2G_REQUIRE(rq >= 1 && rk >= 1 && rv >= 1 && H % rq == 0 && H % rk == 0 && H % rv == 0, "%s: %d heads shared by %d / %d / %d", what, H, rq, rk, rv);
     HA2G_REQUIRE(B == 0 || (g && (T == 0 || operands)), "%s: null operand", what);
     a.g = g; a.lengths = lengths; a.B = B; a.T = T; a.H = H;
-    segments(B, T, H, b16_io, &a.nseg, &a.seg_len);
+    segments(B, T, H, Dv, b16_io, &a.nseg, &a.seg_len);
     HA2G_REQUIRE((long)B * H * a.nseg <= 0x7fffffffL, "%s: B * H * segments = %ld", what, (long)B * H * a.nseg);
     HA2G_REQUIRE((long)T + a.seg_len <= 0x7fffffffL, "%s: T = %d", what, T);
     return 0;
@@ -639,7 +640,7 @@ extern "C" {
 long ha2g_linattn_workspace_floats(int B, int T, int H, int Dk, int Dv, int b16_io) {
     int nseg, len;
     if (B < 1 || H < 1 || T < 1) return 0;
-    segments(B, T, H, b16_io, &nseg, &len);
+    segments(B, T, H, Dv, b16_io, &nseg, &len);
     return (long)B * H * (nseg - 1) * Dk * Dv;
 }
 
