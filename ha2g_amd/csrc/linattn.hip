@@ -274,6 +274,7 @@ __global__ __launch_bounds__(waves_of(DKP, DVP) * 64, occupancy_of(DKP, DVP)) vo
     // powers of the decay: between the tokens of this wave's score tiles (nothing where s > t), in front of a tile of tokens, to the chunk's end
     float pw[MINE][4], pin[CT], wst[CF][KB / 4];
     int tx[MINE], ts[MINE];
+    unsigned past = 0;                                              // a token to come counts as nothing, whatever its score (0 * inf is not 0)
     if constexpr (!STATE_ONLY) {
 #pragma unroll
         for (int m = 0; m < MINE; ++m) {
@@ -283,7 +284,8 @@ __global__ __launch_bounds__(waves_of(DKP, DVP) * 64, occupancy_of(DKP, DVP)) vo
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int d = 16 * (tx[m] - ts[m]) + col - M::srow(grp, i);
-                pw[m][i] = d >= 0 ? J.uscale * J.oscale * decay_power(g, d) : 0.f;
+                pw[m][i] = J.uscale * J.oscale * decay_power(g, max(0, d));
+                past |= (unsigned)(d >= 0) << (4 * m + i);
             }
         }
     }
@@ -335,7 +337,7 @@ __global__ __launch_bounds__(waves_of(DKP, DVP) * 64, occupancy_of(DKP, DVP)) vo
                     for (int w = 0; w < KF; ++w)
                         z = M::mma(M::row(ks, SK::LD, 16 * ts[m] + M::krow(col), w, grp), M::row(qs, SK::LD, 16 * tx[m] + col, w, grp), z);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) z[i] *= pw[m][i];
+                    for (int i = 0; i < 4; ++i) z[i] = past >> (4 * m + i) & 1 ? z[i] * pw[m][i] : 0.f;
                     M::put(ps + (wave + m * NW) * (M::NS * 64) + lane, z);
                 }
             f32x4 acc[CT][VT];

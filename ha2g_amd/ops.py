@@ -2047,6 +2047,7 @@ def linear_attention(q, k, v, log_decay, scale=None, state=None, lengths=None, r
     read in place), Dk and Dv from 1 to 128.  log_decay [H] fp32 <= 0, a constant; Hq, Hk, Hv divide H, head h reads head h // (H // Hx).
     state [B, H, Dk, Dv] fp32: what stands before the first token (None: zero).  lengths [B] int32 on the device: row b ends after lengths[b]
     tokens (clipped to 0 .. T); what lies behind is not read, the output and the gradients there are zero.
+    A value that is not finite reaches the tokens behind it, and may reach up to 31 in front of it (its tile of the products).
     Returns o [B, T, H, Dv] in v's type, with return_state also the state behind each row's last token, fp32."""
     _, Dk, _ = _la_check('linear_attention', q, k, v, log_decay, state, 4)
     if lengths is not None:
@@ -2077,7 +2078,8 @@ def linear_attention_step(q, k, v, log_decay, state, scale=None):
         check(lib.ha2g_linattn_step(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), log_decay.data_ptr(), state.data_ptr(),
                                     array('l', (qb, 0, qh, kb, 0, kh, vb, 0, vh, H * Dv, 0, Dv)), B, H, H // q.shape[1], H // k.shape[1], H // v.shape[1], Dk, Dv,
                                     float(Dk ** -0.5 if scale is None else scale), q.dtype == torch.bfloat16, _stream()))
-    torch.autograd.graph.increment_version(state)
+    if not state.is_inference():
+        torch.autograd.graph.increment_version(state)
     return o
 
 

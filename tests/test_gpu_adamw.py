@@ -269,3 +269,20 @@ def test_the_trainer_steps_with_it(kind):
     for o, b in zip(tr.gen_opts, before):
         d = (o.flat_p - b).abs()
         assert torch.isfinite(o.flat_p).all() and 0 < float(d.max()) <= 2 * float(tr.args.learning_rate) * 2.0 ** 0.5 * (1 + 0.05) * 4
+
+
+def test_a_tensor_of_more_than_two_to_the_31_elements():
+    n, m0 = 2 ** 31 + 300, 2 ** 31 - 128
+    p, g = torch.zeros(n, dtype=torch.bfloat16, device=DEV), torch.zeros(n, dtype=torch.bfloat16, device=DEV)
+    m, v = optim.adamw_state8(p), optim.adamw_state8(p)
+    (pt,), (gt,) = tensors((n - m0,), torch.bfloat16, 1), tensors((n - m0,), torch.bfloat16, 2, 1e-3)
+    p[m0:], g[m0:] = pt, gt
+    step = torch.full((1,), 9, dtype=torch.int32, device=DEV)
+    optim.adamw_step([p], [g], [m], [v], step, seed=3, **HP)
+    wp, wm, wv, tp, tm, _ = formula(pt, gt, torch.zeros(n - m0), torch.zeros(n - m0), 10)
+    tp = tp + 2.0 ** -8 * (wp.abs() + tp)
+    assert ((p[m0:].double().cpu() - wp).abs() <= tp).all() and not p[:m0:65537].any()
+    key = hash32(torch.tensor(int(hash32(torch.tensor(int(hash32(torch.tensor(3))) ^ 10)))))
+    d = hash32(torch.arange(m0, n) ^ int(key))
+    check_codes(wm, tm, m[0][m0:], m[1][m0 // 128:], d >> 16)
+    check_codes(wv.sqrt(), 4 * U * wv.sqrt(), v[0][m0:], v[1][m0 // 128:], d & 0xffff)

@@ -267,3 +267,40 @@ def test_two_streams_and_a_captured_graph():
         eager = run(a)
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(out, w)) and all(torch.equal(p, q) for p, q in zip(eager, want[0]))
+
+
+def test_inference_mode_and_values_past_the_range_of_masked_scores():
+    q, k, v, g, state, _, _ = make(2, 40, 2, 2, 2, 2, 16, 16, torch.float32, seed=15)
+    with torch.inference_mode():
+        s = state.clone()
+        ops.linear_attention_step(q[:, 0].clone(), k[:, 0].clone(), v[:, 0].clone(), g, s)
+        o, last = ops.linear_attention(q[:, :1].clone(), k[:, :1].clone(), v[:, :1].clone(), g, state=state, return_state=True)
+        assert float((s - last).norm() / last.norm()) <= 2.0 ** -20
+    # scores of tokens to come that overflow do not reach the tokens in front of them
+    want = ops.linear_attention(q[:, :20], k[:, :20], v[:, :20], g, state=state)
+    q2, k2 = q.clone(), k.clone()
+    k2[:, 20:] = 3e38
+    k2[:, 20:, :, ::2] = -3e38
+    got = ops.linear_attention(q2, k2, torch.where(torch.arange(40, device=DEV)[None, :, None, None] < 20, v, 0.0), g, state=state)
+    assert torch.equal(got[:, :20], want)
+
+
+def test_rows_past_two_to_the_32_elements():
+    """batch rows 2^32 elements apart (8.6 GB of bf16): the addresses of q, k, v and do of the second row need more than 32 bits"""
+    q, k, v, g, state, do, ds = make(2, 70, 2, 2, 2, 2, 16, 24, torch.bfloat16, seed=16)
+    far = 2 ** 32 + 8
+    buf = torch.empty(far + 4 * 70 * 2 * 24, dtype=torch.bfloat16, device=DEV)
+    views = []
+    at = 0
+    for x in (q, k, v, do):
+        y = buf.as_strided(x.shape, (far, x.shape[2] * x.shape[3], x.shape[3], 1), at)
+        y.copy_(x)
+        at += x[0].numel()
+        views.append(y)
+
+    def run(q, k, v, do):
+        ls = [x.detach().requires_grad_() for x in (q, k, v, state)]
+        o, s = ops.linear_attention(*ls[:3], g, state=ls[3], return_state=True)
+        return [o.detach(), s.detach(), *torch.autograd.grad([o, s], ls, [do, ds])]
+    for a, b in zip(run(q, k, v, do), run(*views)):
+        assert torch.equal(a, b)

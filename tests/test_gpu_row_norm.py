@@ -235,3 +235,22 @@ def test_graph_replays_and_streams():
         eager = run(*a)
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(out, w)) and all(torch.equal(p, q) for p, q in zip(eager, want[0]))
+
+
+def test_rows_past_two_to_the_32_elements():
+    """2^32 + elements of bf16, forward and backward: the rows at the end are those of a small call"""
+    C, rows = 4100, 2 ** 20 + 5
+    assert rows * C > 2 ** 32
+    y = torch.empty(rows, C, dtype=torch.bfloat16, device=DEV)
+    y[:8].normal_()
+    y[8:-8] = 0.0
+    y[-8:].normal_()
+    w = torch.randn(C, device=DEV)
+    h = ops.row_norm(y, w)
+    assert torch.equal(h[-8:], ops.row_norm(y[-8:], w)) and torch.equal(h[:8], ops.row_norm(y[:8], w)) and not h[8:-8:4097].any()
+    y.requires_grad_()
+    h = ops.row_norm(y, w)
+    dy, = torch.autograd.grad(h, y, h.detach())
+    tail = y.detach()[-8:].clone().requires_grad_()
+    ht = ops.row_norm(tail, w)
+    assert torch.equal(dy[-8:], torch.autograd.grad(ht, tail, ht.detach())[0])
