@@ -11,6 +11,7 @@
 namespace {
 
 constexpr int AW_TENSORS = 64;      // per launch: the table travels by value in the kernel's arguments
+constexpr long AW_CHUNKS = (1L << 24) - 1;      // per launch: a grid has less than 2^32 threads
 
 struct AdamWTable {
     void *p[AW_TENSORS], *g[AW_TENSORS], *m[AW_TENSORS], *v[AW_TENSORS];
@@ -238,7 +239,7 @@ int ha2g_adamw_multi(int n, const long* p, const long* g, const long* m, const l
     t.vec = 0;
     t.start[0] = 0;
     auto flush = [&]() {
-        if (t.count == 0) return 0;
+        if (t.count == 0 || t.start[t.count] == 0) { t.count = 0; t.vec = 0; return 0; }      // nothing, or tensors without elements
         const hipStream_t st = (hipStream_t)stream;
         if (p_b16) { if (g_b16) adamw_launch<b16, b16>(t, sc, bits, st); else adamw_launch<b16, float>(t, sc, bits, st); }
         else { if (g_b16) adamw_launch<float, b16>(t, sc, bits, st); else adamw_launch<float, float>(t, sc, bits, st); }
@@ -250,8 +251,8 @@ int ha2g_adamw_multi(int n, const long* p, const long* g, const long* m, const l
     for (int i = 0; i < n; ++i) {
         HA2G_REQUIRE(len[i] >= 0, "adamw: tensor %d has %ld elements", i, len[i]);
         const long chunks = (len[i] + chunk - 1) / chunk;
-        HA2G_REQUIRE(chunks <= 0x7fffffffL / 2, "adamw: tensor %d has %ld elements", i, len[i]);
-        if (t.count == AW_TENSORS || (t.count && t.start[t.count] + chunks > 0x7fffffffL)) {
+        HA2G_REQUIRE(chunks <= AW_CHUNKS, "adamw: tensor %d has %ld elements", i, len[i]);
+        if (t.count == AW_TENSORS || (t.count && t.start[t.count] + chunks > AW_CHUNKS)) {
             if (const int rc = flush()) return rc;
         }
         if (t.count == 0) t.first = first + i;

@@ -177,17 +177,23 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9, 
         _adamw_check(params, grads, ms, vs, sm, sr, q8, dev, pt, gt, num)
     if n == 0:
         return
-    pp = _ptrs(params)
-    _need(len(set(pp)) >= n - num.count(0), 'adamw_step: a parameter is listed twice')
+    pp, pm, pv = _ptrs(params), _ptrs(ms), _ptrs(vs)
+    own = pp + pm + pv if 0 not in num else [x for t in (pp, pm, pv) for x, k in zip(t, num) if k]
+    _need(len(set(own)) == len(own), 'adamw_step: a parameter or a state is listed twice')
     with _on(step):
         st, gp = _stream(), None if guard is None else guard.data_ptr()
         sc = torch.empty(4, dtype=f32, device=dev)
         sp = sc.data_ptr()
         b1, b2, lr = float(betas[0]), float(betas[1]), float(lr)
         check(lib.ha2g_adamw_scalars(step.data_ptr(), gp, lr, b1, b2, sp, st))
-        check(lib.ha2g_adamw_multi(n, pp, _ptrs(grads), _ptrs(ms), _ptrs(vs), _ptrs(sm) if q8 else None, _ptrs(sr) if q8 else None, array.array('l', num),
+        check(lib.ha2g_adamw_multi(n, pp, _ptrs(grads), pm, pv, _ptrs(sm) if q8 else None, _ptrs(sr) if q8 else None, array.array('l', num),
                                    pt is torch.bfloat16, gt is torch.bfloat16, 8 if q8 else 32, lr, b1, b2, float(eps), float(weight_decay),
                                    int(seed) & 0xffffffff, 0, sp, gp, st))
+    # a graph that saved a parameter's old value refuses its backward pass from here on
+    try:
+        torch.autograd.graph.increment_version(params)
+    except RuntimeError:                                  # inference tensors have no versions
+        torch.autograd.graph.increment_version([p for p in params if not p.is_inference()])
 
 
 def _adamw_check(params, grads, ms, vs, sm, sr, q8, dev, pt, gt, num):

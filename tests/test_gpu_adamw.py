@@ -286,3 +286,37 @@ def test_a_tensor_of_more_than_two_to_the_31_elements():
     d = hash32(torch.arange(m0, n) ^ int(key))
     check_codes(wm, tm, m[0][m0:], m[1][m0 // 128:], d >> 16)
     check_codes(wv.sqrt(), 4 * U * wv.sqrt(), v[0][m0:], v[1][m0 // 128:], d & 0xffff)
+
+
+def test_lists_without_elements_and_tensors_listed_twice():
+    none = lambda k: [torch.empty(0, device=DEV) for _ in range(k)]      # noqa: E731
+    step = torch.zeros(1, dtype=torch.int32, device=DEV)
+    optim.adamw_step(none(70), none(70), none(70), none(70), step)
+    assert int(step) == 1
+    # a whole launch's table of them in front of one that has elements
+    p, g, m, v = ([*none(64), x] for x in (torch.ones(5, device=DEV), torch.ones(5, device=DEV), torch.zeros(5, device=DEV), torch.zeros(5, device=DEV)))
+    optim.adamw_step(p, g, m, v, step, **HP)
+    want, _, _, tol, _, _ = formula(torch.ones(5), torch.ones(5), torch.zeros(5), torch.zeros(5), 2)
+    assert ((p[-1].double().cpu() - want).abs() <= tol).all()
+    a, b, c, d = (torch.ones(8, device=DEV) for _ in range(4))
+    e = torch.empty(0, device=DEV)
+    for ps, gs, ms, vs in (([a], [b], [c], [c]), ([a], [b], [a], [c]), ([a, a, e], [b, b, e], [c, d, e], [b.clone(), b.clone(), e])):
+        with pytest.raises(ValueError, match='twice'):
+            optim.adamw_step(ps, gs, ms, vs, step)
+    s8 = [optim.adamw_state8(a)]
+    with pytest.raises(ValueError, match='twice'):
+        optim.adamw_step([a], [b], s8, s8, step)
+    assert int(step) == 2 and (a == 1).all()
+
+
+def test_a_graph_that_saved_the_old_parameter_refuses_its_backward_pass():
+    p = torch.ones(8, device=DEV).requires_grad_()
+    y = (p * p).sum()
+    step, z = torch.zeros(1, dtype=torch.int32, device=DEV), [torch.zeros(8, device=DEV) for _ in range(2)]
+    optim.adamw_step([p], [torch.ones(8, device=DEV)], z[:1], z[1:], step)
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        y.backward()
+    with torch.inference_mode():
+        q, z = torch.ones(8, device=DEV), [torch.zeros(8, device=DEV) for _ in range(2)]
+        optim.adamw_step([q], [torch.ones(8, device=DEV)], z[:1], z[1:], step)
+    assert (q < 1).all()
