@@ -630,7 +630,7 @@ int check_args(LinAttnArgs& a, const char* what, const float* g, const int* leng
     HA2G_REQUIRE(B == 0 || (g && (T == 0 || operands)), "%s: null operand", what);
     a.g = g; a.lengths = lengths; a.B = B; a.T = T; a.H = H;
     segments(B, T, H, Dv, b16_io, &a.nseg, &a.seg_len);
-    HA2G_REQUIRE((long)B * H * a.nseg <= 0x7fffffffL, "%s: B * H * segments = %ld", what, (long)B * H * a.nseg);
+    HA2G_REQUIRE((long)B * H * a.nseg < 1L << 23, "%s: B * H * segments = %ld (a grid has less than 2^32 threads)", what, (long)B * H * a.nseg);
     HA2G_REQUIRE((long)T + a.seg_len <= 0x7fffffffL, "%s: T = %d", what, T);
     return 0;
 }

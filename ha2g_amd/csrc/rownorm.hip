@@ -666,7 +666,7 @@ template <typename T> void tail_fwd_launch(const TailArgs& a, int vec, bool rag,
 #undef FWD_CASE
 }
 template <typename T> void tail_bwd_launch(const TailArgs& a, int vec, bool rag, int slices, hipStream_t st) {
-    const bool full = a.res || a.gate || a.s || a.w2 || !a.w;
+    const bool full = a.dres || a.gate || a.s || a.w2 || !a.w;
 #define BWD_CASE(TPR, NI, VEC, RAG)                                                                                                             \
     {                                                                                                                                           \
         if (full) hipLaunchKernelGGL((tail_bwd_kernel<T, TPR, NI, VEC, RAG, true>), dim3(slices, a.outer), dim3(block_of<TPR>()), 0, st, a);    \

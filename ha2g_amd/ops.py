@@ -7,6 +7,7 @@ import os
 from array import array
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from ._lib import check, lib
 
@@ -1930,6 +1931,12 @@ def _on(t):
     return _here if t.device.index == _cur_device() else torch.cuda.device(t.device)
 
 
+def _once(backward):
+    """a backward pass without one of its own: create_graph=True gets a node that refuses a second derivative (the check costs its time only there)"""
+    guarded = once_differentiable(backward)
+    return lambda ctx, *grads: (guarded if torch.is_grad_enabled() else backward)(ctx, *grads)
+
+
 def _inner1(x):
     return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
 
@@ -2012,6 +2019,7 @@ class LinearAttentionFunction(torch.autograd.Function):
         return o, s
 
     @staticmethod
+    @_once
     def backward(ctx, do, ds):
         q, k, v, g, state, lengths, ws_fwd = ctx.saved_tensors
         (B, T, Hq, Dk), H, Hk, Hv, Dv = q.shape, g.shape[0], k.shape[2], v.shape[2], v.shape[3]
@@ -2124,10 +2132,13 @@ class BlockTailFunction(torch.autograd.Function):
     def forward(ctx, y, res, gate, w, b, s, w2, b2, groups, layer, act, alpha, eps):
         ctx.set_materialize_grads(False)
         h, z, ops, st, ctx.shape = _tail_forward(y, res, gate, w, b, s, w2, b2, groups, layer, act, alpha, eps, True)
+        if w2 is None:
+            ops[1] = None                        # only the second norm's gradient reads the residual: otherwise it is free to be changed in place
         ctx.save_for_backward(*ops, st)
         return h, z
 
     @staticmethod
+    @_once
     def backward(ctx, dh, dz):
         y, res, gate, w, b, s, w2, b2, st = ctx.saved_tensors
         outer, inner, shared, C, groups, layer, act, alpha, eps = ctx.shape
@@ -2135,7 +2146,7 @@ class BlockTailFunction(torch.autograd.Function):
         dh, dz = (None if t is None else t.contiguous() for t in (dh, dz))
         with _on(y):
             dy = torch.empty_like(y) if need[0] else None
-            dres = torch.empty_like(y) if res is not None and need[1] else None
+            dres = torch.empty_like(y) if need[1] else None
             dgate = torch.empty_like(gate) if gate is not None and (need[2] or shared) else None
             nvec = 2 * (w is not None) + (s is not None) + 2 * (w2 is not None)
             n = lib.ha2g_block_tail_slices(outer, inner, C)

@@ -304,3 +304,20 @@ def test_rows_past_two_to_the_32_elements():
         return [o.detach(), s.detach(), *torch.autograd.grad([o, s], ls, [do, ds])]
     for a, b in zip(run(q, k, v, do), run(*views)):
         assert torch.equal(a, b)
+
+
+def test_a_second_derivative_is_refused():
+    q, k, v, g, _, _, _ = make(2, 5, 2, 2, 2, 2, 8, 8, torch.float32, seed=17)
+    q = q.detach().requires_grad_()
+    gq, = torch.autograd.grad(ops.linear_attention(q, k.detach(), v.detach(), g).square().sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError, match='once_differentiable'):
+        (gq.sum() + q.sum()).backward()
+
+
+def test_more_rows_and_heads_than_a_grid_holds_are_refused():
+    x = torch.empty(1, 1, 1, 1, device=DEV).expand(1 << 16, 1, 1 << 7, 1)
+    g = torch.zeros(1 << 7, device=DEV)
+    with pytest.raises(RuntimeError, match=r'2\^32'):
+        ops.linear_attention(x, x, x, g)
+    with pytest.raises(RuntimeError, match=r'2\^32'):
+        ops.linear_attention_step(x[:, 0], x[:, 0], x[:, 0], g, torch.zeros(1 << 16, 1 << 7, 1, 1, device=DEV))

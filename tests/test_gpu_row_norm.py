@@ -254,3 +254,25 @@ def test_rows_past_two_to_the_32_elements():
     tail = y.detach()[-8:].clone().requires_grad_()
     ht = ops.row_norm(tail, w)
     assert torch.equal(dy[-8:], torch.autograd.grad(ht, tail, ht.detach())[0])
+
+
+def test_the_residual_may_be_changed_in_place_unless_the_second_norm_reads_it():
+    y, res, w, w2 = (torch.randn(*s, device=DEV).requires_grad_() for s in ((6, 40), (6, 40), (40,), (40,)))
+    dh = torch.randn(6, 40, device=DEV)
+    want = torch.autograd.grad(ops.block_tail(y, res * 1, weight=w, alpha=0.5), (y, res, w), dh)
+    r = res * 1
+    h = ops.block_tail(y, r, weight=w, alpha=0.5)
+    r.add_(1.0)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(h, (y, res, w), dh), want)) and torch.equal(want[1], 0.5 * dh)
+    r = res * 1
+    h, z = ops.block_tail(y, r, weight=w, next_weight=w2)
+    r.add_(1.0)
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        torch.autograd.grad(z, y, dh)
+
+
+def test_a_second_derivative_is_refused():
+    y, w = torch.randn(3, 8, device=DEV).requires_grad_(), torch.ones(8, device=DEV)
+    gy, = torch.autograd.grad(ops.row_norm(y, w).square().sum(), y, create_graph=True)
+    with pytest.raises(RuntimeError, match='once_differentiable'):
+        (gy.sum() + y.sum()).backward()
