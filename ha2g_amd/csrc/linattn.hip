@@ -198,6 +198,18 @@ template <typename T, int D, int C, int NT, bool WHOLE> struct Stage {     // a 
     }
 };
 
+// Items of work whose operands come from LDS, each read D items ahead of its use: left alone, the compiler reads every operand right in front of the
+// product that waits for it.  Vector arithmetic may move between the items, reads and products may not.
+template <int N, int D, typename Load, typename Use> __device__ __forceinline__ void ahead(Load load, Use use) {
+    decltype(load(0)) f[D + 1];
+#pragma unroll
+    for (int i = 0; i < N + D; ++i) {
+        if (i < N) f[i % (D + 1)] = load(i);
+        if (i >= D) use(i - D, f[(i - D) % (D + 1)]);
+        __builtin_amdgcn_sched_barrier(0x6);
+    }
+}
+
 __device__ __forceinline__ float decay_power(float g, int n) { return n == 0 ? 1.f : expf(g * (float)n); }
 __device__ __forceinline__ int row_length(const LinAttnArgs& a, int b) { return a.lengths ? min(max(a.lengths[b], 0), a.T) : a.T; }
 
@@ -333,9 +345,9 @@ __global__ __launch_bounds__(waves_of(DKP, DVP) * 64, occupancy_of(DKP, DVP)) vo
             for (int m = 0; m < MINE; ++m)
                 if (wave + m * NW < TILES) {
                     f32x4 z = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int w = 0; w < KF; ++w)
-                        z = M::mma(M::row(ks, SK::LD, 16 * ts[m] + M::krow(col), w, grp), M::row(qs, SK::LD, 16 * tx[m] + col, w, grp), z);
+                    struct Pair { typename M::Frag k, q; };
+                    ahead<KF, KF>([&](int w) { return Pair{M::row(ks, SK::LD, 16 * ts[m] + M::krow(col), w, grp), M::row(qs, SK::LD, 16 * tx[m] + col, w, grp)}; },
+                                  [&](int, const Pair& f) { z = M::mma(f.k, f.q, z); });
 #pragma unroll
                     for (int i = 0; i < 4; ++i) z[i] = past >> (4 * m + i) & 1 ? z[i] * pw[m][i] : 0.f;
                     M::put(ps + (wave + m * NW) * (M::NS * 64) + lane, z);
@@ -346,25 +358,23 @@ __global__ __launch_bounds__(waves_of(DKP, DVP) * 64, occupancy_of(DKP, DVP)) vo
 #pragma unroll
                 for (int y = 0; y < VT; ++y) acc[x][y] = f32x4{0.f, 0.f, 0.f, 0.f};
             // q S
+            typename M::Frag sf[VT][M::NS];
+            ahead<KF * CT, 2>([&](int i) { return M::row(qs, SK::LD, 16 * (i % CT) + col, i / CT, grp); },
+                              [&](int i, const typename M::Frag& qf) {
+                const int x = i % CT, u = i / CT;
+                if (x == 0)
 #pragma unroll
-            for (int u = 0; u < KF; ++u) {
-                typename M::Frag sf[VT][M::NS];
+                    for (int y = 0; y < VT; ++y) {
+                        f32x4 t[TPF];
 #pragma unroll
-                for (int y = 0; y < VT; ++y) {
-                    f32x4 t[TPF];
+                        for (int p = 0; p < TPF; ++p) t[p] = S[u * TPF + p][y];
+                        M::template pieces<M::NS>(t, sf[y]);
+                    }
 #pragma unroll
-                    for (int p = 0; p < TPF; ++p) t[p] = S[u * TPF + p][y];
-                    M::template pieces<M::NS>(t, sf[y]);
-                }
+                for (int p = M::NS - 1; p >= 0; --p)
 #pragma unroll
-                for (int x = 0; x < CT; ++x) {
-                    const typename M::Frag qf = M::row(qs, SK::LD, 16 * x + col, u, grp);
-#pragma unroll
-                    for (int y = 0; y < VT; ++y)
-#pragma unroll
-                        for (int p = M::NS - 1; p >= 0; --p) acc[x][y] = M::mma(sf[y][p], qf, acc[x][y]);
-                }
-            }
+                    for (int y = 0; y < VT; ++y) acc[x][y] = M::mma(sf[y][p], qf, acc[x][y]);
+            });
 #pragma unroll
             for (int x = 0; x < CT; ++x)
 #pragma unroll
@@ -377,12 +387,13 @@ __global__ __launch_bounds__(waves_of(DKP, DVP) * 64, occupancy_of(DKP, DVP)) vo
 #pragma unroll
                 for (int u = 0; u * TPF <= x; ++u) {
                     const typename M::Tile* t = ps + (x * (x + 1) / 2 + u * TPF) * (M::NS * 64) + lane;
+                    typename M::Frag pf[M::NS];
 #pragma unroll
-                    for (int p = M::NS - 1; p >= 0; --p) {
-                        const typename M::Frag pf = M::get(t + 64 * p, u * TPF + 1 <= x);
+                    for (int p = 0; p < M::NS; ++p) pf[p] = M::get(t + 64 * p, u * TPF + 1 <= x);
 #pragma unroll
-                        for (int y = 0; y < VT; ++y) acc[x][y] = M::mma(vf[u][y], pf, acc[x][y]);
-                    }
+                    for (int p = M::NS - 1; p >= 0; --p)
+#pragma unroll
+                        for (int y = 0; y < VT; ++y) acc[x][y] = M::mma(vf[u][y], pf[p], acc[x][y]);
                 }
                 const int r = 16 * x + col;
                 if (r < L) {
@@ -392,7 +403,7 @@ __global__ __launch_bounds__(waves_of(DKP, DVP) * 64, occupancy_of(DKP, DVP)) vo
                         const int j = v0 + 16 * y + 4 * grp;
                         if (j >= Dv) continue;
                         char* const at = row + 16 * y * osize + olane;
-                        if (j + 4 <= Dv) {
+                        if (WHOLE || j + 4 <= Dv) {
                             if (J.o16) store4((b16*)at, acc[x][y]); else store4((float*)at, acc[x][y]);
                         } else {
 #pragma unroll
@@ -418,24 +429,22 @@ __global__ __launch_bounds__(waves_of(DKP, DVP) * 64, occupancy_of(DKP, DVP)) vo
             for (int y = 0; y < VT; ++y)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) S[x][y][i] = __builtin_fmaf(S[x][y][i], m1, S[x][y][i]);
+        typename M::Frag wf[VT][M::NV];
+        ahead<CF * KT, 2>([&](int i) { return M::state_col(ks, SK::LD, i % KT, i / KT, lane); },
+                          [&](int i, const typename M::Frag& kf) {
+            const int x = i % KT, u = i / KT;
+            if (x == 0)
 #pragma unroll
-        for (int u = 0; u < CF; ++u) {
-            typename M::Frag wf[VT][M::NV];
+                for (int y = 0; y < VT; ++y) {
+                    f32x4 t[TPF];
+                    M::scaled(vf[u][y], wst[u], t);
+                    M::template pieces<M::NV>(t, wf[y]);
+                }
 #pragma unroll
-            for (int y = 0; y < VT; ++y) {
-                f32x4 t[TPF];
-                M::scaled(vf[u][y], wst[u], t);
-                M::template pieces<M::NV>(t, wf[y]);
-            }
+            for (int p = M::NV - 1; p >= 0; --p)
 #pragma unroll
-            for (int x = 0; x < KT; ++x) {
-                const typename M::Frag kf = M::state_col(ks, SK::LD, x, u, lane);
-#pragma unroll
-                for (int y = 0; y < VT; ++y)
-#pragma unroll
-                    for (int p = M::NV - 1; p >= 0; --p) S[x][y] = M::mma(kf, wf[y][p], S[x][y]);
-            }
-        }
+                for (int y = 0; y < VT; ++y) S[x][y] = M::mma(kf, wf[y][p], S[x][y]);
+        });
     }
     float* s_out;
     int oi = J.si, oj = J.sj;
