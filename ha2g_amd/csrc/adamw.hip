@@ -62,8 +62,11 @@ __device__ __forceinline__ int find_tensor(const AdamWTable& t, int c) {
     return lo;
 }
 
+// A block per chunk: long enough that its search in the table is small beside its memory time, short enough for a model's tensors to fill the chip
 constexpr int CHUNK32 = 4096, CHUNK8 = 4096;
 
+// Bound by memory: 28 bytes an element with everything in fp32.  A generator's 13.1 million parameters in 53 tensors: 57 us = 6.4 TB/s where the last
+// step's data is partly in the last-level cache; 80 us = 4.6 TB/s where it is not.
 template <typename TP, typename TG>
 __global__ __launch_bounds__(256) void adamw32_kernel(const AdamWTable tab, const AdamWScalars sc) {
     if (sc.guard != nullptr && *sc.guard != 0) return;
@@ -117,7 +120,8 @@ __device__ __forceinline__ unsigned encode(float x, float inv, float dither) {
     return code | (x < 0.f ? 0x80u : 0u);
 }
 
-// 16 lanes hold a block of 128 elements, 8 consecutive ones each; a thread does this for CHUNK8 / 2048 places
+// 16 lanes hold a block of 128 elements, 8 consecutive ones each; a thread does this for CHUNK8 / 2048 places.  Bound by memory: 14 bytes an element
+// with bf16 gradients; 115 million parameters 315 us = 5.1 TB/s.
 template <typename TP, typename TG>
 __global__ __launch_bounds__(256) void adamw8_kernel(const AdamWTable tab, const AdamWScalars sc) {
     if (sc.guard != nullptr && *sc.guard != 0) return;

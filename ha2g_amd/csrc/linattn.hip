@@ -37,14 +37,18 @@ template <> __device__ __forceinline__ void st1<b16>(b16* p, long i, float v) {
 }
 
 // ---- chunked form --------------------------------------------------------------------------------------------------------------------------
-// C tokens at a time (fp32: 32, bf16: 64), positions i, j inside the chunk, e = 1 forward and 0 from the end:
+// C tokens at a time (fp32: 32, bf16: 64; half of that for Dk > 64), positions i, j inside the chunk, e = 1 forward and 0 from the end:
 //     o_i = e^{g (i + e)} q_i S + sum_{j <= i} e^{g (i - j)} (q_i k_j) v_j,        S <- e^{g C} S + sum_j e^{g (C - e - j)} k_j v_j^T
 // A workgroup owns a (batch row, head, segment of the time axis); its waves split the columns of v, each keeps its Dk x DVW slice of S in MFMA
 // accumulators for the whole segment.  The accumulator layout (column = lane & 15, row = 4 (lane >> 4) + i) is that of an operand whose k runs along
-// the rows, up to an order of k that both operands may share: S and the scores k q^T go from accumulators into the next product without
-// touching the state's LDS copy.  Rows of LDS are padded by 32 bytes: 16-byte reads of 16 rows and transpose reads of 4 x 16 blocks meet every bank once (row reads
-// of 2 x 8 bytes had two thirds of the LDS time in conflicts).
+// the rows, up to an order of k that both operands may share: S goes from accumulators straight into the next product and is never laid out again.
+// The scores k q^T are the same for all columns of v: each wave computes its share of their 16 x 16 tiles and leaves them in LDS as the next
+// product's operands, for all.  Rows of LDS are padded by 32 bytes: 16-byte reads of 16 rows and transpose reads of 4 x 16 blocks meet every bank
+// once (row reads of 2 x 8 bytes had two thirds of the LDS time in conflicts).
 //     o^T = S^T q^T + v^T (k q^T):  a lane ends with 4 consecutive columns of one token.
+// Measured: 512 (row, head) pairs of 1 024 tokens, bf16: Dk = Dv = 64 59 us (q, k, v and o at 4.5 TB/s; a large copy 4.9), 128 132 us (4.1 TB/s);
+// fp32: 122 us (4.4 TB/s) and 358 us (3.0).  Bound by memory at 64, at 128 by the issue of two waves per SIMD: per chunk and wave ~500 vector
+// instructions (200 of them split S, 64 decay it) beside 91 matrix instructions, matrix units 30 % busy.
 // fp32 operands run on the fp32 MFMA.  bf16 operands are exact as they are; what is computed is split into bf16 pieces: S and the scores, which
 // only reach the bf16 result, into two (2^-17), the decayed v that is added to S into three (all 24 bits: S stays fp32-exact).
 // The decay of S is S + S (e^{gC} - 1): a factor rounded to fp32 is off the same way in every chunk, 1e-4 of a state with a memory of 2^12 tokens.
@@ -199,7 +203,8 @@ template <typename T, int D, int C, int NT, bool WHOLE> struct Stage {     // a 
 };
 
 // Items of work whose operands come from LDS, each read D items ahead of its use: left alone, the compiler reads every operand right in front of the
-// product that waits for it.  Vector arithmetic may move between the items, reads and products may not.
+// product that waits for it (8 heads of 32 768 tokens in fp32: 75 us, 68 this way).  Vector arithmetic may move between the items, reads and
+// products may not.
 template <int N, int D, typename Load, typename Use> __device__ __forceinline__ void ahead(Load load, Use use) {
     decltype(load(0)) f[D + 1];
 #pragma unroll
@@ -218,11 +223,13 @@ __device__ __forceinline__ int row_length(const LinAttnArgs& a, int b) { return 
 __device__ __forceinline__ long xcd_order(long i, long n) { return n % 8 == 0 ? i % 8 * (n / 8) + i / 8 : i; }
 
 // Waves of a workgroup: 16 columns of v each, 32 where Dk and v are both long (or Dk is too short for eight waves to share its rows).  Dk = 64 with
-// 128 columns fits 128 registers, so that two workgroups of eight waves run on a compute unit (ragged prompts: 45 us, 50 with four waves);
-// Dk = 128 does not, and eight waves of one workgroup in step with each other are slower than two workgroups of four (164 us, 137).
+// 128 columns fits 128 registers, so that two workgroups of eight waves run on a compute unit (three rows of up to 5 003 tokens, 12 heads, bf16:
+// 42 us, 50 with four waves); Dk = 128 does not, and eight waves of one workgroup in step with each other are slower than two workgroups of four
+// (512 pairs of 1 024 tokens: 141 us, 132).  With three waves per SIMD (168 registers, some of them spilled) Dk = Dv = 128 takes 217 us.
 constexpr int waves_of(int DKP, int DVP) { return DVP < 64 ? DVP / 16 : (DKP == 64 && DVP == 128 ? 8 : 4); }
 constexpr int occupancy_of(int DKP, int DVP) { return waves_of(DKP, DVP) == 8 ? 4 : 2; }
-// With Dk > 64 the state takes up to 64 registers of a wave: a chunk half as long leaves room for two waves per SIMD.
+// With Dk > 64 the state takes up to 64 registers of a wave: a chunk half as long leaves room for two waves per SIMD (bf16, 512 pairs of 1 024
+// tokens: 132 us, 144 with the whole chunk; for Dk <= 64 half a chunk gains 3 % in bf16 and loses 6 % in fp32).
 template <typename T> constexpr int chunk_of(int DKP) { return DKP > 64 ? Mma<T>::C / 2 : Mma<T>::C; }
 
 // STATE_ONLY: the segment's own contribution to the state (from zero), nothing is read of q and no o is written.  Two waves per SIMD at least:
@@ -473,7 +480,8 @@ __global__ __launch_bounds__(waves_of(DKP, DVP) * 64, occupancy_of(DKP, DVP)) vo
             }
 }
 
-// seg[i] <- the state behind segment i: one thread per element, the segments' own contributions loaded eight at a time
+// seg[i] <- the state behind segment i: one thread per element, the segments' own contributions loaded eight at a time (8 pairs of 64 states of
+// 64 x 64: 10.5 us, the latency of eight such rounds; 36 pairs of 15 states of 64 x 128: 7 us)
 __global__ __launch_bounds__(256) void linattn_segment_scan_kernel(const LinAttnArgs a) {
     const Job& J = a.job[0];
     const int x = blockIdx.y * 256 + threadIdx.x, D = J.Dk * J.Dv, bh = blockIdx.x;
@@ -497,7 +505,8 @@ __global__ __launch_bounds__(256) void linattn_segment_scan_kernel(const LinAttn
 }
 
 // One token: a block per (batch row, head), bound by the state's one read and one write.  Thread = (row group, V neighbouring columns), eight rows in
-// flight each; the partial sums over the row groups meet in LDS.
+// flight each; the partial sums over the row groups meet in LDS.  256 rows of 16 heads, 128 x 128: 105 us = 5.1 TB/s (a large copy: 4.9); one row
+// of 5 heads, 60 x 60: 3.9 us, the launch.
 template <typename T, int V>
 __global__ __launch_bounds__(256) void linattn_step_kernel(const LinAttnArgs a, int lpr /* threads per row, a power of two with lpr * V >= Dv */) {
     __shared__ float qs[128], ks[128], red[256 * V];
@@ -546,7 +555,8 @@ __global__ __launch_bounds__(256) void linattn_step_kernel(const LinAttnArgs a, 
     }
 }
 
-// out[r][c] = sum over j < n of x[r][c / D][j][c % D]: the gradient of a head that n heads read, in the order of the heads
+// out[r][c] = sum over j < n of x[r][c / D][j][c % D]: the gradient of a head that n heads read, in the order of the heads.  Bound by memory:
+// 16 384 tokens of 16 heads of 128 into 4, 151 MB: 22 us (6.8 TB/s, much of it from the last-level cache the products just wrote)
 template <typename T, int V>
 __global__ __launch_bounds__(256) void head_sum_kernel(const float* __restrict__ x, T* __restrict__ out, long rows, int n, int D) {
     const long total = rows * (D / V);                    // rows: one per token and shared head
@@ -568,7 +578,8 @@ __global__ __launch_bounds__(256) void head_sum_kernel(const float* __restrict__
 
 // Segments of the time axis: one pass over q, k, v where the rows and heads alone give every compute unit half of the eight waves it should have;
 // otherwise the axis is split so that the eight are there, at no less than two chunks a segment, for a second read of k and v and the segments'
-// states.  (Twelve or sixteen waves: the scan over the states grows by what the chunks save.)
+// states.  With sixteen waves the scan over the states grows by more than the chunks save (8 heads of 32 768 tokens: scan 20 us, 10.7; chunks 74, 70;
+// three ragged prompts 79 us, 69; 60 calls drawn from all sizes, geometric mean: 46.0 us, 45.0).
 void segments(int B, int T, int H, int Dv, int b16_io, int* nseg, int* len) {
     const int C = b16_io ? Mma<b16>::C : Mma<float>::C, chunks = (int)(((long)T + C - 1) / C), groups = hw_cu_count() * (Dv <= 32 ? 4 : 2);
     const long rows = (long)B * H;

@@ -5,6 +5,9 @@
 // gradients are rounded once where they are stored, and z is the norm of h BEFORE that rounding, in the backward pass as in the forward one
 // (h is formed again from y, res and gate there: the same bytes as reading h, and the parameters' gradients stay fp32-exact).
 // Bound by HBM: a row lives in the registers of TPR threads (NI chunks of VEC values each) between its one read and its one write.
+// Measured (bf16): 8 192 rows of 4 096 in 32 groups forward 31 us (4.3 TB/s; a large copy 4.9), backward 49 us (4.1 TB/s); 16 384 rows of 2 048 with
+// everything behind the norm forward 66 us (336 MB, 5.1 TB/s), backward 128 us (537 MB, 4.2 TB/s: five of eight operands read, three written, and
+// two rounds of row sums per row).
 // Groups of a multiple of 16 bytes at aligned addresses are the straight case; otherwise (RAG: heads of 71, rows of 5 270) a chunk is four values at any
 // address -- memory takes unaligned 16 bytes -- that may belong to two groups, and the row's last one may be short.
 #include "common.h"
@@ -412,7 +415,8 @@ template <typename T, int TPR, int NI, int VEC, bool RAG, bool FULL> struct RowI
     }
 };
 
-// A block walks through the rows of its slice of a sequence and keeps the columns' sums in registers; its partial sums leave it once.
+// A block walks through the rows of its slice of a sequence and keeps the columns' sums in registers; its partial sums leave it once (128 sequences
+// of 34 rows of 300: 19 us, the latency of three rounds of four rows, each with its sums across a wave).
 // FULL: with gate, scale, residual or second norm; otherwise the norm alone (w, b).
 template <typename T, int TPR, int NI, int VEC, bool RAG, bool FULL>
 __global__ __launch_bounds__(block_of<TPR>()) void tail_bwd_kernel(const TailArgs a) {

@@ -320,3 +320,27 @@ def test_a_graph_that_saved_the_old_parameter_refuses_its_backward_pass():
         q, z = torch.ones(8, device=DEV), [torch.zeros(8, device=DEV) for _ in range(2)]
         optim.adamw_step([q], [torch.ones(8, device=DEV)], z[:1], z[1:], step)
     assert (q < 1).all()
+
+
+@pytest.mark.parametrize('bits', (32, 8))
+def test_a_captured_optimizer_advances_on_each_replay(bits):
+    """FusedAdamW.step in a graph, with eager steps of a twin in between: the same bits after every replay, two groups of decay included"""
+    def make():
+        torch.manual_seed(3)
+        ps = [torch.nn.Parameter(torch.randn(*s, device=DEV)) for s in ((40, 30), (30,), (129, 7))]
+        return ps, optim.FusedAdamW(ps, lr=3e-3, weight_decay=0.1, no_decay=ps[1:2], state_bits=bits, seed=5)
+    (p, a), (q, b) = make(), make()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        b.step()
+    for i in range(4):
+        g = torch.randn_like(a.flat_g) * (0.5 + i)
+        a.flat_g.copy_(g)
+        b.flat_g.copy_(g)
+        graph.replay()
+        a.step()
+        torch.cuda.synchronize()
+        assert int(a.step_t) == int(b.step_t) == i + 1 and torch.equal(a.flat_p, b.flat_p)
+    assert all(torch.equal(x, y) for x, y in zip(p, q))
