@@ -23,6 +23,7 @@ struct TailArgs {
     const void *dh, *dz;
     void *dy, *dres, *dgate;
     float *part;                     // [blocks][nvec][C] sums over a block's rows: w, b, then s, then w2, b2
+    float *rowsum;                   // [rows][2] the second norm's sums over a row (wide rows)
     float *gpart;                    // [outer][slices][C] sums of the gate's gradient over the slice's rows (gate shared by a sequence's rows)
     long inner;                      // rows of a sequence (= all rows where the gate is per row)
     int outer, C, G, layer, act, gate_shared;
@@ -416,7 +417,7 @@ template <typename T, int TPR, int NI, int VEC, bool RAG, bool FULL> struct RowI
 };
 
 // A block walks through the rows of its slice of a sequence and keeps the columns' sums in registers; its partial sums leave it once (128 sequences
-// of 34 rows of 300: 19 us, the latency of three rounds of four rows, each with its sums across a wave).
+// of 34 rows of 300: 18 us, the latency of five rounds of two rows, each with its sums across two waves).
 // FULL: with gate, scale, residual or second norm; otherwise the norm alone (w, b).
 template <typename T, int TPR, int NI, int VEC, bool RAG, bool FULL>
 __global__ __launch_bounds__(block_of<TPR>()) void tail_bwd_kernel(const TailArgs a) {
@@ -424,10 +425,10 @@ __global__ __launch_bounds__(block_of<TPR>()) void tail_bwd_kernel(const TailArg
     typedef RowSum<TPR, NI, VEC, RAG> Sum;
     constexpr int COLS = RPB > 1 ? RPB * TPR * NI * VEC : 1;
     __shared__ __attribute__((aligned(16))) float lds[RPB * Sum::PLACES > COLS ? RPB * Sum::PLACES : COLS];
-    __shared__ float meet[2][2 * (TPR / 64)];
+    __shared__ float meet[RPB][2][2 * (TPR / 64)];
     const int sub = threadIdx.x / TPR, lane = threadIdx.x % TPR, nch = (a.C + VEC - 1) / VEC;
     float* const mine = lds + sub * Sum::PLACES;
-    Sum gsum{mine, meet[0], lane, a.G, a.C / a.G, nch, 0}, rsum{mine, meet[1], lane, 1, a.C, nch, 0};
+    Sum gsum{mine, meet[sub][0], lane, a.G, a.C / a.G, nch, 0}, rsum{mine, meet[sub][1], lane, 1, a.C, nch, 0};
     Place<TPR, NI, VEC, RAG> pl;
     pl.init(a, lane);
     const bool whole = a.G == 1;
@@ -606,6 +607,284 @@ __global__ __launch_bounds__(block_of<TPR>()) void tail_bwd_kernel(const TailArg
     }
 }
 
+// What a chunk of a row is computed from
+template <typename T, int VEC, bool RAG, bool FULL> struct ChunkIn {
+    static constexpr int PARTS = RAG ? 2 : 1, V2 = FULL ? VEC : 1;
+    Raw<T, VEC> y, dh;
+    Raw<T, V2> dz, gate, res;
+    float mu[PARTS], rs[PARTS];
+    // the chunk at column c, of which n values exist, k of them in group g; row and gat (the gate's row) are the same for a whole wave
+    __device__ __forceinline__ void load(const TailArgs& a, long row, long gat, unsigned c, unsigned g, int n, int k, bool in) {
+        fill<PARTS>(mu, 0.f);
+        fill<PARTS>(rs, 0.f);
+        if (!in) return;
+        const long at = row * a.C;
+        y = load_raw<T, VEC>((const T*)a.y + at, c, n);
+        if (a.dh) dh = load_raw<T, VEC>((const T*)a.dh + at, c, n);
+        if (a.w) {
+            const float *rsp = a.rs + row * a.G, *mup = a.mu + row * a.G;
+#pragma unroll
+            for (int q = 0; q < PARTS; ++q)
+                if (q == 0 || k < n) {
+                    rs[q] = rsp[g + q];
+                    if (a.layer) mu[q] = mup[g + q];
+                }
+        }
+        if constexpr (FULL) {
+            if (a.dz) dz = load_raw<T, VEC>((const T*)a.dz + at, c, n);
+            if (a.gate) gate = load_raw<T, VEC>((const T*)a.gate + gat, c, n);
+            if (a.res && a.w2) res = load_raw<T, VEC>((const T*)a.res + at, c, n);
+        }
+    }
+};
+
+// One chunk on its way back.  open(): x^, n, the gate's activation and derivative, and with a second norm h^ and dz.  back(): d = the whole gradient
+// of h -> that of x^, what it adds to the columns' sums (w, b, s, w2, b2, gate), and the gradients of
+// residual and gate at their places (nullptr = not wanted).
+template <typename T, int VEC, bool RAG, bool FULL> struct Chunk {
+    static constexpr int V2 = FULL ? VEC : 1, PARTS = RAG ? 2 : 1;
+    float xh[VEC], n[V2], ga[V2], gd[V2], hh[V2], e[V2];
+    template <int NI> __device__ __forceinline__ void open(const TailArgs& a, const ChunkIn<T, VEC, RAG, FULL>& in, const Columns<NI, VEC>& col, int have,
+                                                           int k, float mu2, float rs2, bool there) {      // zeros where there is nothing
+        fill<VEC>(xh, 0.f);
+        if constexpr (FULL) { fill<VEC>(n, 0.f); fill<VEC>(ga, 1.f); fill<VEC>(gd, 0.f); fill<VEC>(hh, 0.f); fill<VEC>(e, 0.f); }
+        if (!there) return;
+        unpack<VEC>(in.y, xh);
+        if (a.w) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) xh[j] = (xh[j] - pick<RAG>(in.mu, j, k)) * pick<RAG>(in.rs, j, k);
+        }
+        if constexpr (FULL) {
+            float t[VEC];
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) n[j] = a.w ? xh[j] * col.w[j] + col.b[j] : xh[j];
+            if (a.gate) {
+                unpack<VEC>(in.gate, t);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) gate_act(t[j], a.act, ga[j], gd[j]);
+            }
+            if (a.w2) {
+                fill<VEC>(t, 0.f);
+                if (a.res) unpack<VEC>(in.res, t);
+                if (a.dz) unpack<VEC>(in.dz, e);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    float h = n[j] * ga[j];
+                    if (a.s) h *= col.s[j];
+                    if (a.res) h = a.alpha * t[j] + h;
+                    hh[j] = j < have ? (h - mu2) * rs2 : 0.f;
+                }
+            }
+        }
+    }
+    // what the second norm's gradient needs of the whole row
+    template <int NI> __device__ __forceinline__ void second(const Columns<NI, VEC>& col, float& s1, float& s2) const {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            const float t = e[j] * col.w2[j];
+            s1 += t * hh[j];
+            s2 += t;
+        }
+    }
+    template <int NI, int NA> __device__ __forceinline__ void back(const TailArgs& a, const ChunkIn<T, VEC, RAG, FULL>& in, const Columns<NI, VEC>& col, int have,
+                                                                   float rs2, float s1, float s2, float (&d)[VEC], float (&acc)[NA][VEC], T* dres,
+                                                                   T* dgate) const {
+        constexpr bool SUMS = NA > 1;
+        fill<VEC>(d, 0.f);
+        if (a.dh) unpack<VEC>(in.dh, d);
+        if constexpr (FULL)
+            if (a.w2) {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    if constexpr (SUMS) { acc[3][j] += e[j] * hh[j]; acc[4][j] += e[j]; }
+                    d[j] += rs2 * (e[j] * col.w2[j] - hh[j] * s1 - s2);
+                }
+            }
+        if constexpr (RAG)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j)
+                if (j >= have) d[j] = 0.f;
+        if constexpr (FULL) {
+            float t[VEC];
+            if (dres) {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) t[j] = a.alpha * d[j];
+                store_row<VEC>(dres, 0, t, have);
+            }
+            if (a.s) {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    if constexpr (SUMS) acc[2][j] += d[j] * (n[j] * ga[j]);
+                    d[j] *= col.s[j];
+                }
+            }
+            if (a.gate) {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    t[j] = d[j] * n[j] * gd[j];
+                    if constexpr (SUMS) acc[5][j] += t[j];
+                    d[j] *= ga[j];
+                }
+                if (dgate) store_row<VEC>(dgate, 0, t, have);
+            }
+        }
+        if (a.w) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                if constexpr (SUMS) { acc[0][j] += d[j] * xh[j]; acc[1][j] += d[j]; }
+                d[j] *= col.w[j];
+            }
+        }
+    }
+};
+
+// Rows of more than a chunk for each of 1 024 threads, whose 128 registers do not hold the columns' sums as well: two kernels.  This one takes the rows:
+// the chunks are opened one by one, once for the sums of the second norm, from the caches again for the rest; only x^ and its gradient are kept.
+// The row's two sums go to memory for the other.  Two chunks' operands are kept in registers, four are read again (16 384 values of bf16: 333 us, kept
+// and spilled 423).  8 192 values, 2^25 in all: bf16 199 us (2.7 TB/s), fp32 310 (3.5); bound by its one block per compute unit, whose loads, two
+// row sums and stores follow one another.
+template <typename T, int NI, bool RAG, bool FULL>
+__global__ __launch_bounds__(1024) void tail_wide_kernel(const TailArgs a) {
+    constexpr int TPR = 1024, VEC = 4;
+    constexpr bool KEEP = NI == 2;      // its operands stay in registers, loaded once
+    constexpr int KEPT = KEEP ? NI : 1;
+    typedef RowSum<TPR, NI, VEC, RAG> Sum;
+    __shared__ float lds[Sum::PLACES], meet[2][2 * (TPR / 64)];
+    const int lane = threadIdx.x, nch = (a.C + VEC - 1) / VEC;
+    Sum gsum{lds, meet[0], lane, a.G, a.C / a.G, nch, 0}, rsum{lds, meet[1], lane, 1, a.C, nch, 0};
+    Place<TPR, NI, VEC, RAG> pl;
+    pl.init(a, lane);
+    const bool whole = a.G == 1;
+    const long per = (a.inner + gridDim.x - 1) / gridDim.x, beg = (long)blockIdx.y * a.inner + blockIdx.x * per, end = (long)blockIdx.y * a.inner + min(a.inner, (blockIdx.x + 1) * per);
+    const float inv = (float)a.G / a.C, inv2 = 1.0f / a.C;
+    for (long row = beg; row < end; ++row) {
+        const long at = row * a.C;
+        float mu2 = 0.f, rs2 = 0.f, s1 = 0.f, s2 = 0.f, none[1][VEC];
+        Columns<NI, VEC> col;
+        ChunkIn<T, VEC, RAG, FULL> in[KEPT];
+        Chunk<T, VEC, RAG, FULL> ch;
+        auto load = [&](int i) {
+            const int c = lane + i * TPR;
+            in[KEEP ? i : 0].load(a, row, a.gate_shared ? (long)blockIdx.y * a.C : at, c * VEC, pl.g[i], pl.n(i), pl.k(i), c < nch);
+        };
+        auto open = [&](int i) {
+            const int c = lane + i * TPR;
+            __builtin_amdgcn_sched_barrier(0);                  // one chunk after another: the registers hold one
+            if (c < nch) col.load(a, (long)c * VEC, true, pl.n(i));
+            if constexpr (!KEEP) load(i);
+            ch.open(a, in[KEEP ? i : 0], col, pl.n(i), pl.k(i), mu2, rs2, c < nch);
+        };
+        if constexpr (KEEP)
+#pragma unroll
+            for (int i = 0; i < NI; ++i) load(i);
+        if constexpr (FULL)
+            if (a.w2) {
+                rs2 = a.rs2[row];
+                if (a.layer) mu2 = a.mu2[row];
+#pragma unroll
+                for (int i = 0; i < NI; ++i) {
+                    open(i);
+                    if (lane + i * TPR < nch) ch.second(col, s1, s2);
+                }
+                s1 = rsum.all(s1) * inv2;
+                s2 = a.layer ? rsum.all(s2) * inv2 : 0.f;
+                if (lane == 0) { a.rowsum[2 * row] = s1; a.rowsum[2 * row + 1] = s2; }
+            }
+        float d[NI][VEC], xh[NI][VEC], p1[NI][Sum::PARTS], p2[NI][Sum::PARTS];
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            const int c = lane + i * TPR;
+            fill<Sum::PARTS>(p1[i], 0.f);
+            fill<Sum::PARTS>(p2[i], 0.f);
+            fill<VEC>(d[i], 0.f);
+            open(i);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) xh[i][j] = ch.xh[j];
+            if (c >= nch) continue;
+            ch.back(a, in[KEEP ? i : 0], col, pl.n(i), rs2, s1, s2, d[i], none, FULL && a.dres ? (T*)a.dres + at + c * VEC : nullptr,
+                    FULL && a.dgate && !a.gate_shared ? (T*)a.dgate + at + c * VEC : nullptr);
+            if (a.w) {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    add_to<RAG>(p1[i], j, pl.k(i), whole, d[i][j] * xh[i][j]);
+                    add_to<RAG>(p2[i], j, pl.k(i), whole, d[i][j]);
+                }
+            }
+        }
+        if (a.w) {
+            float c1[NI][Sum::PARTS], c2[NI][Sum::PARTS];
+            gsum.groups(pl, p1, c1);
+            if (a.layer) gsum.groups(pl, p2, c2);
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+                float rs[Sum::PARTS];
+#pragma unroll
+                for (int q = 0; q < Sum::PARTS; ++q) rs[q] = lane + i * TPR < nch && (q == 0 || pl.k(i) < pl.n(i)) ? a.rs[row * a.G + pl.g[i] + q] : 0.f;
+#pragma unroll
+                for (int j = 0; j < VEC; ++j)
+                    d[i][j] = pick<RAG>(rs, j, pl.k(i)) * (d[i][j] - xh[i][j] * (pick<RAG>(c1[i], j, pl.k(i)) * inv) - (a.layer ? pick<RAG>(c2[i], j, pl.k(i)) * inv : 0.f));
+            }
+        }
+        if (a.dy) {
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+                const int c = lane + i * TPR;
+                if (c < nch) store_row<VEC>((T*)a.dy, at + (long)c * VEC, d[i], pl.n(i));
+            }
+        }
+    }
+}
+
+// The columns' sums of wide rows: a block has 256 columns (four per lane) of a slice of a sequence's rows, which its four waves take in turn; the row
+// sums are there already, so that nothing is shared until the end.  Bound by memory, five operands a second time: 8 192 values, 2^25 in all: bf16
+// 75 us (4.5 TB/s), fp32 140 (4.8).
+template <typename T, bool RAG>
+__global__ __launch_bounds__(256) void tail_columns_kernel(const TailArgs a) {
+    __shared__ __attribute__((aligned(16))) float lds[4 * 256];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, c0 = blockIdx.x * 256, c = c0 + 4 * lane, D = a.C / a.G, g = c / D;
+    const int n = RAG ? max(0, min(4, a.C - c)) : 4, k = RAG ? min(4, (g + 1) * D - c) : 4;
+    const bool there = c < a.C;
+    const long per = (a.inner + gridDim.y - 1) / gridDim.y, beg = blockIdx.y * per, end = min(a.inner, beg + per), row0 = (long)blockIdx.z * a.inner;
+    float acc[6][4];
+#pragma unroll
+    for (int q = 0; q < 6; ++q) fill<4>(acc[q], 0.f);
+    Columns<1, 4> col;
+    col.load(a, c, there, n);
+    for (long q = beg + wave; q < end; q += 4) {
+        const long row = row0 + q;
+        ChunkIn<T, 4, RAG, true> in;
+        in.load(a, row, a.gate_shared ? (long)blockIdx.z * a.C : row * a.C, c, g, n, k, there);
+        float mu2 = 0.f, rs2 = 0.f, s1 = 0.f, s2 = 0.f;
+        if (a.w2) {
+            rs2 = a.rs2[row];
+            if (a.layer) mu2 = a.mu2[row];
+            s1 = a.rowsum[2 * row];
+            s2 = a.rowsum[2 * row + 1];
+        }
+        Chunk<T, 4, RAG, true> ch;
+        ch.open(a, in, col, n, k, mu2, rs2, there);
+        if (!there) continue;
+        float d[4];
+        ch.back(a, in, col, n, rs2, s1, s2, d, acc, (T*)nullptr, (T*)nullptr);
+    }
+    const bool have[6] = {a.w != nullptr, a.w != nullptr, a.s != nullptr, a.w2 != nullptr, a.w2 != nullptr, a.gate_shared && a.gpart};
+    const long blk = (long)blockIdx.z * gridDim.y + blockIdx.y;
+    int nvec = 0, at = 0;
+#pragma unroll
+    for (int q = 0; q < 5; ++q) nvec += have[q];
+#pragma unroll
+    for (int q = 0; q < 6; ++q) {
+        if (!have[q]) continue;
+        float* out = (q == 5 ? a.gpart + blk * a.C : a.part + (blk * nvec + at) * a.C) + c0;
+        ++at;
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 4; ++j) lds[wave * 256 + 4 * lane + j] = acc[q][j];
+        __syncthreads();
+        if (c0 + (int)threadIdx.x < a.C) out[threadIdx.x] = lds[threadIdx.x] + lds[256 + threadIdx.x] + lds[512 + threadIdx.x] + lds[768 + threadIdx.x];
+    }
+}
+
 // out[o][c] = sum over p of x[o][p][c], p in ascending order within each of 16 interleaved runs, in double
 template <typename T>
 __global__ __launch_bounds__(1024) void slab_sum_kernel(const float* __restrict__ x, T* __restrict__ out, int n, int C) {
@@ -669,22 +948,67 @@ template <typename T> void tail_fwd_launch(const TailArgs& a, int vec, bool rag,
     TAIL_VECS(FWD_CASE)
 #undef FWD_CASE
 }
+// The backward pass.  With anything behind the norm a value costs some 25 registers, so a thread has one chunk of the row while 256 threads hold it, 512
+// with chunks of eight or ragged ones, and two chunks of four beyond.  Measured on 2^25 values, us, the other choice behind it: bf16 1 024 values
+// per row 136 (two chunks of eight in a wave: 211), 4 096 171 (two in 256 threads: 235; one of four in 1 024: 273); fp32 2 048 256 (one in 512
+// threads: 268), 4 096 268 (one in 1 024: 426); ragged fp32 1 500 368 (two in 256: 550), 2 700 404 (one in 1 024: 436).
+// Rows beyond 4 096 values, and the norm alone beyond 2 048 chunks, go to tail_wide_kernel and tail_columns_kernel: bf16 8 192 values 273 us (two chunks
+// of eight in 1 024 threads, spilling: 392), 16 384 333 (1 020); fp32 8 192 443 (840), 16 384 581 (1 307), the norm alone there 124 (208).
+bool tail_full(const TailArgs& a) { return a.dres || a.gate || a.s || a.w2 || !a.w; }
+bool tail_wide(int C, int vec, bool full) { return vec > 1 && C > (full ? 4096 : 2048 * vec); }
+
+template <typename T, bool RAG, bool FULL> void tail_wide_launch(const TailArgs& a, int slices, hipStream_t st) {
+    const long want = (2L * hw_cu_count() + a.outer - 1) / a.outer;
+    const dim3 grid((unsigned)(want < a.inner ? want : a.inner), a.outer), block(1024);
+    if (a.C <= 8192) hipLaunchKernelGGL((tail_wide_kernel<T, 2, RAG, FULL>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((tail_wide_kernel<T, 4, RAG, FULL>), grid, block, 0, st, a);
+    if (a.w || a.s || a.w2 || (a.gate && a.gate_shared))
+        hipLaunchKernelGGL((tail_columns_kernel<T, RAG>), dim3((a.C + 255) / 256, slices, a.outer), dim3(256), 0, st, a);
+}
+template <typename T, int TPR, int NI, int VEC, bool RAG, bool FULL> void tail_one_launch(const TailArgs& a, int slices, hipStream_t st) {
+    hipLaunchKernelGGL((tail_bwd_kernel<T, TPR, NI, VEC, RAG, FULL>), dim3(slices, a.outer), dim3(block_of<TPR>()), 0, st, a);
+}
+template <typename T, int VEC, bool RAG> void tail_full_launch(const TailArgs& a, int slices, hipStream_t st) {
+    const int nch = (a.C + VEC - 1) / VEC;
+    if (nch <= 64) tail_one_launch<T, 64, 1, VEC, RAG, true>(a, slices, st);
+    else if (nch <= 128) tail_one_launch<T, 128, 1, VEC, RAG, true>(a, slices, st);
+    else if (nch <= 256) tail_one_launch<T, 256, 1, VEC, RAG, true>(a, slices, st);
+    else if constexpr (VEC == 8) tail_one_launch<T, 512, 1, VEC, RAG, true>(a, slices, st);
+    else if (RAG && nch <= 512) tail_one_launch<T, 512, 1, VEC, RAG, true>(a, slices, st);
+    else if (nch <= 512) tail_one_launch<T, 256, 2, VEC, RAG, true>(a, slices, st);
+    else tail_one_launch<T, 512, 2, VEC, RAG, true>(a, slices, st);
+}
+template <typename T, int VEC, bool RAG> void tail_norm_launch(const TailArgs& a, int slices, hipStream_t st) {
+    const int nch = (a.C + VEC - 1) / VEC;
+    if (nch <= 64) tail_one_launch<T, 64, 1, VEC, RAG, false>(a, slices, st);
+    else if (nch <= 128) tail_one_launch<T, 64, 2, VEC, RAG, false>(a, slices, st);
+    else if (nch <= 256) tail_one_launch<T, 256, 1, VEC, RAG, false>(a, slices, st);
+    else if (nch <= 512) tail_one_launch<T, 256, 2, VEC, RAG, false>(a, slices, st);
+    else if (nch <= 1024) tail_one_launch<T, 512, 2, VEC, RAG, false>(a, slices, st);
+    else tail_one_launch<T, 1024, 2, VEC, RAG, false>(a, slices, st);
+}
+template <typename T, bool FULL> void tail_ones_launch(const TailArgs& a, int slices, hipStream_t st) {
+    if (a.C <= 1024) tail_one_launch<T, 256, 4, 1, false, FULL>(a, slices, st);
+    else tail_one_launch<T, 1024, 16, 1, false, FULL>(a, slices, st);
+}
 template <typename T> void tail_bwd_launch(const TailArgs& a, int vec, bool rag, int slices, hipStream_t st) {
-    const bool full = a.dres || a.gate || a.s || a.w2 || !a.w;
-#define BWD_CASE(TPR, NI, VEC, RAG)                                                                                                             \
-    {                                                                                                                                           \
-        if (full) hipLaunchKernelGGL((tail_bwd_kernel<T, TPR, NI, VEC, RAG, true>), dim3(slices, a.outer), dim3(block_of<TPR>()), 0, st, a);    \
-        else hipLaunchKernelGGL((tail_bwd_kernel<T, TPR, NI, VEC, RAG, false>), dim3(slices, a.outer), dim3(block_of<TPR>()), 0, st, a);        \
+    const bool full = tail_full(a), wide = tail_wide(a.C, vec, full);
+    if (vec == 1) { if (full) tail_ones_launch<T, true>(a, slices, st); else tail_ones_launch<T, false>(a, slices, st); }
+    else if (wide && rag) { if (full) tail_wide_launch<T, true, true>(a, slices, st); else tail_wide_launch<T, true, false>(a, slices, st); }
+    else if (wide) { if (full) tail_wide_launch<T, false, true>(a, slices, st); else tail_wide_launch<T, false, false>(a, slices, st); }
+    else if (rag) { if (full) tail_full_launch<T, 4, true>(a, slices, st); else tail_norm_launch<T, 4, true>(a, slices, st); }
+    else {
+        if constexpr (sizeof(T) == 2)
+            if (vec == 8) return full ? tail_full_launch<T, 8, false>(a, slices, st) : tail_norm_launch<T, 8, false>(a, slices, st);
+        if (full) tail_full_launch<T, 4, false>(a, slices, st); else tail_norm_launch<T, 4, false>(a, slices, st);
     }
-    TAIL_VECS(BWD_CASE)
-#undef BWD_CASE
 }
 
 // values per access (16 bytes' worth, bf16 also 8; 1 for groups of one or two values), and whether chunks may straddle groups or end short
-int tail_vec(const TailArgs& a, int b16_io, bool* rag) {
-    const int D = a.C / a.G;
+int tail_vec(int C, int G, int b16_io, bool* rag) {
+    const int D = C / G;
     *rag = false;
-    if (a.G > 1 && D < 3) return 1;
+    if (G > 1 && D < 3) return 1;
     if (b16_io && D % 8 == 0) return 8;
     *rag = D % 4 != 0;
     return 4;
@@ -701,12 +1025,18 @@ int tail_check(const char* what, const TailArgs& a) {
 
 extern "C" {
 
-// slices of a sequence's rows in the backward pass: ~2 blocks per compute unit over all sequences
-int ha2g_block_tail_slices(int outer, long inner, int C) {
-    if (outer < 1 || inner < 1) return 1;
-    const long rpb = C <= 512 ? 4 : 1;
-    long s = (2L * hw_cu_count() + outer - 1) / outer;
-    const long most = (inner + rpb - 1) / rpb;
+// slices of a sequence's rows in the backward pass: two blocks per compute unit over all sequences (one of 512 threads; four with 8-byte loads: bf16,
+// 1 000 values in two groups 145 us, 211), each at least one turn of its rows.  More of them only write more sums (fp32, 1 024 values: 232 us with two
+// blocks, 273 with four).
+int ha2g_block_tail_slices(int outer, long inner, int C, int G, int full, int b16_io) {
+    if (outer < 1 || inner < 1 || C < 1 || G < 1) return 1;
+    bool rag;
+    const int vec = tail_vec(C, G, b16_io, &rag);
+    long want = 2L * hw_cu_count(), rows = C <= 256 ? 4 : (C <= 512 ? 2 : 1);
+    if (tail_wide(C, vec, full != 0)) { want = 4L * hw_cu_count() / ((C + 255) / 256); rows = 16; }
+    else if (full && C > 2048) want = hw_cu_count();
+    else if (full && b16_io && vec == 4) want *= 2;              // 8-byte loads: more waves to have as much in flight
+    const long s = (want + outer - 1) / outer, most = (inner + rows - 1) / rows;
     return (int)(s < 1 ? 1 : (s < most ? s : most));
 }
 
@@ -721,7 +1051,7 @@ int ha2g_block_tail_fwd(const void* y, const void* res, const void* gate, const 
     if (outer == 0 || inner == 0) return 0;
     HA2G_REQUIRE(y && h && (!w2 || z) && (!layer || !rs || mu) && (!layer || !rs2 || mu2), "block_tail_fwd: null operand");
     bool rag;
-    const int vec = tail_vec(a, b16_io, &rag);
+    const int vec = tail_vec(C, G, b16_io, &rag);
     if (b16_io) tail_fwd_launch<b16>(a, vec, rag, (hipStream_t)stream);
     else tail_fwd_launch<float>(a, vec, rag, (hipStream_t)stream);
     HA2G_CHECK_LAUNCH("block_tail_fwd");
@@ -738,13 +1068,14 @@ int ha2g_block_tail_bwd(const void* y, const void* res, const void* gate, const 
     a.dh = dh; a.dz = dz; a.dy = dy; a.dres = dres; a.dgate = dgate; a.part = part; a.gpart = gpart;
     a.outer = outer; a.inner = inner; a.gate_shared = gate_shared; a.C = C; a.G = G; a.layer = layer; a.act = act; a.alpha = alpha; a.eps = eps;
     if (const int rc = tail_check("block_tail_bwd", a)) return rc;
-    HA2G_REQUIRE(slices >= 1 && slices <= 65535 * 8, "block_tail_bwd: %d slices", slices);
+    HA2G_REQUIRE(slices >= 1 && slices <= 65535, "block_tail_bwd: %d slices", slices);
     if (outer == 0 || inner == 0) return 0;
     const int nvec = (w ? 2 : 0) + (s ? 1 : 0) + (w2 ? 2 : 0);
+    a.rowsum = part + (long)slices * outer * nvec * C;
     HA2G_REQUIRE(y && (!w || rs) && (!w2 || rs2) && (!layer || !w || mu) && (!layer || !w2 || mu2) && (nvec == 0 || (part && dparams)) &&
                  (!(gate && gate_shared) || (gpart && dgate)), "block_tail_bwd: null operand");
     bool rag;
-    const int vec = tail_vec(a, b16_io, &rag);
+    const int vec = tail_vec(C, G, b16_io, &rag);
     const hipStream_t st = (hipStream_t)stream;
     if (b16_io) tail_bwd_launch<b16>(a, vec, rag, slices, st);
     else tail_bwd_launch<float>(a, vec, rag, slices, st);

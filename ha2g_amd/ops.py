@@ -2149,10 +2149,13 @@ class BlockTailFunction(torch.autograd.Function):
             dres = torch.empty_like(y) if need[1] else None
             dgate = torch.empty_like(gate) if gate is not None and (need[2] or shared) else None
             nvec = 2 * (w is not None) + (s is not None) + 2 * (w2 is not None)
-            n = lib.ha2g_block_tail_slices(outer, inner, C)
+            bf = y.dtype == torch.bfloat16
+            full = dres is not None or gate is not None or s is not None or w2 is not None or w is None
+            n = lib.ha2g_block_tail_slices(outer, inner, C, groups, full, bf)
             slabs = n * outer * C
+            sums = (slabs * nvec + (2 * rows if w2 is not None else 0) + 3) // 4 * 4
             dp = torch.empty(nvec * C, dtype=torch.float32, device=dev)
-            ws = torch.empty(slabs * (nvec + shared) + 4, dtype=torch.float32, device=dev)
+            ws = torch.empty(sums + slabs * shared, dtype=torch.float32, device=dev)
             part = ws.data_ptr()
             mu, rs, mu2, rs2 = _tail_stats(st, rows * groups if w is not None else 0, rows if w2 is not None else 0, layer) if st is not None else (0, 0, 0, 0)
             if rows == 0:                # no rows: the sums over them are zero
@@ -2160,8 +2163,8 @@ class BlockTailFunction(torch.autograd.Function):
                 if dgate is not None:
                     dgate.zero_()
             check(lib.ha2g_block_tail_bwd(y.data_ptr(), _p(res), _p(gate), _p(w), _p(b), _p(s), _p(w2), _p(b2), mu, rs, mu2, rs2, _p(dh), _p(dz), _p(dy),
-                                          _p(dres), _p(dgate), part, part + 4 * ((slabs * nvec + 3) // 4 * 4) if shared else 0, dp.data_ptr(), n, outer, inner,
-                                          shared, C, groups, layer, act, alpha, eps, y.dtype == torch.bfloat16, _stream()))
+                                          _p(dres), _p(dgate), part, part + 4 * sums if shared else 0, dp.data_ptr(), n, outer, inner,
+                                          shared, C, groups, layer, act, alpha, eps, bf, _stream()))
             grads, at = [None] * 5, 0
             for i, (t, there) in enumerate(((w, w), (b, w), (s, s), (w2, w2), (b2, w2))):
                 if there is not None:

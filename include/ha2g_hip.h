@@ -600,9 +600,9 @@ int ha2g_head_sum(const float* x, void* out, long rows, int heads, int n, int D,
  * no z).  rows = outer * inner; gate_shared: one gate row per `inner` rows.  act: 0 none, 3 sigmoid, 4 SiLU.  mu, rs [rows * G], mu2, rs2 [rows]:
  * kept for the backward pass (NULL = not kept; mu, mu2 only for layer).  C <= 16384.
  * bwd: dh, dz (NULL = zero) -> dy, dres, dgate (NULL = not wanted; with gate_shared required), and dparams = [dw][db][ds][dw2][db2] (those whose
- * weight is there; db with w, db2 with w2); part = slices * outer * (their number) * C floats, gpart = slices * outer * C (gate_shared), slices =
- * ha2g_block_tail_slices().  Every sum has a fixed order. */
-int ha2g_block_tail_slices(int outer, long inner, int C);
+ * weight is there; db with w, db2 with w2); part = slices * outer * (their number) * C floats and with w2 2 * outer * inner more, gpart = slices * outer *
+ * C (gate_shared), slices = ha2g_block_tail_slices(); full = anything but w and b is there or w is not.  Every sum has a fixed order. */
+int ha2g_block_tail_slices(int outer, long inner, int C, int G, int full, int b16_io);
 int ha2g_block_tail_fwd(const void* y, const void* res, const void* gate, const float* w, const float* b, const float* s, const float* w2, const float* b2,
                         void* h, void* z, float* mu, float* rs, float* mu2, float* rs2, int outer, long inner, int gate_shared, int C, int G, int layer,
                         int act, float alpha, float eps, int b16_io, void* stream);

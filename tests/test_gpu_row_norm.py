@@ -276,3 +276,25 @@ def test_a_second_derivative_is_refused():
     gy, = torch.autograd.grad(ops.row_norm(y, w).square().sum(), y, create_graph=True)
     with pytest.raises(RuntimeError, match='once_differentiable'):
         (gy.sum() + y.sum()).backward()
+
+
+@DTS
+@pytest.mark.parametrize('gate', ('token', 'sequence'))
+@pytest.mark.parametrize('C,G,kind', ((300, 2, 'layer'), (480, 4, 'rms'), (512, 1, 'rms'), (1000, 2, 'layer'), (1500, 2, 'rms'), (2000, 5, 'layer'), (2702, 2, 'rms'),
+                                      (4096, 1, 'layer'), (4097, 1, 'layer'), (4100, 2, 'rms'), (4104, 3, 'layer'), (8192, 64, 'rms'), (8196, 4, 'layer'),
+                                      (12001, 11, 'layer'), (16384, 1, 'rms')))
+def test_everything_behind_the_norm_at_each_width(C, G, kind, gate, dt):
+    check_all((2, 7, C), dt, kind=kind, G=G, parts=('w', 'b', 'res', 'scale', 'w2', 'b2'), gate=gate, alpha=0.7)
+
+
+@pytest.mark.parametrize('parts,gate,grads', ((('w',), None, ('dh',)), (('res',), None, ('dh',)), (('scale', 'res'), 'sequence', ('dh',)), (('w2', 'b2'), None, ('dz',)),
+                                              (('w2',), 'token', ('dh', 'dz')), (('w', 'b', 'w2'), None, ('dz',)), ((), 'sequence', ('dh',))))
+@pytest.mark.parametrize('C,G', ((4200, 2), (16383, 3)))
+def test_parts_of_wide_rows(C, G, parts, gate, grads):
+    check_all((3, 5, C), torch.float32, kind='layer', G=G, parts=parts, gate=gate, grads=grads)
+
+
+def test_wide_rows_of_many_slices():
+    """more rows than a turn of every block, in slices that end inside one: the sums over 2 x 333 rows, and a gate for each sequence"""
+    check_all((2, 333, 4098), torch.bfloat16, G=3, parts=('w', 'b', 'res', 'scale', 'w2', 'b2'), gate='sequence', odd=True)
+    check_all((1, 700, 8200), torch.float32, kind='layer', parts=('w', 'b', 'res', 'scale', 'w2', 'b2'), gate='token')
