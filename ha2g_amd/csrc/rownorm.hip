@@ -279,11 +279,11 @@ template <typename T, int TPR, int NI, int VEC, bool RAG>
 __global__ __launch_bounds__(block_of<TPR>()) void tail_fwd_kernel(const TailArgs a) {
     typedef RowSum<TPR, NI, VEC, RAG> Sum;
     constexpr int RPB = block_of<TPR>() / TPR;
-    __shared__ float lds[RPB * Sum::PLACES], meet[2][2 * (TPR / 64)];
+    __shared__ float lds[RPB * Sum::PLACES], meet[RPB][2][2 * (TPR / 64)];
     const int sub = threadIdx.x / TPR, lane = threadIdx.x % TPR, nch = (a.C + VEC - 1) / VEC;
     const long rows = a.inner * a.outer;
     float* const mine = lds + sub * Sum::PLACES;
-    Sum gsum{mine, meet[0], lane, a.G, a.C / a.G, nch, 0}, rsum{mine, meet[1], lane, 1, a.C, nch, 0};
+    Sum gsum{mine, meet[sub][0], lane, a.G, a.C / a.G, nch, 0}, rsum{mine, meet[sub][1], lane, 1, a.C, nch, 0};
     Place<TPR, NI, VEC, RAG> pl;
     pl.init(a, lane);
     Columns<NI, VEC> col;
@@ -911,15 +911,17 @@ __global__ __launch_bounds__(1024) void slab_sum_kernel(const float* __restrict_
     }
 }
 
-// Threads per row and chunks per thread: a wave alone up to 128 chunks, then one chunk per thread as far as 256 threads go, then two; the widest rows
-// take what the registers of 1 024 threads hold.  Groups of one or two values (VEC = 1) are taken one by one.
+// The forward pass: threads per row and chunks per thread.  A wave alone up to 128 chunks, then one chunk per thread as far as 256 threads go, then two; the
+// widest rows take what the registers of 1 024 threads hold.  Ragged chunks cost more registers: one per thread up to 512 threads (2^25 values,
+// fp32: 300 per row 199 us, 242 with two per thread; 1 500 145 us, 195; but 2 700 224 us with one in 1 024 threads, 219 with two in 512).  Groups
+// of one or two values (VEC = 1) are taken one by one.
 #define TAIL_SHAPES(VEC, RAG, CASE)                                                                                                                \
     {                                                                                                                                              \
         const int nch = (a.C + VEC - 1) / VEC;                                                                                                     \
         if (nch <= 64) CASE(64, 1, VEC, RAG)                                                                                                       \
-        else if (nch <= 128) CASE(64, 2, VEC, RAG)                                                                                                 \
+        else if (nch <= 128) CASE((RAG ? 128 : 64), (RAG ? 1 : 2), VEC, RAG)                                                                       \
         else if (nch <= 256) CASE(256, 1, VEC, RAG)                                                                                                \
-        else if (nch <= 512) CASE(256, 2, VEC, RAG)                                                                                                \
+        else if (nch <= 512) CASE((RAG ? 512 : 256), (RAG ? 1 : 2), VEC, RAG)                                                                      \
         else if (nch <= 1024) CASE(512, 2, VEC, RAG)                                                                                               \
         else if (nch <= 2048) CASE(1024, 2, VEC, RAG)                                                                                              \
         else CASE(1024, (VEC == 8 ? 2 : 4), VEC, RAG)                                                                                              \
