@@ -143,22 +143,25 @@ template <> struct Mma<b16> {
     }
 };
 
-// 16 bytes of a row, at any address, of which `left` elements exist; WHOLE: all or none
+// 16 bytes at any multiple of an element's size
 typedef u32x4_t u32x4_a2 __attribute__((aligned(2)));
 typedef unsigned u32x2_a2 __attribute__((ext_vector_type(2), aligned(2)));
-template <typename T, bool WHOLE> __device__ __forceinline__ u32x4_t load16(const T* p, int left) {
-    constexpr int E = 16 / sizeof(T);
+// a row of `left` elements, less than 16 bytes of them; zeros behind
+template <typename T> __device__ __forceinline__ u32x4_t load_short(const T* p, int left) {
     u32x4_t r = {0u, 0u, 0u, 0u};
-    if (WHOLE ? left > 0 : left >= E) r = *reinterpret_cast<const u32x4_a2*>(p);
-    else if constexpr (!WHOLE) {
-        if (left > 0)
 #pragma unroll
-            for (int j = 0; j < E - 1; ++j)
-                if (j < left) {
-                    if constexpr (sizeof(T) == 4) r[j] = __float_as_uint(p[j]);
-                    else r[j >> 1] |= (unsigned)p[j] << (16 * (j & 1));
-                }
-    }
+    for (int j = 0; j < (int)(16 / sizeof(T)) - 1; ++j)
+        if (j < left) {
+            if constexpr (sizeof(T) == 4) r[j] = __float_as_uint(p[j]);
+            else r[j >> 1] |= (unsigned)p[j] << (16 * (j & 1));
+        }
+    return r;
+}
+// 16 bytes shifted towards the front by n < 128 bits (a multiple of 16, the same for all lanes), zeros behind
+__device__ __forceinline__ u32x4_t shift_down(u32x4_t r, int n) {
+    if (n & 64) r = u32x4_t{r[2], r[3], 0u, 0u};
+    if (n & 32) r = u32x4_t{r[1], r[2], r[3], 0u};
+    if (n & 16) r = u32x4_t{r[0] >> 16 | r[1] << 16, r[1] >> 16 | r[2] << 16, r[2] >> 16 | r[3] << 16, r[3] >> 16};
     return r;
 }
 __device__ __forceinline__ void store4(float* p, const f32x4& v) { *reinterpret_cast<u32x4_a2*>(p) = __builtin_bit_cast(u32x4_t, v); }
@@ -170,7 +173,10 @@ __device__ __forceinline__ void store4(b16* p, const f32x4& v) {
     *reinterpret_cast<u32x2_a2*>(p) = w;
 }
 
-template <typename T, int D, int C, int NT, bool WHOLE> struct Stage {     // a chunk of one operand: registers on the way from memory to LDS
+// A chunk of one operand: registers on the way from memory to LDS.  WHOLE: rows of whole 16-byte pieces.  Otherwise a row's last piece is read as the
+// row's last 16 bytes and shifted on its way to LDS (512 pairs of 1 024 tokens in bf16, 60 x 60: 70 us, 123 element by element; 75 x 75 139, 255; in
+// fp32, where three elements at most are read one by one, 368 and 380).
+template <typename T, int D, int C, int NT, bool WHOLE> struct Stage {
     static constexpr int E = 16 / sizeof(T), V = D / E, N = C * V / NT, LD = D + Mma<T>::PADK, RS = NT / V;
     static_assert(N * NT == C * V && RS * V == NT, "a chunk is a whole number of pieces per thread, a pass over the threads whole rows");
     u32x4_t r[N];
@@ -178,27 +184,34 @@ template <typename T, int D, int C, int NT, bool WHOLE> struct Stage {     // a 
     const char* base;            // lowest row of the next chunk's first pass
     unsigned off;
     long pass, chunk;            // bytes from one row pass to the next, and from one chunk
-    int row, left;               // first row, elements of it from here on
+    int row, left, shift;        // first row, elements of it from here on; bits that a last piece moves by; -1: rows of less than 16 bytes
     // rows: token `first` and on in steps of `step` elements (negative from the end; less than 2^22)
     __device__ __forceinline__ void start(const T* first, long step, int dim) {
         row = threadIdx.x / V;
         const int c = threadIdx.x % V * E, low = step < 0 ? RS - 1 - row : row;
         left = dim - c;
         base = (const char*)(first + (step < 0 ? (RS - 1) * step : 0));
-        off = (unsigned)(low * (int)(step < 0 ? -step : step) + c) * sizeof(T);
+        shift = dim < E ? -1 : (E - dim % E) % E * 8 * (int)sizeof(T);
+        off = (unsigned)(low * (int)(step < 0 ? -step : step) + (WHOLE || shift < 0 ? c : min(c, dim - E))) * sizeof(T);
         pass = RS * step * (long)sizeof(T);
         chunk = C * step * (long)sizeof(T);
     }
     // the next chunk, of which n rows exist
     __device__ __forceinline__ void load(int n) {
 #pragma unroll
-        for (int j = 0; j < N; ++j) r[j] = load16<T, WHOLE>((const T*)(base + j * pass + off), row + j * RS < n ? left : 0);
+        for (int j = 0; j < N; ++j) {
+            const char* p = base + j * pass + off;
+            const int have = row + j * RS < n ? left : 0;
+            r[j] = u32x4_t{0u, 0u, 0u, 0u};
+            if (!WHOLE && shift < 0) r[j] = load_short<T>((const T*)p, have);
+            else if (have > 0) r[j] = *reinterpret_cast<const u32x4_a2*>(p);
+        }
         base += chunk;
     }
     __device__ __forceinline__ void store(T* lds) const {
         T* p = lds + threadIdx.x / V * LD + threadIdx.x % V * E;
 #pragma unroll
-        for (int j = 0; j < N; ++j) *reinterpret_cast<u32x4_t*>(p + j * RS * LD) = r[j];
+        for (int j = 0; j < N; ++j) *reinterpret_cast<u32x4_t*>(p + j * RS * LD) = !WHOLE && shift > 0 && left < E ? shift_down(r[j], shift) : r[j];
     }
 };
 

@@ -321,3 +321,19 @@ def test_more_rows_and_heads_than_a_grid_holds_are_refused():
         ops.linear_attention(x, x, x, g)
     with pytest.raises(RuntimeError, match=r'2\^32'):
         ops.linear_attention_step(x[:, 0], x[:, 0], x[:, 0], g, torch.zeros(1 << 16, 1 << 7, 1, 1, device=DEV))
+
+
+@pytest.mark.parametrize('dt', (torch.float32, torch.bfloat16), ids=('fp32', 'bf16'))
+@pytest.mark.parametrize('Dk,Dv', ((9, 10), (11, 13), (14, 15), (12, 7), (5, 3), (39, 66), (122, 109)))
+def test_rows_that_end_inside_a_piece(Dk, Dv, dt):
+    """every remainder of a row by 16 bytes, rows shorter than that, and what lies around the rows is not a number: it is not read, or not used"""
+    check_all(*make(2, 35, 2, 2, 1, 2, Dk, Dv, dt, seed=Dk))
+    q, k, v, g, state, _, _ = make(2, 35, 2, 2, 2, 2, Dk, Dv, dt, seed=Dk)
+
+    def inside(x):
+        wide = torch.full((*x.shape[:-1], x.shape[-1] + 2), float('nan'), dtype=x.dtype, device=x.device)
+        wide[..., 1:-1] = x
+        return wide[..., 1:-1]
+    a = ops.linear_attention(q.detach(), k.detach(), v.detach(), g, state=state.detach(), return_state=True)
+    b = ops.linear_attention(inside(q.detach()), inside(k.detach()), inside(v.detach()), g, state=state.detach(), return_state=True)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
