@@ -962,8 +962,10 @@ bool tail_wide(int C, int vec, bool full) { return vec > 1 && C > (full ? 4096 :
 template <typename T, bool RAG, bool FULL> void tail_wide_launch(const TailArgs& a, int slices, hipStream_t st) {
     const long want = (2L * hw_cu_count() + a.outer - 1) / a.outer;
     const dim3 grid((unsigned)(want < a.inner ? want : a.inner), a.outer), block(1024);
-    if (a.C <= 8192) hipLaunchKernelGGL((tail_wide_kernel<T, 2, RAG, FULL>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((tail_wide_kernel<T, 4, RAG, FULL>), grid, block, 0, st, a);
+    bool two = false;                                             // the norm alone comes here with more than 8 192 values only
+    if constexpr (FULL)
+        if ((two = a.C <= 8192)) hipLaunchKernelGGL((tail_wide_kernel<T, 2, RAG, FULL>), grid, block, 0, st, a);
+    if (!two) hipLaunchKernelGGL((tail_wide_kernel<T, 4, RAG, FULL>), grid, block, 0, st, a);
     if (a.w || a.s || a.w2 || (a.gate && a.gate_shared))
         hipLaunchKernelGGL((tail_columns_kernel<T, RAG>), dim3((a.C + 255) / 256, slices, a.outer), dim3(256), 0, st, a);
 }
