@@ -215,7 +215,8 @@ template <bool RAG, int PARTS> __device__ __forceinline__ void add_to(float (&p)
     else p[0] += v;
 }
 
-// x -> x^ in place; m / r: mean and 1 / std per chunk and part.  Values that do not exist are zeros and stay zeros.
+// x -> x^ in place; m / r: mean and 1 / std per chunk and part.  Values that do not exist are zeros and stay zeros: their r is 0, not the 1 / sqrt(eps)
+// of an empty sum, which is infinite for eps = 0.
 template <int TPR, int NI, int VEC, bool RAG>
 __device__ __forceinline__ void normalise(RowSum<TPR, NI, VEC, RAG>& rsum, const Place<TPR, NI, VEC, RAG>& pl, float (&x)[NI][VEC],
                                           float (&m)[NI][RowSum<TPR, NI, VEC, RAG>::PARTS], float (&r)[NI][RowSum<TPR, NI, VEC, RAG>::PARTS], bool layer,
@@ -251,8 +252,9 @@ __device__ __forceinline__ void normalise(RowSum<TPR, NI, VEC, RAG>& rsum, const
     rsum.groups(pl, p, r);
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
+        const bool in = rsum.lane + i * TPR < rsum.nch;
 #pragma unroll
-        for (int q = 0; q < PARTS; ++q) r[i][q] = 1.0f / sqrtf(r[i][q] * inv + eps);
+        for (int q = 0; q < PARTS; ++q) r[i][q] = in && (q == 0 || pl.k(i) < pl.n(i)) ? 1.0f / sqrtf(r[i][q] * inv + eps) : 0.f;
 #pragma unroll
         for (int j = 0; j < VEC; ++j) x[i][j] *= pick<RAG>(r[i], j, pl.k(i));
     }

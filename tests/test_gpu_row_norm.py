@@ -298,3 +298,12 @@ def test_wide_rows_of_many_slices():
     """more rows than a turn of every block, in slices that end inside one: the sums over 2 x 333 rows, and a gate for each sequence"""
     check_all((2, 333, 4098), torch.bfloat16, G=3, parts=('w', 'b', 'res', 'scale', 'w2', 'b2'), gate='sequence', odd=True)
     check_all((1, 700, 8200), torch.float32, kind='layer', parts=('w', 'b', 'res', 'scale', 'w2', 'b2'), gate='token')
+
+
+@DTS
+@pytest.mark.parametrize('kind', ('rms', 'layer'))
+@pytest.mark.parametrize('C,G', ((40, 2), (300, 5), (300, 2), (1000, 8), (1500, 2), (2000, 8), (2702, 2), (4200, 3), (9000, 4), (12, 6)))
+def test_without_an_eps(C, G, kind, dt, monkeypatch):
+    """eps = 0 on rows that have a scale of their own: places that a row does not fill reach neither the second norm nor a gradient"""
+    monkeypatch.setitem(globals(), 'EPS', 0.0)
+    check_all((2, 5, C), dt, kind=kind, G=G, parts=('w', 'b', 'res', 'scale', 'w2', 'b2'), gate='sequence', alpha=0.7, seed=C + G)
