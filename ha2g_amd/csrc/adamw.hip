@@ -5,7 +5,9 @@
 // blocks of 128 consecutive elements of a tensor hold m and r = sqrt(v) as e4m3 codes times one power of two each, the smallest that brings the
 // block's largest finite magnitude to at most 448.  r instead of v halves the range in octaves.  A code has 4 significant bits, so a round to
 // nearest would never let v decay by its 0.1 % a step: the part below a code rounds up with its own probability, by a dither that a counter hash
-// makes of (seed, t, tensor, place), the same on every run.  A value that is not finite keeps to its own element (the NaN code).
+// makes of (seed, t, tensor, place), the same on every run.  A root above zero keeps at least the smallest code: it divides the next update, and as
+// 0 beside an m that survived (m has a scale of its own) it would let that update be lr m / eps.  Such an element's v does not decay below some 2^-36
+// of its block's largest.  A value that is not finite keeps to its own element (the NaN code).
 #include "common.h"
 
 namespace {
@@ -190,7 +192,7 @@ __global__ __launch_bounds__(256) void adamw8_kernel(const AdamWTable tab, const
         for (int k = 0; k < 8; ++k) {
             const unsigned d = hash32(((unsigned)at + k) ^ place);
             cm[k >> 2] |= encode(M[k], im, (float)(d >> 16) * 0x1p-16f) << (8 * (k & 3));
-            cr[k >> 2] |= encode(R[k], ir, (float)(d & 0xffffu) * 0x1p-16f) << (8 * (k & 3));
+            cr[k >> 2] |= max(encode(R[k], ir, (float)(d & 0xffffu) * 0x1p-16f), R[k] > 0.f ? 1u : 0u) << (8 * (k & 3));
         }
         if (wide) {
 #pragma unroll

@@ -614,7 +614,7 @@ int ha2g_block_tail_bwd(const void* y, const void* res, const void* gate, const 
 /* ---- AdamW over many tensors in one launch (torch.optim.AdamW semantics; the reference sets up Adam, train.py:155-170) ----
  * p, g, m, v, sm, sr: HOST arrays of n device pointers; len: HOST array of n lengths.  p fp32 or (p_b16) bf16, g likewise.  bits = 32: m, v fp32.
  * bits = 8: m, v = e4m3 codes of m and of sqrt(v), sm / sr = fp32 scales (powers of two), one per 128 consecutive elements of a tensor; the rounding
- * to codes is dithered by a hash of (seed, step, first + tensor, place).  ha2g_adamw_scalars advances `step` (device int32; guard as in
+ * to codes is dithered by a hash of (seed, step, first + tensor, place); a root above zero is never rounded to zero.  ha2g_adamw_scalars advances `step` (device int32; guard as in
  * ha2g_adam_guarded_f32) and leaves what the step's number gives in `scalars` (3 words of device memory) for the calls of the step. */
 int ha2g_adamw_scalars(int* step, const int* guard, double lr, double b1, double b2, float* scalars, void* stream);
 int ha2g_adamw_multi(int n, const long* p, const long* g, const long* m, const long* v, const long* sm, const long* sr, const long* len, int p_b16,

@@ -344,3 +344,39 @@ def test_a_captured_optimizer_advances_on_each_replay(bits):
         torch.cuda.synchronize()
         assert int(a.step_t) == int(b.step_t) == i + 1 and torch.equal(a.flat_p, b.flat_p)
     assert all(torch.equal(x, y) for x, y in zip(p, q))
+
+
+def test_a_root_that_is_not_zero_is_not_stored_as_zero():
+    """A root far below its block's largest is held as the smallest code: it divides the next update.  A root of zero stays zero."""
+    n = 640
+    p, g = [torch.zeros(n, device=DEV)], [torch.full((n,), 1e-9, device=DEV)]
+    g[0][::128] = 1.0
+    g[0][1::128] = 0.0
+    m, v = [optim.adamw_state8(p[0])], [optim.adamw_state8(p[0])]
+    step = torch.zeros(1, dtype=torch.int32, device=DEV)
+    for _ in range(3):
+        optim.adamw_step(p, g, m, v, step, seed=11, **HP)
+        codes = v[0][0].view(torch.uint8).cpu().view(5, 128)
+        assert (codes[:, 1] == 0).all() and (codes[:, 0] > 100).all() and (codes[:, 2:] == 1).all()
+
+
+def test_small_gradients_beside_a_large_one_move_a_parameter_by_no_more_than_a_few_steps():
+    """One gradient of 1 and 127 of 1e-8 in each block, which vanish after 20 of 40 steps.  With b1 = 1/2: a code of m is off by at most an eighth of
+    its value and the smallest code step s, so a small m is held as at most (9/16 g + s) / (1 - 9/16) = 9/7 g + 16/7 s, s <= 2^-9 (2 / 448) (1 - b1^t)
+    (the scale is within a factor of 2 of the largest m / 448).  A root is at least sqrt(b2) times the smallest code, 2^-9 / 448 sqrt(1 - b2^t).  So
+    an update is at most lr (16/7 + 1.15 g / (1 - b1) / (2^-9 / 448)) / sqrt(b2) = 2.30 lr where the large element's m and root are exact; they are off
+    by their own codes, an eighth a step at most and without bias: 8 lr leaves a factor of three for them.  After the gradients have vanished m
+    falls faster than its root, and the bound stays."""
+    n, lr = 128 * 40, 1e-3
+    p = [torch.zeros(n, device=DEV)]
+    g = [torch.full((n,), 1e-8, device=DEV)]
+    g[0][::128] = 1.0
+    m, v = [optim.adamw_state8(p[0])], [optim.adamw_state8(p[0])]
+    step = torch.zeros(1, dtype=torch.int32, device=DEV)
+    small = torch.arange(n, device=DEV) % 128 != 0
+    for t in range(40):
+        if t == 20:
+            g[0].zero_()
+        old = p[0].clone()
+        optim.adamw_step(p, g, m, v, step, lr=lr, betas=(0.5, 0.999), weight_decay=0.0, seed=2)
+        assert float((p[0] - old)[small].abs().max()) <= 8 * lr, t
