@@ -149,7 +149,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9, 
     laid out like the parameters.  In 8 bits:
     pairs (codes, scales) as adamw_state8 makes them, exp_avg_sqs holding the ROOT of the second moment; `seed` (32 bits) varies the rounding's dither.
     A root above zero is held as at least the smallest code of its block (some 2^-18 of the largest root): it divides the next update.
-    No tensor appears twice.  guard: optional int32 device word; while it is not zero the step changes nothing.  Everything lies on one device."""
+    No two of the written tensors share memory (one listed twice is refused).  guard: optional int32 device word; while it is not zero the step changes nothing.  Everything lies on one device."""
     n = len(params)
     _need(n == len(grads) == len(exp_avgs) == len(exp_avg_sqs), 'adamw_step: %d parameters, %d gradients, %d and %d states', n, len(grads), len(exp_avgs),
           len(exp_avg_sqs))
@@ -178,8 +178,9 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9, 
         _adamw_check(params, grads, ms, vs, sm, sr, q8, dev, pt, gt, num)
     if n == 0:
         return
-    pp, pm, pv = _ptrs(params), _ptrs(ms), _ptrs(vs)
-    own = pp + pm + pv if 0 not in num else [x for t in (pp, pm, pv) for x, k in zip(t, num) if k]
+    pp, pm, pv, psm, psr = (_ptrs(ts) for ts in (params, ms, vs, sm, sr))
+    written = (pp, pm, pv, psm, psr) if q8 else (pp, pm, pv)
+    own = [x for t in written for x in t] if 0 not in num else [x for t in written for x, k in zip(t, num) if k]
     _need(len(set(own)) == len(own), 'adamw_step: a parameter or a state is listed twice')
     with _on(step):
         st, gp = _stream(), None if guard is None else guard.data_ptr()
@@ -187,7 +188,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9, 
         sp = sc.data_ptr()
         b1, b2, lr = float(betas[0]), float(betas[1]), float(lr)
         check(lib.ha2g_adamw_scalars(step.data_ptr(), gp, lr, b1, b2, sp, st))
-        check(lib.ha2g_adamw_multi(n, pp, _ptrs(grads), pm, pv, _ptrs(sm) if q8 else None, _ptrs(sr) if q8 else None, array.array('l', num),
+        check(lib.ha2g_adamw_multi(n, pp, _ptrs(grads), pm, pv, psm if q8 else None, psr if q8 else None, array.array('l', num),
                                    pt is torch.bfloat16, gt is torch.bfloat16, 8 if q8 else 32, lr, b1, b2, float(eps), float(weight_decay),
                                    int(seed) & 0xffffffff, 0, sp, gp, st))
     # a graph that saved a parameter's old value refuses its backward pass from here on

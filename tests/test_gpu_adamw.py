@@ -380,3 +380,13 @@ def test_small_gradients_beside_a_large_one_move_a_parameter_by_no_more_than_a_f
         old = p[0].clone()
         optim.adamw_step(p, g, m, v, step, lr=lr, betas=(0.5, 0.999), weight_decay=0.0, seed=2)
         assert float((p[0] - old)[small].abs().max()) <= 8 * lr, t
+
+
+def test_scales_listed_twice_are_refused():
+    p, g = [torch.zeros(200, device=DEV)], [torch.zeros(200, device=DEV)]
+    (mc, s), (vc, r) = optim.adamw_state8(p[0]), optim.adamw_state8(p[0])
+    step = torch.zeros(1, dtype=torch.int32, device=DEV)
+    with pytest.raises(ValueError, match='twice'):
+        optim.adamw_step(p, g, [(mc, s)], [(vc, s)], step)
+    assert int(step) == 0
+    optim.adamw_step(p, g, [(mc, s)], [(vc, r)], step)
