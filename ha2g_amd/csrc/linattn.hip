@@ -51,7 +51,8 @@ template <> __device__ __forceinline__ void st1<b16>(b16* p, long i, float v) {
 // instructions (200 of them split S, 64 decay it) beside 91 matrix instructions, matrix units 30 % busy.
 // fp32 operands run on the fp32 MFMA.  bf16 operands are exact as they are; what is computed is split into bf16 pieces: S and the scores, which
 // only reach the bf16 result, into two (2^-17), the decayed v that is added to S into three (all 24 bits: S stays fp32-exact).
-// The decay of S is S + S (e^{gC} - 1): a factor rounded to fp32 is off the same way in every chunk, 1e-4 of a state with a memory of 2^12 tokens.
+// The decay of S is S + S (e^{gC} - 1) where more than half is kept: a factor rounded to fp32 is off the same way in every chunk, 1e-4 of a state with a
+// memory of 2^12 tokens.  Where less is kept it is S e^{gC}: the sum is exact to 2^-24 of the S before, not of what is left of it.
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
 typedef short s16x8_t __attribute__((ext_vector_type(8)));
@@ -229,6 +230,17 @@ template <int N, int D, typename Load, typename Use> __device__ __forceinline__ 
 }
 
 __device__ __forceinline__ float decay_power(float g, int n) { return n == 0 ? 1.f : expf(g * (float)n); }
+// x e^{g n} as told in front of this file's chunked form; g and n are the same for all lanes, and so are the factor and the choice (in scalar registers)
+struct Decay {
+    float f;
+    int most;                    // of x is kept: f = e^{g n} - 1, otherwise f = e^{g n}
+    __device__ __forceinline__ Decay(float g, int n) {
+        const float e = g * (float)n;
+        most = __builtin_amdgcn_readfirstlane(e > -0.6931472f);
+        f = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(most ? expm1f(e) : expf(e))));
+    }
+    __device__ __forceinline__ float operator()(float x) const { return __builtin_fmaf(x, f, most ? x : 0.f); }
+};
 __device__ __forceinline__ int row_length(const LinAttnArgs& a, int b) { return a.lengths ? min(max(a.lengths[b], 0), a.T) : a.T; }
 
 // The workgroups of one XCD (every eighth) take neighbouring heads of the same tokens: rows of all heads lie together in memory, and heads that
@@ -335,7 +347,7 @@ __global__ __launch_bounds__(waves_of(DKP, DVP) * 64, occupancy_of(DKP, DVP)) vo
 #pragma unroll
         for (int x = 0; x < CT; ++x) wst[x / TPF][4 * (x % TPF) + i] = p0 * pt[CT - 1 - x];
     }
-    float m1 = expm1f(g * (float)C);
+    Decay fade(g, C);
 
     // o likewise: the lowest row of 16 tokens, and this lane's place from there
     const int osize = J.o16 ? 2 : 4;
@@ -441,14 +453,23 @@ __global__ __launch_bounds__(waves_of(DKP, DVP) * 64, occupancy_of(DKP, DVP)) vo
 #pragma unroll
                 for (int j = 0; j < KB / 4; ++j)
                     wst[u][j] = J.uscale * decay_power(g, max(0, L - e - (KB * u + 16 * (j >> 2) + M::srow(grp, j & 3))));
-            m1 = expm1f(g * (float)L);
+            fade = Decay(g, L);
         }
+        if (fade.most) {
 #pragma unroll
-        for (int x = 0; x < KT; ++x)
+            for (int x = 0; x < KT; ++x)
 #pragma unroll
-            for (int y = 0; y < VT; ++y)
+                for (int y = 0; y < VT; ++y)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) S[x][y][i] = __builtin_fmaf(S[x][y][i], m1, S[x][y][i]);
+                    for (int i = 0; i < 4; ++i) S[x][y][i] = __builtin_fmaf(S[x][y][i], fade.f, S[x][y][i]);
+        } else {
+#pragma unroll
+            for (int x = 0; x < KT; ++x)
+#pragma unroll
+                for (int y = 0; y < VT; ++y)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) S[x][y][i] *= fade.f;
+        }
         typename M::Frag wf[VT][M::NV];
         ahead<CF * KT, 2>([&](int i) { return M::state_col(ks, SK::LD, i % KT, i / KT, lane); },
                           [&](int i, const typename M::Frag& kf) {
@@ -503,7 +524,7 @@ __global__ __launch_bounds__(256) void linattn_segment_scan_kernel(const LinAttn
     const float g = a.g[bh % a.H];
     float* p = J.seg + (long)bh * (a.nseg - 1) * D + x;
     float run = J.s_in ? J.s_in[(long)bh * D + x] : 0.f;
-    const float em1 = expm1f(g * (float)a.seg_len);
+    const Decay fade(g, a.seg_len);
     for (int i0 = 0; i0 < a.nseg - 1; i0 += 8) {
         float y[8];
 #pragma unroll
@@ -511,7 +532,7 @@ __global__ __launch_bounds__(256) void linattn_segment_scan_kernel(const LinAttn
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             if (i0 + i >= a.nseg - 1 || (long)(i0 + i + 1) * a.seg_len >= n) return;      // what follows enters no token's segment
-            run = __builtin_fmaf(run, em1, run) + y[i];
+            run = fade(run) + y[i];
             p[(long)(i0 + i) * D] = run;
         }
     }

@@ -337,3 +337,35 @@ def test_rows_that_end_inside_a_piece(Dk, Dv, dt):
     a = ops.linear_attention(q.detach(), k.detach(), v.detach(), g, state=state.detach(), return_state=True)
     b = ops.linear_attention(inside(q.detach()), inside(k.detach()), inside(v.detach()), g, state=state.detach(), return_state=True)
     assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def kept(T, g, seed, dt=torch.float32, B=1, H=2, Dk=64, Dv=64):
+    """a first state that nothing is added to (k = 0), and a last gradient likewise (do = 0): what is left of them after T tokens"""
+    q, k, v, _, state, do, ds = make(B, T, H, H, H, H, Dk, Dv, dt, seed=seed)
+    g = torch.tensor(g, dtype=torch.float64).log() if min(g) > 0 else torch.tensor(g, dtype=torch.float64)
+    g = g.float().to(DEV)
+    s0 = state.requires_grad_()
+    _, s = ops.linear_attention(q, torch.zeros_like(k), v, g, state=s0, return_state=True)
+    d, = torch.autograd.grad(s, s0, ds)
+    want = torch.exp(g.double() * T)[None, :, None, None]
+    return (s.detach().double() / s0.detach().double() / want - 1, d.double() / ds.double() / want - 1), float(g.abs().max()) * T
+
+
+@pytest.mark.parametrize('dt', (torch.float32, torch.bfloat16), ids=('fp32', 'bf16'))
+@pytest.mark.parametrize('T,g', ((16, -0.5), (64, -0.25), (64, -0.5), (64, -1.0), (70, -0.9), (640, -0.1), (2000, -0.02), (2000, -0.0113)))
+def test_strongly_decayed_states_keep_their_digits(T, g, dt):
+    """What the decay leaves of a state is known to a relative error, however small it is: an exponent of at most |g| T is rounded once in pieces, its
+    exponential is within 2 ulp, and each of at most T / 16 factors is multiplied with one rounding."""
+    off, size = kept(T, [g, g / 2], T, dt)
+    for x in off:
+        assert float(x.abs().max()) <= (size + 4 * (T // 16 + 2)) * 2.0 ** -24
+
+
+@pytest.mark.parametrize('T', (4096, 9001, 30000))
+def test_slow_decays_are_not_off_the_same_way_in_every_chunk(T):
+    """The mean relative error of 2 x 4 096 kept elements: roundings of single products are independent, 2^-24 sqrt(chunks) / sqrt(elements), here 5 sigma;
+    e^x - 1 is known to 2 ulp of itself, 2^-22 |g| T over all chunks.  A factor rounded to fp32 is off by up to 2^-25 in each of T / 32 chunks."""
+    for p in (10.3, 11.6):
+        off, size = kept(T, [1 - 2.0 ** -p, 1 - 2.0 ** -(p + 0.37)], T)
+        for x in off:
+            assert float(x.mean((0, 2, 3)).abs().max()) <= (5 * (T / 32 + 2) ** 0.5 / 64 + 4 * size) * 2.0 ** -24
