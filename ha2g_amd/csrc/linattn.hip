@@ -538,7 +538,8 @@ __global__ __launch_bounds__(256) void linattn_segment_scan_kernel(const LinAttn
     }
 }
 
-// One token: a block per (batch row, head), bound by the state's one read and one write.  Thread = (row group, V neighbouring columns), eight rows in
+// One token: a block per (batch row, head), bound by the state's one read and one write.  The decay is that of the chunked form: a factor rounded to
+// fp32 would let a long stream drift from the same prompt (5e-4 after 16 384 tokens at 1 - 2^-12).  Thread = (row group, V neighbouring columns), eight rows in
 // flight each; the partial sums over the row groups meet in LDS.  256 rows of 16 heads, 128 x 128: 105 us = 5.1 TB/s (a large copy: 4.9); one row
 // of 5 heads, 60 x 60: 3.9 us, the launch.
 template <typename T, int V>
@@ -556,7 +557,7 @@ __global__ __launch_bounds__(256) void linattn_step_kernel(const LinAttnArgs a, 
     for (int c = 0; c < V; ++c) { vv[c] = j < Dv ? ld1(v, j + c) : 0.f; acc[c] = 0.f; }
     if (tid < Dk) { qs[tid] = ld1(q, tid); ks[tid] = ld1(k, tid); }
     __syncthreads();
-    const float lam = expf(a.g[h]);
+    const Decay fade(a.g[h], 1);
     if (j < Dv)
         for (int d0 = r0; d0 < Dk; d0 += 8 * groups) {
             float s[8][V];
@@ -573,7 +574,7 @@ __global__ __launch_bounds__(256) void linattn_step_kernel(const LinAttnArgs a, 
                 const int d = d0 + u * groups;
                 if (d < Dk) {
 #pragma unroll
-                    for (int c = 0; c < V; ++c) { s[u][c] = lam * s[u][c] + ks[d] * vv[c]; acc[c] += qs[d] * s[u][c]; }
+                    for (int c = 0; c < V; ++c) { s[u][c] = fade(s[u][c]) + ks[d] * vv[c]; acc[c] += qs[d] * s[u][c]; }
                     if constexpr (V == 4) st4(S + (long)d * Dv, 0, make_float4(s[u][0], s[u][1], s[u][2], s[u][3]));
                     else S[(long)d * Dv] = s[u][0];
                 }

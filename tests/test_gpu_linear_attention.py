@@ -369,3 +369,22 @@ def test_slow_decays_are_not_off_the_same_way_in_every_chunk(T):
         off, size = kept(T, [1 - 2.0 ** -p, 1 - 2.0 ** -(p + 0.37)], T)
         for x in off:
             assert float(x.mean((0, 2, 3)).abs().max()) <= (5 * (T / 32 + 2) ** 0.5 / 64 + 4 * size) * 2.0 ** -24
+
+
+@pytest.mark.parametrize('dt', (torch.float32, torch.bfloat16), ids=('fp32', 'bf16'))
+def test_a_long_stream_of_single_tokens_does_not_drift(dt):
+    """16 384 single tokens with k = 0: as above, each token one rounding.  Strong decays: a relative error of (|g| + 4) 2^-24 a token."""
+    N, B, H, D = 16384, 4, 3, 64
+    q, k, v, _, state, _, _ = make(B, 1, H, H, H, H, D, D, dt, seed=21)
+    g = torch.log1p(-torch.exp2(-torch.tensor([10.3, 11.6, 12.45], dtype=torch.float64))).float().to(DEV)
+    s, zero = state.clone(), torch.zeros_like(k[:, 0])
+    for _ in range(N):
+        ops.linear_attention_step(q[:, 0], zero, v[:, 0], g, s)
+    off = s.double() / state.double() / torch.exp(g.double() * N)[None, :, None, None] - 1
+    size = float(g.abs().max()) * N
+    assert float(off.mean((0, 2, 3)).abs().max()) <= (5 * N ** 0.5 / (B * D * D) ** 0.5 + 4 * size) * 2.0 ** -24
+    g, s = torch.tensor([-0.5, -1.0, -4.0], device=DEV), state.clone()
+    for _ in range(16):
+        ops.linear_attention_step(q[:, 0], zero, v[:, 0], g, s)
+    off = s.double() / state.double() / torch.exp(g.double() * 16)[None, :, None, None] - 1
+    assert float(off.abs().max()) <= 16 * 8 * 2.0 ** -24
