@@ -664,11 +664,18 @@ int run_scan(const LinAttnArgs& a, hipStream_t st) {
 int tile_of(int d) { return d <= 32 ? 32 : (d <= 64 ? 64 : 128); }
 
 constexpr long STRIDE_LIMIT = 1L << 22;      // of a token, in elements: a workgroup's rows lie within 32 bits of each other
+// one token has no next one: its stride may be anything
+int check_strides(const char* what, const long* strides, int n, int T) {
+    for (int i = 1; T > 1 && i < 3 * n; i += 3)
+        HA2G_REQUIRE(strides[i] >= 0 && strides[i] < STRIDE_LIMIT, "%s: a token stride of %ld elements (0 to %ld)", what, strides[i], STRIDE_LIMIT - 1);
+    return 0;
+}
+long token_stride(const long* s, int T) { return T > 1 ? s[1] : 0; }
 
-Operand operand(const void* p, const long* s, int r) { return {p, s[0], s[1], s[2], r}; }
+Operand operand(const void* p, const long* s, int r, int T) { return {p, s[0], token_stride(s, T), s[2], r}; }
 
-void set_out(Job& j, void* o, const long* s, int o16) {
-    j.o = o; j.ob = s[0]; j.ot = s[1]; j.oh = s[2]; j.o16 = o16;
+void set_out(Job& j, void* o, const long* s, int o16, int T) {
+    j.o = o; j.ob = s[0]; j.ot = token_stride(s, T); j.oh = s[2]; j.o16 = o16;
 }
 // one segment's worth of states lies as the forward pass has it, [Dk][Dv]; `turned` where the job's state is that transposed
 void set_state(Job& j, const float* s_in, float* s_out, float* seg, bool turned) {
@@ -706,13 +713,12 @@ int ha2g_linattn_fwd(const void* q, const void* k, const void* v, void* o, const
     LinAttnArgs a;
     if (const int rc = check_args(a, "linattn_fwd", log_decay, lengths, B, T, H, rq, rk, rv, Dk, Dv, b16_io, q && k && v && o)) return rc;
     if (B == 0) return 0;
-    for (int i = 1; i < 12; i += 3)
-        HA2G_REQUIRE(strides[i] >= 0 && strides[i] < STRIDE_LIMIT, "linattn_fwd: a token stride of %ld elements (0 to %ld)", strides[i], STRIDE_LIMIT - 1);
+    if (const int rc = check_strides("linattn_fwd", strides, 4, T)) return rc;
     HA2G_REQUIRE(a.nseg == 1 || ws, "linattn_fwd: no workspace (ha2g_linattn_workspace_floats)");
     Job& j = a.job[0];
-    j.q = operand(q, strides, rq); j.k = operand(k, strides + 3, rk); j.v = operand(v, strides + 6, rv);
+    j.q = operand(q, strides, rq, T); j.k = operand(k, strides + 3, rk, T); j.v = operand(v, strides + 6, rv, T);
     j.Dk = Dk; j.Dv = Dv; j.rev = 0; j.oscale = scale; j.uscale = 1.f;
-    set_out(j, o, strides + 9, b16_io);
+    set_out(j, o, strides + 9, b16_io, T);
     set_state(j, s_in, s_out, ws, false);
     const hipStream_t st = (hipStream_t)stream;
     if (a.nseg > 1) {
@@ -729,20 +735,19 @@ int ha2g_linattn_bwd(const void* q, const void* k, const void* v, const void* do
     if (const int rc = check_args(a, "linattn_bwd", log_decay, lengths, B, T, H, rq, rk, rv, Dk, Dv, b16_io, q && k && v && dout)) return rc;
     HA2G_REQUIRE(B == 0 || dv || !ds_in || T == 0, "linattn_bwd: the gradient of the first state comes with dv");
     if (B == 0) return 0;
-    for (int i = 1; i < 21; i += 3)
-        HA2G_REQUIRE(strides[i] >= 0 && strides[i] < STRIDE_LIMIT, "linattn_bwd: a token stride of %ld elements (0 to %ld)", strides[i], STRIDE_LIMIT - 1);
+    if (const int rc = check_strides("linattn_bwd", strides, 7, T)) return rc;
     HA2G_REQUIRE(a.nseg == 1 || (ws && (ws_fwd || !dq)), "linattn_bwd: no workspace (ha2g_linattn_workspace_floats)");
-    const Operand oq_ = operand(q, strides, rq), ok_ = operand(k, strides + 3, rk), ov_ = operand(v, strides + 6, rv),
-                  od_ = operand(dout, strides + 9, 1);
+    const Operand oq_ = operand(q, strides, rq, T), ok_ = operand(k, strides + 3, rk, T), ov_ = operand(v, strides + 6, rv, T),
+                  od_ = operand(dout, strides + 9, 1, T);
     Job jv, jk, jq;
     jv.q = ok_; jv.k = oq_; jv.v = od_; jv.Dk = Dk; jv.Dv = Dv; jv.rev = 1; jv.oscale = 1.f; jv.uscale = scale;
-    set_out(jv, dv, strides + 18, dv_b16);
+    set_out(jv, dv, strides + 18, dv_b16, T);
     set_state(jv, ds_out, ds_in, ws, false);
     jk.q = ov_; jk.k = od_; jk.v = oq_; jk.Dk = Dv; jk.Dv = Dk; jk.rev = 1; jk.oscale = 1.f; jk.uscale = scale;
-    set_out(jk, dk, strides + 15, dk_b16);
+    set_out(jk, dk, strides + 15, dk_b16, T);
     set_state(jk, ds_out, nullptr, ws, true);
     jq.q = od_; jq.k = ov_; jq.v = ok_; jq.Dk = Dv; jq.Dv = Dk; jq.rev = 0; jq.oscale = scale; jq.uscale = 1.f;
-    set_out(jq, dq, strides + 12, dq_b16);
+    set_out(jq, dq, strides + 12, dq_b16, T);
     set_state(jq, s_in, nullptr, const_cast<float*>(ws_fwd), true);
     const hipStream_t st = (hipStream_t)stream;
     if (a.nseg > 1 && (dv || dk)) {                      // both walk through the same states; dq through the forward pass's
@@ -768,9 +773,9 @@ int ha2g_linattn_step(const void* q, const void* k, const void* v, void* o, cons
     if (const int rc = check_args(a, "linattn_step", log_decay, nullptr, B, 1, H, rq, rk, rv, Dk, Dv, b16_io, q && k && v && o && state)) return rc;
     if (B == 0) return 0;
     Job& j = a.job[0];
-    j.q = operand(q, strides, rq); j.k = operand(k, strides + 3, rk); j.v = operand(v, strides + 6, rv);
+    j.q = operand(q, strides, rq, 1); j.k = operand(k, strides + 3, rk, 1); j.v = operand(v, strides + 6, rv, 1);
     j.Dk = Dk; j.Dv = Dv; j.oscale = scale;
-    set_out(j, o, strides + 9, b16_io);
+    set_out(j, o, strides + 9, b16_io, 1);
     j.s_out = state;
     const bool wide = Dv % 4 == 0 && (uintptr_t)state % 16 == 0;
     int lpr = 1;

@@ -1942,9 +1942,9 @@ def _inner1(x):
 
 
 def _rows(x):
-    """[B, T, H, D] as the kernels read it: unit inner stride, tokens less than 2^22 elements apart"""
+    """[B, T, H, D] as the kernels read it: unit inner stride, tokens less than 2^22 elements apart (one token: anywhere)"""
     st = x.stride()
-    return x if (st[3] == 1 or x.shape[3] == 1) and st[1] < 4194304 else x.contiguous()
+    return x if (st[3] == 1 or x.shape[3] == 1) and (st[1] < 4194304 or x.shape[1] <= 1) else x.contiguous()
 
 
 _FLOATS = (torch.float32, torch.bfloat16)

@@ -574,7 +574,7 @@ int ha2g_logmel_f32(const float* y, int B, long n_samples, int pad_reflect, cons
 
 /* ---- linear attention with one decay per head (no reference counterpart; stands beside the GRU recurrence of model/hierarchy_net.py:87-88,144) ----
  *   S_t = e^{log_decay} S_{t-1} + k_t v_t^T,  o_t = scale q_t S_t     per batch row and head, S fp32 [Dk][Dv], 1 <= Dk, Dv <= 128
- * q, k, v, o: fp32, or (b16_io) bf16; strides = HOST array {batch, token, head} x {q, k, v, o} in elements, inner stride 1, token strides below 2^22.
+ * q, k, v, o: fp32, or (b16_io) bf16; strides = HOST array {batch, token, head} x {q, k, v, o} in elements, inner stride 1, token strides below 2^22 (not read for T = 1).
  * Head h of H reads head
  * h / rq of q, h / rk of k, h / rv of v.  s_in / s_out [B][H][Dk][Dv]: states in front of the first and behind the last token (NULL = zero, = not
  * wanted).  lengths [B] (device int32, NULL = T): tokens at and behind a row's length are not read, o is zero there.

@@ -388,3 +388,20 @@ def test_a_long_stream_of_single_tokens_does_not_drift(dt):
         ops.linear_attention_step(q[:, 0], zero, v[:, 0], g, s)
     off = s.double() / state.double() / torch.exp(g.double() * 16)[None, :, None, None] - 1
     assert float(off.abs().max()) <= 16 * 8 * 2.0 ** -24
+
+
+def test_one_token_of_any_token_stride():
+    """a time-major tensor turned to batch-major keeps a token stride of 2^22 elements and more that no second token uses; q, k, v and the output's
+    gradient, against the same values close together"""
+    B, H, D = 2048, 16, 128
+    big = [torch.randn(1, B, H, D, device=DEV).bfloat16().transpose(0, 1) for _ in range(4)]
+    assert big[0].stride(1) >= 2 ** 22 and big[0].shape == (B, 1, H, D)
+    g = torch.linspace(-0.5, -0.01, H, device=DEV)
+
+    def run(ts):
+        ls = [x.detach().requires_grad_() for x in ts[:3]]
+        o = ops.linear_attention(*ls, g)
+        return [o.detach(), *torch.autograd.grad(o, ls, ts[3])]
+    small = [x.squeeze(1).unsqueeze(1) for x in big]
+    assert small[0].stride(1) < 2 ** 22
+    assert all(torch.equal(a, b) for a, b in zip(run(big), run(small)))
