@@ -7,7 +7,6 @@ import os
 from array import array
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from ._lib import check, lib
 
@@ -1931,10 +1930,35 @@ def _on(t):
     return _here if t.device.index == _cur_device() else torch.cuda.device(t.device)
 
 
+class _NoSecondDerivative(torch.autograd.Function):
+    """passes gradients through; what they were computed from stands behind them in the graph, and differentiating them raises"""
+
+    @staticmethod
+    def forward(ctx, n, *tensors):
+        return tensors[:n]
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError('ha2g_amd: this gradient cannot be differentiated again (once_differentiable)')
+
+
 def _once(backward):
-    """a backward pass without one of its own: create_graph=True gets a node that refuses a second derivative (the check costs its time only there)"""
-    guarded = once_differentiable(backward)
-    return lambda ctx, *grads: (guarded if torch.is_grad_enabled() else backward)(ctx, *grads)
+    """a backward pass without one of its own: create_graph=True gets gradients that refuse a second derivative, whether the incoming gradients are constants
+    or not (the check costs its time only there)"""
+    def run(ctx, *grads):
+        if not torch.is_grad_enabled():
+            return backward(ctx, *grads)
+        with torch.no_grad():
+            out = backward(ctx, *grads)
+        there = [i for i, x in enumerate(out) if x is not None]
+        sources = [x for x in (*ctx.saved_tensors, *grads) if x is not None and x.requires_grad]
+        if not sources or not there:
+            return out
+        out = list(out)
+        for i, x in zip(there, _NoSecondDerivative.apply(len(there), *(out[i] for i in there), *sources)):
+            out[i] = x
+        return tuple(out)
+    return run
 
 
 def _inner1(x):
@@ -2202,7 +2226,8 @@ def _norm_check(what, y, groups, kind, vectors):
 def _tail_call(*args):
     """args of BlockTailFunction.forward; without a gradient to come no node is built and no statistics are kept"""
     if torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in args[:8]]):
-        return BlockTailFunction.apply(*args)
+        # contiguous here, under autograd: what the node saves are its own inputs, which a second derivative finds behind the gradients
+        return BlockTailFunction.apply(*[t if t is None or t.is_contiguous() else t.contiguous() for t in args[:8]], *args[8:])
     return _tail_forward(*args, False)[:2]
 
 

@@ -405,3 +405,20 @@ def test_one_token_of_any_token_stride():
     small = [x.squeeze(1).unsqueeze(1) for x in big]
     assert small[0].stride(1) < 2 ** 22
     assert all(torch.equal(a, b) for a, b in zip(run(big), run(small)))
+
+
+@pytest.mark.parametrize('cotangent', ('constant', 'of_the_input'))
+def test_a_second_derivative_is_refused_whatever_the_cotangent(cotangent):
+    q, k, v, g, _, _, _ = make(2, 5, 2, 2, 2, 2, 8, 8, torch.float32, seed=18)
+    q, k = q.detach().requires_grad_(), k.detach().requires_grad_()
+    o = ops.linear_attention(q, k, v.detach(), g)
+    loss = o.sum() if cotangent == 'constant' else (o * q).sum()
+    dq, = torch.autograd.grad(loss, q, create_graph=True)
+    with pytest.raises(RuntimeError, match='once_differentiable'):
+        (loss + dq.square().sum()).backward()
+    y, w = torch.randn(3, 8, 2, device=DEV).transpose(1, 2).requires_grad_(), torch.ones(8, device=DEV, requires_grad=True)      # a copy is made of y
+    h = ops.row_norm(y, w)
+    loss = h.sum() if cotangent == 'constant' else (h * y).sum()
+    dy, = torch.autograd.grad(loss, y, create_graph=True)
+    with pytest.raises(RuntimeError, match='once_differentiable'):
+        torch.autograd.grad(dy.square().sum(), y)

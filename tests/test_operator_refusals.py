@@ -127,3 +127,35 @@ def test_c_entries_return_errors_instead_of_launching():
     assert tail(0, 8, 2, 4) == 0
     for bad in ((1, 8, 2, 4), (0, 8, 3, 4), (0, 8, 2, 1), (0, 20000, 1, 4), (70000, 8, 2, 4)):
         assert tail(*bad) != 0 and lib.ha2g_last_error()
+
+
+class _Cube(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, y):
+        ctx.save_for_backward(x)
+        return x ** 3 + y
+
+    @staticmethod
+    @ops._once
+    def backward(ctx, d):
+        x, = ctx.saved_tensors
+        return 3 * x * x * d, d if ctx.needs_input_grad[1] else None
+
+
+def test_gradients_of_a_pass_without_a_backward_of_its_own_refuse_a_second_derivative():
+    """a gradient penalty whose incoming gradient is a constant would lose its term in silence (12 instead of 300 at x = 2)"""
+    x = torch.tensor(2.0, requires_grad=True)
+    for loss in (lambda o: o, lambda o: o * x, lambda o: o.square()):
+        o = _Cube.apply(x, torch.tensor(1.0))
+        g, = torch.autograd.grad(loss(o), x, create_graph=True)
+        assert g.requires_grad
+        with pytest.raises(RuntimeError, match='once_differentiable'):
+            (o + g.square()).backward()
+        with pytest.raises(RuntimeError, match='once_differentiable'):
+            torch.autograd.grad(g, x)
+    # first derivatives are what they were, with and without a graph of them, and a gradient that depends on nothing is a constant
+    assert torch.autograd.grad(_Cube.apply(x, torch.tensor(1.0)), x)[0] == 12
+    assert torch.autograd.grad(_Cube.apply(x, torch.tensor(1.0)), x, create_graph=True)[0] == 12
+    y = torch.tensor(1.0, requires_grad=True)
+    g, = torch.autograd.grad(_Cube.apply(x.detach(), y), y, create_graph=True)
+    assert g == 1 and not g.requires_grad
