@@ -7,6 +7,7 @@ import os
 from array import array
 
 import torch
+from torch.autograd import forward_ad
 
 from ._lib import check, lib
 
@@ -1930,6 +1931,12 @@ def _on(t):
     return _here if t.device.index == _cur_device() else torch.cuda.device(t.device)
 
 
+def _no_tangents(what, tensors):
+    """a forward-mode tangent would be dropped: a dual tensor does not require grad, and its address is that of its values (no level: one comparison)"""
+    if forward_ad._current_level >= 0:
+        _need(all(t is None or forward_ad.unpack_dual(t).tangent is None for t in tensors), '%s: no forward-mode derivative', what)
+
+
 class _NoSecondDerivative(torch.autograd.Function):
     """passes gradients through; what they were computed from stands behind them in the graph, and differentiating them raises"""
 
@@ -2085,6 +2092,7 @@ def linear_attention(q, k, v, log_decay, scale=None, state=None, lengths=None, r
     if lengths is not None:
         _need(lengths.shape == (q.shape[0],) and lengths.dtype == torch.int32 and lengths.device == q.device and lengths.is_contiguous(),
               'linear_attention: lengths is int32 [%d] on the device of q', q.shape[0])
+    _no_tangents('linear_attention', (q, k, v, log_decay, state))
     scale = float(Dk ** -0.5 if scale is None else scale)
     if state is not None:
         state = state.contiguous()
@@ -2103,6 +2111,7 @@ def linear_attention_step(q, k, v, log_decay, state, scale=None):
         raise ValueError('ha2g_amd: linear_attention_step: needs a contiguous state')
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad):
         raise ValueError('ha2g_amd: linear_attention_step: no gradient (use linear_attention)')
+    _no_tangents('linear_attention_step', (q, k, v, log_decay, state))
     q, k, v = _inner1(q), _inner1(k), _inner1(v)
     B, (qb, qh, _), (kb, kh, _), (vb, vh, _) = q.shape[0], q.stride(), k.stride(), v.stride()
     with _on(q):
@@ -2225,6 +2234,7 @@ def _norm_check(what, y, groups, kind, vectors):
 
 def _tail_call(*args):
     """args of BlockTailFunction.forward; without a gradient to come no node is built and no statistics are kept"""
+    _no_tangents('row_norm / block_tail', args[:8])
     if torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in args[:8]]):
         # contiguous here, under autograd: what the node saves are its own inputs, which a second derivative finds behind the gradients
         return BlockTailFunction.apply(*[t if t is None or t.is_contiguous() else t.contiguous() for t in args[:8]], *args[8:])

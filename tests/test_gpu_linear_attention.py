@@ -422,3 +422,27 @@ def test_a_second_derivative_is_refused_whatever_the_cotangent(cotangent):
     dy, = torch.autograd.grad(loss, y, create_graph=True)
     with pytest.raises(RuntimeError, match='once_differentiable'):
         torch.autograd.grad(dy.square().sum(), y)
+
+
+def test_forward_mode_derivatives_are_refused():
+    from torch.autograd import forward_ad
+    q, k, v, g, state, _, _ = make(2, 3, 2, 2, 2, 2, 8, 8, torch.float32, seed=19)
+    w = torch.ones(8, device=DEV)
+    with forward_ad.dual_level():
+        dual = lambda x: forward_ad.make_dual(x, torch.ones_like(x))      # noqa: E731
+        for i in range(4):
+            a = [q, k, v, state]
+            a[i] = dual(a[i])
+            with pytest.raises(ValueError, match='forward-mode'):
+                ops.linear_attention(*a[:3], g, state=a[3])
+            a = [q[:, 0], k[:, 0], v[:, 0], state.clone()]
+            a[i] = dual(a[i])
+            with pytest.raises(ValueError, match='forward-mode'):
+                ops.linear_attention_step(*a[:3], g, a[3])
+        for call in (lambda x: ops.row_norm(x, w), lambda x: ops.block_tail(x), lambda x: ops.block_tail(q, x), lambda x: ops.block_tail(q, gate=x)):
+            with pytest.raises(ValueError, match='forward-mode'):
+                call(dual(q))
+        with pytest.raises(ValueError, match='forward-mode'):
+            ops.row_norm(q, dual(w))
+        ops.linear_attention(q, k, v, g, state=state)                     # no tangent: as always
+        ops.row_norm(q, w)
