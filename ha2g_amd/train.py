@@ -56,17 +56,17 @@ class HierarchyTrainer:
         a = self.args
         lr = float(a.learning_rate)
         sp = (lambda enc: [enc.embedding.weight]) if self.sparse_embeddings else (lambda enc: [])
-        # args.optimizer: 'adam' (the reference's, default), 'adamw' or 'adamw8' = decoupled weight decay (args.weight_decay; vectors are not decayed)
-        # with fp32 or 8-bit moments
+        # args.optimizer: 'adam' (the reference's, default), 'adamw' or 'adamw8' = decoupled weight decay (args.weight_decay; vectors and the gains of
+        # weight-normalised convolutions, one value per channel, are not decayed) with fp32 or 8-bit moments
         kind = getattr(a, 'optimizer', 'adam')
         if kind in ('adamw', 'adamw8'):
             if self.sparse_embeddings:
                 raise ValueError('ha2g_amd: row-wise embedding updates need args.optimizer = "adam" (sparse_embeddings=False keeps the tables dense)')
 
             def make(m, lr):
-                ps = list(m.parameters())
-                return FusedAdamW(ps, lr=lr, betas=(0.5, 0.999), weight_decay=float(getattr(a, 'weight_decay', 0.01)),
-                                  no_decay=[p for p in ps if p.dim() < 2], state_bits=8 if kind == 'adamw8' else 32, seed=int(getattr(a, 'random_seed', 0)))
+                return FusedAdamW(m.parameters(), lr=lr, betas=(0.5, 0.999), weight_decay=float(getattr(a, 'weight_decay', 0.01)),
+                                  no_decay=[p for n, p in m.named_parameters() if p.dim() < 2 or n.endswith('weight_g')],
+                                  state_bits=8 if kind == 'adamw8' else 32, seed=int(getattr(a, 'random_seed', 0)))
             self.gen_opts = [make(g, lr) for g in self.gens]
             self.audio_opt, self.text_opt = make(self.audio_encoder, lr), make(self.text_encoder, lr)
             self.dis_opt = make(self.discriminator, lr * a.discriminator_lr_weight)

@@ -390,3 +390,25 @@ def test_scales_listed_twice_are_refused():
         optim.adamw_step(p, g, [(mc, s)], [(vc, s)], step)
     assert int(step) == 0
     optim.adamw_step(p, g, [(mc, s)], [(vc, r)], step)
+
+
+@pytest.mark.parametrize('kind', ('adamw', 'adamw8'))
+def test_what_the_trainer_decays(kind):
+    """a step with gradients of zero multiplies what is decayed by fp32(1 - lr wd) and leaves the rest: biases, norm weights, the gains of weight norms"""
+    from bench import Vocab
+    from ha2g_amd.config import hierarchy_args
+    from ha2g_amd.train import HierarchyTrainer
+    torch.manual_seed(0)
+    tr = HierarchyTrainer(hierarchy_args(hidden_size=32, n_layers=2, optimizer=kind, weight_decay=0.05), Vocab(50), Vocab(7), 27, torch.device(DEV))
+    gains = 0
+    for m, o in zip([*tr.gens, tr.audio_encoder, tr.text_encoder, tr.discriminator], [*tr.gen_opts, tr.audio_opt, tr.text_opt, tr.dis_opt]):
+        before = {n: p.detach().clone() for n, p in m.named_parameters() if p.requires_grad}
+        o.zero_grad()
+        o.step()
+        keep = torch.tensor(1.0 - o.param_groups[0]['lr'] * 0.05, dtype=torch.float32, device=DEV)
+        for n, p in m.named_parameters():
+            if p.requires_grad:
+                still = p.dim() < 2 or n.split('.')[-1] == 'weight_g'
+                gains += p.dim() > 1 and still
+                assert torch.equal(p.detach(), before[n] if still else before[n] * keep), n
+    assert gains > 0
