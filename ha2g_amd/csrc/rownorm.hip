@@ -122,10 +122,25 @@ template <int TPR, int NI, int VEC, bool RAG> struct Place {
     __device__ __forceinline__ int k(int i) const { if constexpr (RAG) return k_[i]; else return VEC; }
 };
 
-// the gate's activation and its derivative
-__device__ __forceinline__ void gate_act(float g, int act, float& a, float& d) {
+// 1 / (1 + e^-g) to 2^-22 of its value.  The hardware's 2^t of t = -g log2(e) rounded to fp32 is off by |g| 2^-24 of its value; what the rounding left out,
+// r = -g - t ln 2 (ln 2 in two parts), enters as e^r = 1 + r.  t is held at 127, where r grows instead and the sum overflows as it should; an infinite g
+// leaves r undefined and p infinite or 0: 0 for max(), which also takes a NaN for 0 (gate_act puts it back).
+__device__ __forceinline__ float sigmoid_fp32(float g) {
+    const float t = fminf(g * -1.44269504f, 127.f), p = __builtin_amdgcn_exp2f(t);
+    const float r = __builtin_fmaf(t, 1.9046543e-9f, __builtin_fmaf(t, -0.693147182f, -g));
+    return __builtin_amdgcn_rcpf(1.0f + fmaxf(__builtin_fmaf(p, r, p), 0.f));
+}
+// The gate's activation and its derivative.  Rows of fp32 take the sigmoid above (2^25 values: 2 048 per row, forward 137 us, 135 with
+// the other, backward 250 and 249; at most 1 500 per row forward, 154 and 144).  Rows of bf16 take the hardware's exponential and reciprocal: off by (|g| + 4) 2^-24 of the value, at most 2^-17 where the
+// result is not 0 or 1, and every result of it is rounded to 2^-9 or summed in fp32 with errors of that size (the other one costs 3 to 10 %, and
+// 60 % where it exceeds the registers: 1 500 and 2 002 values per row, backward 233 -> 366 and 261 -> 424 us).
+template <typename T> __device__ __forceinline__ void gate_act(float g, int act, float& a, float& d) {
     if (act == 0) { a = g; d = 1.f; return; }
-    const float s = sigmoidf_(g);
+    float s;
+    if constexpr (sizeof(T) == 4) {
+        s = sigmoid_fp32(g);
+        if (act == 3) s = g == g ? s : g;
+    } else s = sigmoidf_(g);
     a = act == 3 ? s : g * s;
     d = act == 3 ? s * (1.f - s) : s * (1.f + g * (1.f - s));
 }
@@ -342,7 +357,7 @@ __global__ __launch_bounds__(block_of<TPR>()) void tail_fwd_kernel(const TailArg
             if (a.gate) {
                 unpack<VEC>(rg[i], t);
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) { float ga, gd; gate_act(t[j], a.act, ga, gd); x[i][j] *= ga; }
+                for (int j = 0; j < VEC; ++j) { float ga, gd; gate_act<T>(t[j], a.act, ga, gd); x[i][j] *= ga; }
             }
             if (a.s) {
 #pragma unroll
@@ -471,7 +486,7 @@ __global__ __launch_bounds__(block_of<TPR>()) void tail_bwd_kernel(const TailArg
                     float t[VEC];
                     unpack<VEC>(cur.gate[i], t);
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) gate_act(t[j], a.act, ga[i][j], gd[i][j]);
+                    for (int j = 0; j < VEC; ++j) gate_act<T>(t[j], a.act, ga[i][j], gd[i][j]);
                 }
             }
         }
@@ -663,7 +678,7 @@ template <typename T, int VEC, bool RAG, bool FULL> struct Chunk {
             if (a.gate) {
                 unpack<VEC>(in.gate, t);
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) gate_act(t[j], a.act, ga[j], gd[j]);
+                for (int j = 0; j < VEC; ++j) gate_act<T>(t[j], a.act, ga[j], gd[j]);
             }
             if (a.w2) {
                 fill<VEC>(t, 0.f);

@@ -2255,7 +2255,8 @@ def block_tail(y, residual=None, gate=None, weight=None, bias=None, scale=None, 
         u = (norm(y) * weight + bias) * gate_act(gate);   h = alpha * residual + scale * u;   z = norm(h) * next_weight + next_bias
     Every part is optional: weight None = no norm in front of the gate, next_weight None = no z.  The first norm runs over `groups` equal parts of a
     row (heads), the second over the whole row.  gate: y's shape, or [B, 1, ..., C] = one row per sequence y[b].  gate_act: ACT_NONE, ACT_SIGMOID or
-    ACT_SILU.  scale [C] fp32 weights the branch, alpha the residual.  z is taken of h before it is rounded to y's type.
+    ACT_SILU (a bf16 gate's sigmoid is known to 2^-17 of its value).  scale [C] fp32 weights the branch, alpha the residual.  z is taken of h before it
+    is rounded to y's type.
     Returns h, or (h, z) with next_weight."""
     _norm_check('block_tail', y, groups, kind, (weight, bias, scale, next_weight, next_bias))
     if (bias is not None and weight is None) or (next_bias is not None and next_weight is None):

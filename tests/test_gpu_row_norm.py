@@ -307,3 +307,25 @@ def test_without_an_eps(C, G, kind, dt, monkeypatch):
     """eps = 0 on rows that have a scale of their own: places that a row does not fill reach neither the second norm nor a gradient"""
     monkeypatch.setitem(globals(), 'EPS', 0.0)
     check_all((2, 5, C), dt, kind=kind, G=G, parts=('w', 'b', 'res', 'scale', 'w2', 'b2'), gate='sequence', alpha=0.7, seed=C + G)
+
+
+@pytest.mark.parametrize('act', (ops.ACT_SIGMOID, ops.ACT_SILU))
+def test_gates_far_from_zero(act):
+    """y = 1 and a gate from -80 to 80, forward and backward: the exponential is within 2 ulp of its value, the sum, the quotient and the products behind
+    it within half each, 1 - sigmoid by its own distance from 1: 8 2^-24 of the value, for a derivative 8 2^-24 of its terms' magnitudes."""
+    gate = torch.linspace(-80, 80, 4096, device=DEV).view(4, 1024).requires_grad_()
+    y = torch.ones(4, 1024, device=DEV, requires_grad=True)
+    h = ops.block_tail(y, gate=gate, gate_act=act)
+    dy, dg = torch.autograd.grad(h, (y, gate), torch.ones_like(h))
+    x = gate.detach().double()
+    s, c = torch.sigmoid(x), torch.sigmoid(-x)
+    want = s if act == ops.ACT_SIGMOID else x * s
+    der, mag = (s * c, s) if act == ops.ACT_SIGMOID else (s * (1 + x * c), s * (1 + x.abs()))
+    u = 8 * 2.0 ** -24
+    for got, w, m in ((h.detach(), want, want.abs()), (dy, want, want.abs()), (dg, der, mag)):
+        assert ((got.double() - w).abs() <= u * m + 1e-37).all(), float(((got.double() - w).abs() / (u * m)).max())
+    gate = torch.tensor([float('inf'), float('-inf'), float('nan'), 3e38, -3e38, 200.0, -200.0], device=DEV)
+    h = ops.block_tail(torch.ones_like(gate), gate=gate, gate_act=act).cpu()
+    want = [1.0, 0.0, None, 1.0, 0.0, 1.0, 0.0] if act == ops.ACT_SIGMOID else [float('inf'), None, None, 3e38, 0.0, 200.0, 0.0]
+    for x, w in zip(h.tolist(), want):
+        assert x != x if w is None else abs(x - w) <= 1e-37 or x == torch.tensor(w).item(), (x, w)
