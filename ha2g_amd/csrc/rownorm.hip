@@ -130,10 +130,10 @@ __device__ __forceinline__ float sigmoid_fp32(float g) {
     const float r = __builtin_fmaf(t, 1.9046543e-9f, __builtin_fmaf(t, -0.693147182f, -g));
     return __builtin_amdgcn_rcpf(1.0f + fmaxf(__builtin_fmaf(p, r, p), 0.f));
 }
-// The gate's activation and its derivative.  Rows of fp32 take the sigmoid above (2^25 values: 2 048 per row, forward 137 us, 135 with
-// the other, backward 250 and 249; at most 1 500 per row forward, 154 and 144).  Rows of bf16 take the hardware's exponential and reciprocal: off by (|g| + 4) 2^-24 of the value, at most 2^-17 where the
-// result is not 0 or 1, and every result of it is rounded to 2^-9 or summed in fp32 with errors of that size (the other one costs 3 to 10 %, and
-// 60 % where it exceeds the registers: 1 500 and 2 002 values per row, backward 233 -> 366 and 261 -> 424 us).
+// The gate's activation and its derivative.  Rows of fp32 take the sigmoid above (2^25 values: 2 048 per row, forward 137 us, 135 with the other, backward
+// 250 and 249; at most, 1 500 per row, forward 154 and 144).  Rows of bf16 take the hardware's exponential and reciprocal: off by (|g| + 4) 2^-24 of
+// the value, at most 2^-17 where the result is not 0 or 1, and every result of it is rounded to 2^-9 or summed in fp32 with errors of that size (the
+// other one costs 3 to 10 %, and 60 % where it exceeds the registers: 1 500 and 2 002 values per row, backward 233 -> 366 and 261 -> 424 us).
 template <typename T> __device__ __forceinline__ void gate_act(float g, int act, float& a, float& d) {
     if (act == 0) { a = g; d = 1.f; return; }
     float s;
