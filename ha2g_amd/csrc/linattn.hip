@@ -54,6 +54,7 @@ template <> __device__ __forceinline__ void st1<b16>(b16* p, long i, float v) {
 // The decay of S is S + S (e^{gC} - 1) where more than half is kept: a factor rounded to fp32 is off the same way in every chunk, 1e-4 of a state with a
 // memory of 2^12 tokens.  Where less is kept it is S e^{gC}: the sum is exact to 2^-24 of the S before, not of what is left of it.
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
 typedef short s16x8_t __attribute__((ext_vector_type(8)));
 typedef unsigned u32x4_t __attribute__((ext_vector_type(4)));
@@ -144,6 +145,16 @@ template <> struct Mma<b16> {
     }
 };
 
+// z + zeros, NaN if the 16 bytes hold a value that is not finite
+template <typename T> __device__ __forceinline__ float probe(u32x4_t r, float z) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if constexpr (sizeof(T) == 4) z = __builtin_fmaf(__uint_as_float(r[j]), 0.f, z);
+        else z = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, r[j]), __builtin_bit_cast(bf16x2_t, 0u), z, false);
+    }
+    return z;
+}
+
 // 16 bytes at any multiple of an element's size
 typedef u32x4_t u32x4_a2 __attribute__((aligned(2)));
 typedef unsigned u32x2_a2 __attribute__((ext_vector_type(2), aligned(2)));
@@ -209,6 +220,27 @@ template <typename T, int D, int C, int NT, bool WHOLE> struct Stage {
         }
         base += chunk;
     }
+    // Zeros in place of what is not finite; first[c] <- the first row of the chunk in which column c was that (in LDS, the chunk's length before)
+    __device__ __forceinline__ void keep_finite(int* first) {
+        float z = 0.f;
+#pragma unroll
+        for (int j = 0; j < N; ++j) z = probe<T>(r[j], z);
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(z != z) == 0, 1)) return;
+        int me = threadIdx.x;                                        // hidden from the compiler, which would keep this rare path's addresses over all chunks
+        asm volatile("" : "+v"(me));
+        const int c0 = me % V * E + (!WHOLE && shift > 0 && left < E ? left - E : 0), row0 = me / V;
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const int w = e * (int)sizeof(T) / 4;
+                const unsigned mask = sizeof(T) == 4 ? ~0u : 0xffffu << (16 * (e & 1)), top = 0x7f800000u >> (sizeof(T) == 4 || (e & 1) ? 0 : 16);
+                if ((r[j][w] & top) == top) {
+                    r[j][w] &= ~mask;
+                    atomicMin(first + c0 + e, row0 + j * RS);
+                }
+            }
+    }
     __device__ __forceinline__ void store(T* lds) const {
         T* p = lds + threadIdx.x / V * LD + threadIdx.x % V * E;
 #pragma unroll
@@ -272,7 +304,9 @@ __global__ __launch_bounds__(waves_of(DKP, DVP) * 64, occupancy_of(DKP, DVP)) vo
     __shared__ __attribute__((aligned(16))) T ks[C * SK::LD];
     __shared__ __attribute__((aligned(16))) T vs[C * SV::LD];
     __shared__ __attribute__((aligned(16))) typename M::Tile ps[STATE_ONLY ? 1 : TILES * M::NS * 64];
+    __shared__ int first[STATE_ONLY ? 1 : DVP];                  // a column's first token of the chunk that is not finite; C: none
     const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4, wave = threadIdx.x >> 6, v0 = wave * DVW;
+    if (!STATE_ONLY && lane < DVW) first[v0 + lane] = C;
     const long wg = xcd_order(blockIdx.x, gridDim.x);
     const int h = (int)(wg % a.H), seg = (int)(wg / a.H % a.nseg), b = (int)(wg / a.H / a.nseg);
     const long bh = (long)b * a.H + h, D2 = (long)J.Dk * J.Dv;
@@ -358,6 +392,9 @@ __global__ __launch_bounds__(waves_of(DKP, DVP) * 64, occupancy_of(DKP, DVP)) vo
         __syncthreads();
         if constexpr (!STATE_ONLY) rq.store(qs);
         rk.store(ks);
+        // A score of 0 does not keep NaN or infinity in v from the tokens in front of it.  The products take 0 for them, and behind the products what a
+        // column's first one reaches is made NaN: the outputs from its token on, and the state.  (The checks cost 1 to 2 %.)
+        if constexpr (!STATE_ONLY) rv.keep_finite(first);
         rv.store(vs);
         __syncthreads();
         const int L = min(C, end - c0), c1 = c0 + C;
@@ -371,6 +408,13 @@ __global__ __launch_bounds__(waves_of(DKP, DVP) * 64, occupancy_of(DKP, DVP)) vo
         for (int u = 0; u < CF; ++u)
 #pragma unroll
             for (int y = 0; y < VT; ++y) vf[u][y] = M::col(vs, SV::LD, v0 + 16 * y, u, lane);
+        bool finite = true;                                        // this wave's columns
+        if constexpr (!STATE_ONLY) {
+            int n = C;
+#pragma unroll
+            for (int y = 0; y < VT; ++y) n = min(n, first[v0 + 16 * y + col]);
+            finite = __builtin_amdgcn_ballot_w64(n < C) == 0;
+        }
         if constexpr (!STATE_ONLY) {
             // this wave's score tiles, for all
 #pragma unroll
@@ -486,7 +530,27 @@ __global__ __launch_bounds__(waves_of(DKP, DVP) * 64, occupancy_of(DKP, DVP)) vo
 #pragma unroll
                 for (int y = 0; y < VT; ++y) S[x][y] = M::mma(kf, wf[y][p], S[x][y]);
         });
+        if constexpr (!STATE_ONLY)
+            if (__builtin_expect(!finite, 0)) {
+                int me = lane;                                       // hidden likewise
+                asm volatile("" : "+v"(me));
+                const int j = v0 + me % DVW;
+                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");      // behind the outputs that other lanes stored there
+                for (int r = first[j]; r < L && j < Dv; ++r) {
+                    char* const p = (char*)J.o + (obase + (t0 + dir * (c0 + r)) * J.ot + j) * osize;
+                    if (J.o16) st1((b16*)p, 0, __builtin_nanf("")); else st1((float*)p, 0, __builtin_nanf(""));
+                }
+                if (first[j] < C) first[j] = 0;                      // and of all chunks to come
+            }
     }
+    if constexpr (!STATE_ONLY)
+#pragma unroll
+        for (int y = 0; y < VT; ++y)
+            if (first[j_lane + 16 * y] < C)
+#pragma unroll
+                for (int x = 0; x < KT; ++x)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) S[x][y][i] = __builtin_nanf("");
     float* s_out;
     int oi = J.si, oj = J.sj;
     if constexpr (STATE_ONLY) {

@@ -2086,7 +2086,7 @@ def linear_attention(q, k, v, log_decay, scale=None, state=None, lengths=None, r
     read in place), Dk and Dv from 1 to 128.  log_decay [H] fp32 <= 0, a constant; Hq, Hk, Hv divide H, head h reads head h // (H // Hx).
     state [B, H, Dk, Dv] fp32: what stands before the first token (None: zero).  lengths [B] int32 on the device: row b ends after lengths[b]
     tokens (clipped to 0 .. T); what lies behind is not read, the output and the gradients there are zero.
-    A value that is not finite reaches the tokens behind it, and may reach up to 31 in front of it (its tile of the products).
+    A value that is not finite reaches its own token and those behind it (gradients: in front of it), as NaN, and nothing else.
     Returns o [B, T, H, Dv] in v's type, with return_state also the state behind each row's last token, fp32."""
     _, Dk, _ = _la_check('linear_attention', q, k, v, log_decay, state, 4)
     if lengths is not None:

@@ -446,3 +446,34 @@ def test_forward_mode_derivatives_are_refused():
             ops.row_norm(q, dual(w))
         ops.linear_attention(q, k, v, g, state=state)                     # no tangent: as always
         ops.row_norm(q, w)
+
+
+@pytest.mark.parametrize('dt', (torch.float32, torch.bfloat16), ids=('fp32', 'bf16'))
+@pytest.mark.parametrize('T,j', ((5, 3), (20, 16), (64, 31), (70, 40), (70, 69), (300, 130)))
+@pytest.mark.parametrize('bad', (float('nan'), float('inf'), float('-inf')))
+@pytest.mark.parametrize('D', ((16, 24), (60, 64), (128, 128)))
+def test_values_that_are_not_finite_reach_no_earlier_token(T, j, bad, D, dt):
+    """q, k, v of a token reach its own output and those behind it; do the gradients of k and v of its own token and those in front of it.  What they do not
+    reach is what it is without them, to the rounding of sums in another grouping."""
+    q, k, v, g, state, do, ds = make(1, T, 2, 2, 2, 2, *D, dt, seed=T + j)
+    t = torch.arange(T, device=DEV)
+    for i in range(4):
+        a = [x.detach().clone() for x in (q, k, v, do)]
+        a[i][:, j, :, 1] = bad
+        leaves = [x.requires_grad_() for x in a[:3]]
+        o = ops.linear_attention(*leaves, g, state=state.detach())
+        grads = torch.autograd.grad(o, leaves, a[3])
+        base = [x.detach() for x in (q, k, v)]
+        ls = [x.clone().requires_grad_() for x in base]
+        o2 = ops.linear_attention(*ls, g, state=state.detach())
+        grads2 = torch.autograd.grad(o2, ls, do)
+        # (output, which tokens of it the bad value may reach)
+        reach = {0: ((o, o2, t == j), (grads[1], grads2[1], t <= j), (grads[2], grads2[2], t <= j)),
+                 1: ((o, o2, t >= j), (grads[0], grads2[0], t >= j), (grads[2], grads2[2], t == j)),
+                 2: ((o, o2, t >= j), (grads[0], grads2[0], t >= j), (grads[1], grads2[1], t == j)),
+                 3: ((grads[0], grads2[0], t == j), (grads[1], grads2[1], t <= j), (grads[2], grads2[2], t <= j))}[i]
+        for x, y, hit in reach:
+            x, y = x.detach().double()[:, ~hit], y.detach().double()[:, ~hit]
+            assert torch.isfinite(x).all(), (i, j)
+            assert x.numel() == 0 or float((x - y).norm()) <= 2.0 ** (-20 if dt == torch.float32 else -8) * float(y.norm()) + 1e-30
+        assert not torch.isfinite(o[:, j:j + 1].detach() if i < 3 else grads[1][:, j:j + 1]).all()
