@@ -2086,6 +2086,8 @@ def linear_attention(q, k, v, log_decay, scale=None, state=None, lengths=None, r
     read in place), Dk and Dv from 1 to 128.  log_decay [H] fp32 <= 0, a constant; Hq, Hk, Hv divide H, head h reads head h // (H // Hx).
     state [B, H, Dk, Dv] fp32: what stands before the first token (None: zero).  lengths [B] int32 on the device: row b ends after lengths[b]
     tokens (clipped to 0 .. T); what lies behind is not read, the output and the gradients there are zero.
+    bf16 operands: products and states are those of the values given (states fp32-exact), but where a state or a score enters an output's or a
+    gradient's product it is held to 16 bits, 2^-17 of each term; an output that cancels to less than 2^-8 of its terms is less exact than its type.
     A value that is not finite reaches its own token and those behind it (gradients: in front of it), as NaN, and nothing else.
     Returns o [B, T, H, Dv] in v's type, with return_state also the state behind each row's last token, fp32."""
     _, Dk, _ = _la_check('linear_attention', q, k, v, log_decay, state, 4)

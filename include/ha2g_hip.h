@@ -578,6 +578,7 @@ int ha2g_logmel_f32(const float* y, int B, long n_samples, int pad_reflect, cons
  * Head h of H reads head
  * h / rq of q, h / rk of k, h / rv of v.  s_in / s_out [B][H][Dk][Dv]: states in front of the first and behind the last token (NULL = zero, = not
  * wanted).  lengths [B] (device int32, NULL = T): tokens at and behind a row's length are not read, o is zero there.
+ * b16_io: a state or a score enters an output's product with 16 bits (2^-17 of each term); states themselves are fp32-exact.
  * ws: ha2g_linattn_workspace_floats() floats (0: may be NULL), the states between the segments of a time axis that is split over the chip. */
 long ha2g_linattn_workspace_floats(int B, int T, int H, int Dk, int Dv, int b16_io);
 int ha2g_linattn_fwd(const void* q, const void* k, const void* v, void* o, const float* log_decay, const float* s_in, float* s_out, const int* lengths,
