@@ -31,7 +31,14 @@ def _host_staged(t, group):
     return t.is_cuda and dist.get_backend(group) == 'gloo'
 
 
+def _not_in_capture(t):
+    """A step captured together with its RCCL collectives has ended its process with an abort, without a known cause: refused until there is one."""
+    if t.is_cuda and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError('ha2g_amd: a collective inside a graph capture is refused (data-parallel steps run eagerly)')
+
+
 def all_reduce_(t, group=None, async_op=False):
+    _not_in_capture(t)
     if _host_staged(t, group):
         h = t.cpu()
         dist.all_reduce(h, op=dist.ReduceOp.SUM, group=group)
@@ -45,6 +52,7 @@ def sync_flag_(flag, group=None):
     replica applies a step or none does -- a rank-local time-out must not let the replicas diverge.  One 4-byte collective."""
     if flag is None or not active(group):
         return
+    _not_in_capture(flag)
     if _host_staged(flag, group):
         h = flag.cpu()
         dist.all_reduce(h, op=dist.ReduceOp.MAX, group=group)
@@ -54,6 +62,7 @@ def sync_flag_(flag, group=None):
 
 
 def all_gather_(outs, t, group=None):
+    _not_in_capture(t)
     if _host_staged(t, group):
         hs = [torch.empty(o.shape, dtype=o.dtype) for o in outs]
         dist.all_gather(hs, t.cpu(), group=group)
@@ -64,6 +73,7 @@ def all_gather_(outs, t, group=None):
 
 
 def broadcast_one_(t, src=0, group=None):
+    _not_in_capture(t)
     if _host_staged(t, group):
         h = t.cpu()
         dist.broadcast(h, src, group=group)
@@ -133,6 +143,7 @@ class _CountHandle:
 
 def prefetch_max_count(count, group=None):
     """Enqueue (do not wait for) the all-gather of one int32 device count over the ranks and the copy of the result to pinned host memory."""
+    _not_in_capture(count)
     ws = dist.get_world_size(group)
     cnt = count.to(torch.int64).reshape(1)
     if _host_staged(cnt, group) or not cnt.is_cuda:

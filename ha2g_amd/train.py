@@ -129,7 +129,11 @@ class HierarchyTrainer:
     def capture_step(self, epoch, in_text_padded, in_spec, target, vid_indices, warmup=2):
         """Capture one whole train step on these (static) input tensors into a hipGraph.  Returns (graph, names, packed):
         `graph.replay()` runs the step (fresh dropout masks / noise per replay, device-side Adam counters), `packed` then holds
-        the logged scalars in `names` order.  Update the input tensors in place to feed new batches."""
+        the logged scalars in `names` order.  Update the input tensors in place to feed new batches.  Without active collectives: a step captured together
+        with them has ended its process with an abort, without a known cause, and is refused."""
+        from . import ddp
+        if ddp.active():
+            raise RuntimeError('ha2g_amd: capture_step with active collectives is refused (data-parallel steps run eagerly)')
         s = torch.cuda.Stream(self.device)
         s.wait_stream(ops.cur_stream(self.device))
         with torch.cuda.stream(s):                   # allocations / workspaces of the capture stream are created outside capture
