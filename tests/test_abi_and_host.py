@@ -137,3 +137,16 @@ def test_graft_entry_build_passes_on_the_tree_as_it_is():
     """The driver's "does it build" hook: make (a no-op when the objects are current), import of the oracle and the package, ABI version check."""
     import __graft_entry__ as g
     g.build()
+
+
+def test_objects_are_rebuilt_when_the_flags_change():
+    """the compiler's flags live in the Makefile: objects built with other ones must not be linked again"""
+    import glob
+    import shutil
+    import subprocess
+    csrc = os.path.join(ROOT, 'ha2g_amd', 'csrc')
+    if shutil.which('make') is None:
+        pytest.skip('no make here')
+    out = subprocess.run(['make', '-n', '-W', 'Makefile', '-C', csrc], capture_output=True, text=True, check=True).stdout
+    for f in glob.glob(os.path.join(csrc, '*.hip')):
+        assert '-c %s ' % os.path.basename(f) in out, f
