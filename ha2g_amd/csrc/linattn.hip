@@ -150,8 +150,9 @@ template <> struct Mma<b16> {
 template <typename T> __device__ __forceinline__ float probe(u32x4_t r, float z) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        if constexpr (sizeof(T) == 4) z = __builtin_fmaf(__uint_as_float(r[j]), 0.f, z);
-        else z = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, r[j]), __builtin_bit_cast(bf16x2_t, 0u), z, false);
+        const unsigned w = r[j];                                     // a value: a cast of the vector's element takes its first one
+        if constexpr (sizeof(T) == 4) z = __builtin_fmaf(__uint_as_float(w), 0.f, z);
+        else z = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, w), __builtin_bit_cast(bf16x2_t, 0u), z, false);
     }
     return z;
 }

@@ -477,3 +477,23 @@ def test_values_that_are_not_finite_reach_no_earlier_token(T, j, bad, D, dt):
             assert torch.isfinite(x).all(), (i, j)
             assert x.numel() == 0 or float((x - y).norm()) <= 2.0 ** (-20 if dt == torch.float32 else -8) * float(y.norm()) + 1e-30
         assert not torch.isfinite(o[:, j:j + 1].detach() if i < 3 else grads[1][:, j:j + 1]).all()
+
+
+@pytest.mark.parametrize('dt', (torch.float32, torch.bfloat16), ids=('fp32', 'bf16'))
+@pytest.mark.parametrize('T,j', ((40, 33), (150, 70)))
+@pytest.mark.parametrize('Dk,Dv', ((16, 27), (9, 3), (40, 61), (72, 100), (128, 128)))
+def test_a_value_that_is_not_finite_stays_in_its_column(Dk, Dv, T, j, dt):
+    """row b of the batch holds one in column b of v: that column is NaN from its token on and in the state, everything else has the bits it has without"""
+    q, k, v, g, state, _, _ = make(Dv, T, 1, 1, 1, 1, Dk, Dv, dt, seed=T + Dv)
+    want, last = ops.linear_attention(q, k, v, g, state=state, return_state=True)
+    for bad in (float('nan'), float('-inf')):
+        w = v.clone()
+        b = torch.arange(Dv, device=DEV)
+        w[b, j, 0, b] = bad
+        o, s = ops.linear_attention(q, k, w, g, state=state, return_state=True)
+        hit = torch.zeros(Dv, T, 1, Dv, dtype=torch.bool, device=DEV)
+        hit[b, j:, 0, b] = True
+        assert torch.equal(torch.isfinite(o), ~hit) and torch.equal(o[~hit], want[~hit])
+        gone = torch.zeros(Dv, 1, Dk, Dv, dtype=torch.bool, device=DEV)
+        gone[b, 0, :, b] = True
+        assert torch.equal(torch.isfinite(s), ~gone) and torch.equal(s[~gone], last[~gone])
