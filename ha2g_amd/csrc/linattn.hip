@@ -733,6 +733,7 @@ int tile_of(int d) { return d <= 32 ? 32 : (d <= 64 ? 64 : 128); }
 constexpr long STRIDE_LIMIT = 1L << 22;      // of a token, in elements: a workgroup's rows lie within 32 bits of each other
 // one token has no next one: its stride may be anything
 int check_strides(const char* what, const long* strides, int n, int T) {
+    HA2G_REQUIRE(strides, "%s: null strides", what);
     for (int i = 1; T > 1 && i < 3 * n; i += 3)
         HA2G_REQUIRE(strides[i] >= 0 && strides[i] < STRIDE_LIMIT, "%s: a token stride of %ld elements (0 to %ld)", what, strides[i], STRIDE_LIMIT - 1);
     return 0;
@@ -839,6 +840,7 @@ int ha2g_linattn_step(const void* q, const void* k, const void* v, void* o, cons
     LinAttnArgs a;
     if (const int rc = check_args(a, "linattn_step", log_decay, nullptr, B, 1, H, rq, rk, rv, Dk, Dv, b16_io, q && k && v && o && state)) return rc;
     if (B == 0) return 0;
+    if (const int rc = check_strides("linattn_step", strides, 4, 1)) return rc;
     Job& j = a.job[0];
     j.q = operand(q, strides, rq, 1); j.k = operand(k, strides + 3, rk, 1); j.v = operand(v, strides + 6, rv, 1);
     j.Dk = Dk; j.Dv = Dv; j.oscale = scale;
@@ -859,6 +861,7 @@ int ha2g_linattn_step(const void* q, const void* k, const void* v, void* o, cons
 int ha2g_head_sum(const float* x, void* out, long rows, int heads, int n, int D, int b16_out, void* stream) {
     HA2G_REQUIRE(rows >= 0 && heads >= 1 && n >= 1 && D >= 1, "head_sum: rows=%ld heads=%d n=%d D=%d", rows, heads, n, D);
     if (rows == 0) return 0;
+    HA2G_REQUIRE(x && out, "head_sum: null operand");
     const bool wide = D % 4 == 0 && (uintptr_t)x % 16 == 0 && (uintptr_t)out % (b16_out ? 8 : 16) == 0;
     const long want = (rows * heads * (wide ? D / 4 : D) + 255) / 256;
     const dim3 grid((unsigned)(want > 16384 ? 16384 : want)), block(256);

@@ -930,8 +930,8 @@ __global__ __launch_bounds__(1024) void slab_sum_kernel(const float* __restrict_
 
 // The forward pass: threads per row and chunks per thread.  A wave alone up to 128 chunks, then one chunk per thread as far as 256 threads go, then two; the
 // widest rows take what the registers of 1 024 threads hold.  Ragged chunks cost more registers: one per thread up to 512 threads (2^25 values,
-// fp32, before its sigmoid, which adds up to 7 %: 300 per row 199 us, 242 with two per thread; 1 500 145 us, 195; but 2 700 224 us with one in 1 024 threads, 219 with two in 512).  Groups
-// of one or two values (VEC = 1) are taken one by one.
+// fp32, before its sigmoid, which adds up to 7 %: 300 per row 199 us, 242 with two per thread; 1 500 145 us, 195; but 2 700 224 us with one in 1 024
+// threads, 219 with two in 512).  Groups of one or two values (VEC = 1) are taken one by one.
 #define TAIL_SHAPES(VEC, RAG, CASE)                                                                                                                \
     {                                                                                                                                              \
         const int nch = (a.C + VEC - 1) / VEC;                                                                                                     \

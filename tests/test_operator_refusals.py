@@ -159,3 +159,18 @@ def test_gradients_of_a_pass_without_a_backward_of_its_own_refuse_a_second_deriv
     y = torch.tensor(1.0, requires_grad=True)
     g, = torch.autograd.grad(_Cube.apply(x.detach(), y), y, create_graph=True)
     assert g == 1 and not g.requires_grad
+
+
+def test_c_entries_refuse_null_strides_and_operands():
+    """in words of their own, before anything is launched (any address that is not null stands for an operand: none is read)"""
+    from ha2g_amd._lib import lib
+    at = 4096
+
+    def refused(rc):
+        assert rc != 0
+        e = lib.ha2g_last_error()
+        return b'null' in e if isinstance(e, bytes) else 'null' in str(e)
+    assert refused(lib.ha2g_linattn_fwd(at, at, at, at, at, None, None, None, None, 1, 1, 1, 1, 1, 1, 8, 8, 1.0, 0, None, None))
+    assert refused(lib.ha2g_linattn_bwd(at, at, at, at, at, at, at, at, None, None, None, None, None, 1, 1, 1, 1, 1, 1, 8, 8, 1.0, 0, 0, 0, 0, None, None, None))
+    assert refused(lib.ha2g_linattn_step(at, at, at, at, at, at, None, 1, 1, 1, 1, 1, 8, 8, 1.0, 0, None))
+    assert refused(lib.ha2g_head_sum(None, at, 1, 1, 2, 4, 0, None)) and refused(lib.ha2g_head_sum(at, None, 1, 1, 2, 4, 0, None))
