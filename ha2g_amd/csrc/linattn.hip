@@ -539,6 +539,7 @@ __global__ __launch_bounds__(waves_of(DKP, DVP) * 64, occupancy_of(DKP, DVP)) vo
                 asm volatile("" : "+v"(me));
                 const int j = v0 + me % DVW;
                 __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");      // behind the outputs that other lanes stored there
+                __builtin_amdgcn_s_waitcnt(0);
                 for (int r = first[j]; r < L && j < Dv; ++r) {
                     char* const p = (char*)J.o + (obase + (t0 + dir * (c0 + r)) * J.ot + j) * osize;
                     if (J.o16) st1((b16*)p, 0, __builtin_nanf("")); else st1((float*)p, 0, __builtin_nanf(""));
@@ -606,8 +607,8 @@ __global__ __launch_bounds__(256) void linattn_segment_scan_kernel(const LinAttn
 }
 
 // One token: a block per (batch row, head), bound by the state's one read and one write.  The decay is that of the chunked form: a factor rounded to
-// fp32 would let a long stream drift from the same prompt (5e-4 after 16 384 tokens at 1 - 2^-12).  Thread = (row group, V neighbouring columns), eight rows in
-// flight each; the partial sums over the row groups meet in LDS.  256 rows of 16 heads, 128 x 128: 105 us = 5.1 TB/s (a large copy: 4.9); one row
+// fp32 would let a long stream drift from the same prompt (5e-4 after 16 384 tokens at 1 - 2^-12).  Thread = (row group, V neighbouring columns), eight
+// rows in flight each; the partial sums over the row groups meet in LDS.  256 rows of 16 heads, 128 x 128: 105 us = 5.1 TB/s (a large copy: 4.9); one row
 // of 5 heads, 60 x 60: 3.9 us, the launch.
 template <typename T, int V>
 __global__ __launch_bounds__(256) void linattn_step_kernel(const LinAttnArgs a, int lpr /* threads per row, a power of two with lpr * V >= Dv */) {

@@ -1933,7 +1933,7 @@ def _on(t):
 
 def _no_tangents(what, tensors):
     """a forward-mode tangent would be dropped: a dual tensor does not require grad, and its address is that of its values (no level: one comparison)"""
-    if forward_ad._current_level >= 0:
+    if getattr(forward_ad, '_current_level', 0) >= 0:
         _need(all(t is None or forward_ad.unpack_dual(t).tangent is None for t in tensors), '%s: no forward-mode derivative', what)
 
 
@@ -2088,7 +2088,7 @@ def linear_attention(q, k, v, log_decay, scale=None, state=None, lengths=None, r
     tokens (clipped to 0 .. T); what lies behind is not read, the output and the gradients there are zero.
     bf16 operands: products and states are those of the values given (states fp32-exact), but where a state or a score enters an output's or a
     gradient's product it is held to 16 bits, 2^-17 of each term; an output that cancels to less than 2^-8 of its terms is less exact than its type.
-    A value that is not finite reaches its own token and those behind it (gradients: in front of it), as NaN, and nothing else.
+    A value that is not finite reaches its own token and those behind it (gradients: in front of it), from v as NaN, and nothing else.
     Returns o [B, T, H, Dv] in v's type, with return_state also the state behind each row's last token, fp32."""
     _, Dk, _ = _la_check('linear_attention', q, k, v, log_decay, state, 4)
     if lengths is not None:

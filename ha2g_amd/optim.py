@@ -149,7 +149,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9, 
     laid out like the parameters.  In 8 bits:
     pairs (codes, scales) as adamw_state8 makes them, exp_avg_sqs holding the ROOT of the second moment; `seed` (32 bits) varies the rounding's dither.
     A root above zero is held as at least the smallest code of its block (some 2^-18 of the largest root): it divides the next update.
-    No two of the written tensors share memory (one listed twice is refused).  guard: optional int32 device word; while it is not zero the step changes nothing.  Everything lies on one device."""
+    No two of the written tensors share memory (one listed twice is refused).  guard: optional int32 device word; while it is not zero the step changes
+    nothing.  Everything lies on one device."""
     n = len(params)
     _need(n == len(grads) == len(exp_avgs) == len(exp_avg_sqs), 'adamw_step: %d parameters, %d gradients, %d and %d states', n, len(grads), len(exp_avgs),
           len(exp_avg_sqs))

@@ -574,10 +574,10 @@ int ha2g_logmel_f32(const float* y, int B, long n_samples, int pad_reflect, cons
 
 /* ---- linear attention with one decay per head (no reference counterpart; stands beside the GRU recurrence of model/hierarchy_net.py:87-88,144) ----
  *   S_t = e^{log_decay} S_{t-1} + k_t v_t^T,  o_t = scale q_t S_t     per batch row and head, S fp32 [Dk][Dv], 1 <= Dk, Dv <= 128
- * q, k, v, o: fp32, or (b16_io) bf16; strides = HOST array {batch, token, head} x {q, k, v, o} in elements, inner stride 1, token strides below 2^22 (not read for T = 1).
- * Head h of H reads head
- * h / rq of q, h / rk of k, h / rv of v.  s_in / s_out [B][H][Dk][Dv]: states in front of the first and behind the last token (NULL = zero, = not
- * wanted).  lengths [B] (device int32, NULL = T): tokens at and behind a row's length are not read, o is zero there.
+ * q, k, v, o: fp32, or (b16_io) bf16; strides = HOST array {batch, token, head} x {q, k, v, o} in elements, inner stride 1, token strides below 2^22
+ * (not read for T = 1).  Head h of H reads head h / rq of q, h / rk of k, h / rv of v.  s_in / s_out [B][H][Dk][Dv]: states in front of the first and
+ * behind the last token (NULL = zero, = not wanted).  lengths [B] (device int32, NULL = T): tokens at and behind a row's length are not read, o is zero
+ * there.
  * b16_io: a state or a score enters an output's product with 16 bits (2^-17 of each term); states themselves are fp32-exact.
  * ws: ha2g_linattn_workspace_floats() floats (0: may be NULL), the states between the segments of a time axis that is split over the chip. */
 long ha2g_linattn_workspace_floats(int B, int T, int H, int Dk, int Dv, int b16_io);
@@ -615,8 +615,8 @@ int ha2g_block_tail_bwd(const void* y, const void* res, const void* gate, const 
 /* ---- AdamW over many tensors in one launch (torch.optim.AdamW semantics; the reference sets up Adam, train.py:155-170) ----
  * p, g, m, v, sm, sr: HOST arrays of n device pointers; len: HOST array of n lengths.  p fp32 or (p_b16) bf16, g likewise.  bits = 32: m, v fp32.
  * bits = 8: m, v = e4m3 codes of m and of sqrt(v), sm / sr = fp32 scales (powers of two), one per 128 consecutive elements of a tensor; the rounding
- * to codes is dithered by a hash of (seed, step, first + tensor, place); a root above zero is never rounded to zero.  ha2g_adamw_scalars advances `step` (device int32; guard as in
- * ha2g_adam_guarded_f32) and leaves what the step's number gives in `scalars` (3 words of device memory) for the calls of the step. */
+ * to codes is dithered by a hash of (seed, step, first + tensor, place); a root above zero is never rounded to zero.  ha2g_adamw_scalars advances
+ * `step` (device int32; guard as in ha2g_adam_guarded_f32) and leaves what the step's number gives in `scalars` (3 words of device memory) for the calls of the step. */
 int ha2g_adamw_scalars(int* step, const int* guard, double lr, double b1, double b2, float* scalars, void* stream);
 int ha2g_adamw_multi(int n, const long* p, const long* g, const long* m, const long* v, const long* sm, const long* sr, const long* len, int p_b16,
                      int g_b16, int bits, double lr, double b1, double b2, double eps, double wd, unsigned seed, int first, const float* scalars,
