@@ -6,6 +6,8 @@
 // token undecayed, and what is left in front of the first token is the gradient of the first state.
 #include "common.h"
 
+#include <climits>
+
 namespace {
 
 struct Operand { const void* p; long b, t, h; int r; };      // element strides of batch row, token, head; head h reads head h / r
@@ -222,15 +224,15 @@ template <typename T, int D, int C, int NT, bool WHOLE> struct Stage {
         }
         base += chunk;
     }
-    // Zeros in place of what is not finite; first[c] <- the first row of the chunk in which column c was that (in LDS, the chunk's length before)
-    __device__ __forceinline__ void keep_finite(int* first) {
+    // Zeros in place of what is not finite; first[c] (in LDS) <- the first row in which column c was that, the chunk's rows counted from `at`
+    __device__ __forceinline__ void keep_finite(int* first, int at) {
         float z = 0.f;
 #pragma unroll
         for (int j = 0; j < N; ++j) z = probe<T>(r[j], z);
         if (__builtin_expect(__builtin_amdgcn_ballot_w64(z != z) == 0, 1)) return;
         int me = threadIdx.x;                                        // hidden from the compiler, which would keep this rare path's addresses over all chunks
         asm volatile("" : "+v"(me));
-        const int c0 = me % V * E + (!WHOLE && shift > 0 && left < E ? left - E : 0), row0 = me / V;
+        const int c0 = me % V * E + (!WHOLE && shift > 0 && left < E ? left - E : 0), row0 = at + me / V;
 #pragma unroll
         for (int j = 0; j < N; ++j)
 #pragma unroll
@@ -307,9 +309,9 @@ __global__ __launch_bounds__(waves_of(DKP, DVP) * 64, occupancy_of(DKP, DVP)) vo
     __shared__ __attribute__((aligned(16))) T ks[C * SK::LD];
     __shared__ __attribute__((aligned(16))) T vs[C * SV::LD];
     __shared__ __attribute__((aligned(16))) typename M::Tile ps[STATE_ONLY ? 1 : TILES * M::NS * 64];
-    __shared__ int first[STATE_ONLY ? 1 : DVP];                  // a column's first token of the chunk that is not finite; C: none
+    __shared__ int first[STATE_ONLY ? 1 : DVP];                  // a column's first token that is not finite
     const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4, wave = threadIdx.x >> 6, v0 = wave * DVW;
-    if (!STATE_ONLY && lane < DVW) first[v0 + lane] = C;
+    if (!STATE_ONLY && lane < DVW) first[v0 + lane] = INT_MAX;
     const long wg = xcd_order(blockIdx.x, gridDim.x);
     const int h = (int)(wg % a.H), seg = (int)(wg / a.H % a.nseg), b = (int)(wg / a.H / a.nseg);
     const long bh = (long)b * a.H + h, D2 = (long)J.Dk * J.Dv;
@@ -395,9 +397,10 @@ __global__ __launch_bounds__(waves_of(DKP, DVP) * 64, occupancy_of(DKP, DVP)) vo
         __syncthreads();
         if constexpr (!STATE_ONLY) rq.store(qs);
         rk.store(ks);
-        // A score of 0 does not keep NaN or infinity in v from the tokens in front of it.  The products take 0 for them, and behind the products what a
-        // column's first one reaches is made NaN: the outputs from its token on, and the state.  (The checks cost 1 to 2 %.)
-        if constexpr (!STATE_ONLY) rv.keep_finite(first);
+        // A score of 0 does not keep NaN or infinity in v from the tokens in front of it.  The products take 0 for them, and behind the last chunk what a
+        // column's first one reaches is made NaN.  (1 % of a call; looking at the state at a segment's end and doing it again where one is there 2 to 3 %, a
+        // second pass costs the first its registers.)
+        if constexpr (!STATE_ONLY) rv.keep_finite(first, c0);
         rv.store(vs);
         __syncthreads();
         const int L = min(C, end - c0), c1 = c0 + C;
@@ -411,13 +414,6 @@ __global__ __launch_bounds__(waves_of(DKP, DVP) * 64, occupancy_of(DKP, DVP)) vo
         for (int u = 0; u < CF; ++u)
 #pragma unroll
             for (int y = 0; y < VT; ++y) vf[u][y] = M::col(vs, SV::LD, v0 + 16 * y, u, lane);
-        bool finite = true;                                        // this wave's columns
-        if constexpr (!STATE_ONLY) {
-            int n = C;
-#pragma unroll
-            for (int y = 0; y < VT; ++y) n = min(n, first[v0 + 16 * y + col]);
-            finite = __builtin_amdgcn_ballot_w64(n < C) == 0;
-        }
         if constexpr (!STATE_ONLY) {
             // this wave's score tiles, for all
 #pragma unroll
@@ -533,28 +529,28 @@ __global__ __launch_bounds__(waves_of(DKP, DVP) * 64, occupancy_of(DKP, DVP)) vo
 #pragma unroll
                 for (int y = 0; y < VT; ++y) S[x][y] = M::mma(kf, wf[y][p], S[x][y]);
         });
-        if constexpr (!STATE_ONLY)
-            if (__builtin_expect(!finite, 0)) {
-                int me = lane;                                       // hidden likewise
-                asm volatile("" : "+v"(me));
-                const int j = v0 + me % DVW;
-                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");      // behind the outputs that other lanes stored there
-                __builtin_amdgcn_s_waitcnt(0);
-                for (int r = first[j]; r < L && j < Dv; ++r) {
-                    char* const p = (char*)J.o + (obase + (t0 + dir * (c0 + r)) * J.ot + j) * osize;
+    }
+    if constexpr (!STATE_ONLY) {
+        // from a column's first value on that is not finite: the outputs, behind those that other lanes stored there, and the state
+        const int f = lane < DVW ? first[v0 + lane] : INT_MAX;
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(f != INT_MAX) != 0, 0)) {
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+            __builtin_amdgcn_s_waitcnt(0);
+            const int j = v0 + lane % DVW, from = first[j];
+            if (from != INT_MAX && j < Dv)
+                for (int c = from + lane / DVW; c < end; c += 64 / DVW) {
+                    char* const p = (char*)J.o + (obase + (t0 + dir * c) * J.ot + j) * osize;
                     if (J.o16) st1((b16*)p, 0, __builtin_nanf("")); else st1((float*)p, 0, __builtin_nanf(""));
                 }
-                if (first[j] < C) first[j] = 0;                      // and of all chunks to come
-            }
+#pragma unroll
+            for (int y = 0; y < VT; ++y)
+                if (first[j_lane + 16 * y] != INT_MAX)
+#pragma unroll
+                    for (int x = 0; x < KT; ++x)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) S[x][y][i] = __builtin_nanf("");
+        }
     }
-    if constexpr (!STATE_ONLY)
-#pragma unroll
-        for (int y = 0; y < VT; ++y)
-            if (first[j_lane + 16 * y] < C)
-#pragma unroll
-                for (int x = 0; x < KT; ++x)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) S[x][y][i] = __builtin_nanf("");
     float* s_out;
     int oi = J.si, oj = J.sj;
     if constexpr (STATE_ONLY) {
