@@ -48,8 +48,8 @@ template <> __device__ __forceinline__ void st1<b16>(b16* p, long i, float v) {
 // product's operands, for all.  Rows of LDS are padded by 32 bytes: 16-byte reads of 16 rows and transpose reads of 4 x 16 blocks meet every bank
 // once (row reads of 2 x 8 bytes had two thirds of the LDS time in conflicts).
 //     o^T = S^T q^T + v^T (k q^T):  a lane ends with 4 consecutive columns of one token.
-// Measured: 512 (row, head) pairs of 1 024 tokens, bf16: Dk = Dv = 64 62 us (q, k, v and o at 4.3 TB/s; a large copy 4.9), 128 134 us (4.0 TB/s);
-// fp32: 123 us (4.4 TB/s) and 365 us (2.9).  Bound by memory at 64, at 128 by the issue of two waves per SIMD: per chunk and wave ~500 vector
+// Measured: 512 (row, head) pairs of 1 024 tokens, bf16: Dk = Dv = 64 62 us (q, k, v and o at 4.3 TB/s; a large copy 4.9), 128 131 us (4.1 TB/s);
+// fp32: 125 us (4.3 TB/s) and 365 us (2.9).  Bound by memory at 64, at 128 by the issue of two waves per SIMD: per chunk and wave ~500 vector
 // instructions (200 of them split S, 64 decay it) beside 91 matrix instructions, matrix units 30 % busy.
 // fp32 operands run on the fp32 MFMA.  bf16 operands are exact as they are; what is computed is split into bf16 pieces: S and the scores, which
 // only reach the bf16 result, into two (2^-17 of a term, 2^-8 of the result's own rounding; a third piece costs 10 to 22 %: 512 pairs, 128 x 128,
@@ -285,7 +285,7 @@ __device__ __forceinline__ long xcd_order(long i, long n) { return n % 8 == 0 ? 
 
 // Waves of a workgroup: 16 columns of v each, 32 where Dk and v are both long (or Dk is too short for eight waves to share its rows).  Dk = 64 with
 // 128 columns fits 128 registers, so that two workgroups of eight waves run on a compute unit (three rows of up to 5 003 tokens, 12 heads, bf16, the
-// call: 71 us, 72.5 with four waves; fp32, 16 heads of 8 192 tokens 98, 100; bf16 with 512 pairs of 1 024 tokens is better off with four, 121 us, 106);
+// call: 70.5 us, 72.5 with four waves; fp32, 16 heads of 8 192 tokens 99.5, 101; bf16 with 512 pairs of 1 024 tokens is better off with four, 110, 105);
 // Dk = 128 does not, and eight waves of one workgroup in step with each other are slower than two workgroups of four (512 pairs of 1 024 tokens, before
 // the check for NaN: 141 us, 132).  With three waves per SIMD (168 registers, some of them spilled) Dk = Dv = 128 takes 217 us.
 constexpr int waves_of(int DKP, int DVP) { return DVP < 64 ? DVP / 16 : (DKP == 64 && DVP == 128 ? 8 : 4); }
